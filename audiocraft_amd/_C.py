@@ -54,6 +54,7 @@ if not os.path.exists(LIB_PATH):
 lib = C.CDLL(LIB_PATH)
 
 vp, i32, f32, u64, i64p = C.c_void_p, C.c_int, C.c_float, C.c_uint64, C.c_void_p
+i64 = C.c_longlong
 
 
 class ConvDesc(C.Structure):
@@ -148,6 +149,37 @@ class FfnEngineDesc(C.Structure):
                 ('err', vp), ('M', i32), ('d', i32), ('ffn', i32), ('eps', f32), ('acq_mode', i32), ('waves', i32), ('dma_chunk', i32), ('dma_epi', i32), ('poll_sleep', i32), ('trace', vp)]
 
 
+class KV8CacheDesc(C.Structure):
+    _fields_ = [('k_codes', vp), ('v_codes', vp), ('k_scale', vp), ('v_scale', vp), ('k_tail', vp), ('v_tail', vp),
+                ('tail_dtype', i32), ('rows', i32), ('H', i32), ('hd', i32), ('nblk', i32)]
+
+
+class KV8StoreDesc(C.Structure):
+    _fields_ = [('k', vp), ('v', vp), ('dtype', i32), ('k_row', i64), ('k_tok', i64), ('k_head', i64), ('v_row', i64),
+                ('v_tok', i64), ('v_head', i64), ('L', i32), ('start', vp), ('n', vp)]
+
+
+class KV8AttnDesc(C.Structure):
+    _fields_ = [('q', vp), ('q_dtype', i32), ('q_row', i64), ('q_tok', i64), ('q_head', i64), ('S', i32), ('Hq', i32),
+                ('len', vp), ('len_stride', i32), ('len_bias', i32), ('q_len', vp), ('start_rows', vp), ('causal', i32),
+                ('past_context', i32), ('k_new', vp), ('v_new', vp), ('new_dtype', i32), ('kn_row', i64), ('kn_head', i64),
+                ('vn_row', i64), ('vn_head', i64), ('complete', i32), ('out', vp), ('out_mode', i32), ('out_dtype', i32),
+                ('out_rbs', i32), ('out_col0', i32), ('work', vp)]
+
+
+class LinearI8Desc(C.Structure):
+    _fields_ = [('a', vp), ('a_scale', vp), ('w', vp), ('w_scale', vp), ('bias', vp), ('residual', vp), ('out', vp),
+                ('out_dtype', i32), ('ldo', i64), ('act', i32), ('M', i32), ('N', i32), ('K', i32)]
+
+
+KV8_BLOCK = 64
+_kv8_store = _sig('acmi_kv8_store', [C.POINTER(KV8CacheDesc), C.POINTER(KV8StoreDesc), vp])
+_kv8_load = _sig('acmi_kv8_load', [C.POINTER(KV8CacheDesc), vp, i32, vp, vp, i32, vp])
+_kv8_attn_work = _sig('acmi_kv8_attn_work_floats', [C.POINTER(KV8CacheDesc), i32, i32], C.c_size_t)
+_kv8_attn = _sig('acmi_kv8_attn', [C.POINTER(KV8CacheDesc), C.POINTER(KV8AttnDesc), vp])
+_quantize_rows_i8 = _sig('acmi_quantize_rows_i8', [vp, i32, i64, i32, i32, vp, vp, vp])
+_linear_i8 = _sig('acmi_linear_i8', [C.POINTER(LinearI8Desc), vp])
+
 _linear_ex = _sig('acmi_linear_ex', [C.POINTER(LinearDesc), vp])
 FFN_ENGINE_FLAG_BYTES = 16384
 _ffn_engine = _sig('acmi_ffn_engine', [C.POINTER(FfnEngineDesc), vp])
@@ -182,14 +214,16 @@ EXPORTS = ['acmi_group_norm_work_floats', 'acmi_group_norm', 'acmi_channel_add',
            'acmi_fir_bank', 'acmi_band_stats', 'acmi_band_mix', 'acmi_linear_big', 'acmi_attn_prefill', 'acmi_resample_frac', 'acmi_chroma', 'acmi_chroma_frames', 'acmi_version', 'acmi_last_error', 'acmi_rvq_codebook_norms', 'acmi_rvq_encode', 'acmi_rvq_decode',
            'acmi_conv1d', 'acmi_conv1d_gn', 'acmi_conv1d_tile_weights', 'acmi_conv1d_weight_floats', 'acmi_conv1d_work_floats', 'acmi_lstm_layer', 'acmi_lstm_work_floats', 'acmi_lstm_layer_ex', 'acmi_lstm_layer_work_floats', 'acmi_lstm_stack2', 'acmi_lstm_stack2_work_floats', 'acmi_lstm_stack2_supported', 'acmi_lm_step', 'acmi_linear',
            'acmi_attn_decode', 'acmi_kv_store', 'acmi_sample', 'acmi_pos_table', 'acmi_ln_tile', 'acmi_linear_ex', 'acmi_ln_tile_reduce', 'acmi_linear_pair', 'acmi_attn_decode_ex', 'acmi_layer_norm_rows',
-           'acmi_ffn_engine', 'acmi_ffn_engine_supported', 'acmi_cross_fold', 'acmi_qkv_attn_launches']
+           'acmi_ffn_engine', 'acmi_ffn_engine_supported', 'acmi_cross_fold', 'acmi_qkv_attn_launches',
+           'acmi_kv8_store', 'acmi_kv8_load', 'acmi_kv8_attn_work_floats', 'acmi_kv8_attn', 'acmi_quantize_rows_i8', 'acmi_linear_i8']
 
 
 # ctypes mirror -> C type of include/acmi.h (tests/test_host_cpu.py compiles the header with gcc and compares every
 # field's offset: a mirror that drifts from the header would corrupt every call silently)
 STRUCT_MIRRORS = {'acmi_conv_desc': ConvDesc, 'acmi_lm_layer': LMLayer, 'acmi_lm_model': LMModelDesc, 'acmi_lm_state': LMState,
                   'acmi_linear_desc': LinearDesc, 'acmi_attn_desc': AttnDesc, 'acmi_ffn_engine_desc': FfnEngineDesc,
-                  'acmi_cross_fold_desc': CrossFoldDesc}
+                  'acmi_cross_fold_desc': CrossFoldDesc, 'acmi_kv8_cache': KV8CacheDesc, 'acmi_kv8_store_desc': KV8StoreDesc,
+                  'acmi_kv8_attn_desc': KV8AttnDesc, 'acmi_linear_i8_desc': LinearI8Desc}
 
 
 def version() -> int:
@@ -622,6 +656,67 @@ def attn_prefill(q, k_cache, vt, out, npos, npos_pad, pos, past_context=0, out_r
     check(_attn_prefill(ptr(q), ptr(k_cache), ptr(vt), dtype_code(k_cache.dtype), ptr(out), dtype_code(out.dtype), out_rbs,
                         rows, H, hd, Tcap, vt.shape[3], npos, npos_pad, ptr(pos), int(past_context), stream()),
           'acmi_attn_prefill')
+    return out
+
+
+# ---------------------------------------------------------------------------------- 8-bit cache and projection
+# (the callers, modules/kv8_cache.py and modules/int8_linear.py, check shapes, types and devices)
+
+def on_device(t: torch.Tensor):
+    """The device guard of a call on `t`: kernels are launched on the current device's current stream."""
+    import contextlib
+    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def kv8_store(cache: KV8CacheDesc, k, v, start, n):
+    """k / v [rows, L, H, hd] (any strides over the first three), start / n int32 [rows] (n None: L)."""
+    d = KV8StoreDesc(k.data_ptr(), v.data_ptr(), dtype_code(k.dtype), k.stride(0), k.stride(1), k.stride(2), v.stride(0),
+                     v.stride(1), v.stride(2), k.shape[1], start.data_ptr(), None if n is None else n.data_ptr())
+    with on_device(k):
+        check(_kv8_store(C.byref(cache), C.byref(d), stream()), 'acmi_kv8_store')
+
+
+def kv8_load(cache: KV8CacheDesc, lens, T, k_out, v_out):
+    with on_device(k_out):
+        check(_kv8_load(C.byref(cache), lens.data_ptr(), T, k_out.data_ptr(), v_out.data_ptr(), dtype_code(k_out.dtype), stream()),
+              'acmi_kv8_load')
+
+
+def kv8_attn(cache: KV8CacheDesc, q, out, lens, len_bias=0, causal=True, past_context=0, q_lens=None, starts=None, k_new=None,
+             v_new=None):
+    """q [rows, S, Hq, hd] (any strides over the first three) -> out [rows, S, Hq, hd] dense; k_new / v_new [rows, H, hd]."""
+    S, Hq = q.shape[1], q.shape[2]
+    new = (None, None, 0, 0, 0, 0, 0) if k_new is None else (
+        k_new.data_ptr(), v_new.data_ptr(), dtype_code(k_new.dtype), k_new.stride(0), k_new.stride(1), v_new.stride(0), v_new.stride(1))
+    with on_device(q):
+        nw = _kv8_attn_work(C.byref(cache), S, Hq)
+        work = torch.empty(nw, device=q.device, dtype=torch.float32) if nw else None
+        d = KV8AttnDesc(q.data_ptr(), dtype_code(q.dtype), q.stride(0), q.stride(1), q.stride(2), S, Hq, lens.data_ptr(), 1, len_bias,
+                        None if q_lens is None else q_lens.data_ptr(), None if starts is None else starts.data_ptr(), int(causal),
+                        past_context, *new, 0, out.data_ptr(), OUT_BF16 if out.dtype == torch.bfloat16 else OUT_F32,
+                        dtype_code(out.dtype), 0, 0, None if work is None else work.data_ptr())
+        check(_kv8_attn(C.byref(cache), C.byref(d), stream()), 'acmi_kv8_attn')
+    return out
+
+
+def quantize_rows_i8(x: torch.Tensor):
+    """x [R, K] (rows contiguous, any pitch) -> (int8 fragments, scales [R] f32), include/acmi.h."""
+    R, K = x.shape
+    codes = torch.empty(-(-R // 16) * -(-K // 64) * 1024, device=x.device, dtype=torch.int8)
+    scale = torch.empty(R, device=x.device, dtype=torch.float32)
+    with on_device(x):
+        check(_quantize_rows_i8(x.data_ptr(), dtype_code(x.dtype), x.stride(0) if R > 1 else K, R, K, codes.data_ptr(), scale.data_ptr(),
+                                stream()), 'acmi_quantize_rows_i8')
+    return codes, scale
+
+
+def linear_i8(a, a_scale, w, w_scale, out, K, bias=None, residual=None, act=0):
+    """out [M, N] = act(a_scale w_scale (a . w) + bias) + residual on int8 fragments (acmi_linear_i8)."""
+    M, N = out.shape
+    d = LinearI8Desc(a.data_ptr(), a_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(), None if bias is None else bias.data_ptr(),
+                     None if residual is None else residual.data_ptr(), out.data_ptr(), dtype_code(out.dtype), N, act, M, N, K)
+    with on_device(out):
+        check(_linear_i8(C.byref(d), stream()), 'acmi_linear_i8')
     return out
 
 

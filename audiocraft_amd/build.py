@@ -12,9 +12,9 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, 'csrc')
-SOURCES = ['acmi_core.hip', 'acmi_gemm.hip', 'acmi_gemm_f32.hip', 'acmi_engine.hip', 'acmi_attn.hip', 'acmi_crossfold.hip', 'acmi_lm.hip', 'acmi_prefill.hip', 'acmi_rvq.hip', 'acmi_conv.hip', 'acmi_chroma.hip', 'acmi_audio.hip', 'acmi_diffusion.hip']
+SOURCES = ['acmi_core.hip', 'acmi_gemm.hip', 'acmi_gemm_f32.hip', 'acmi_engine.hip', 'acmi_attn.hip', 'acmi_crossfold.hip', 'acmi_lm.hip', 'acmi_prefill.hip', 'acmi_kv8.hip', 'acmi_i8.hip', 'acmi_rvq.hip', 'acmi_conv.hip', 'acmi_chroma.hip', 'acmi_audio.hip', 'acmi_diffusion.hip']
 HEADERS = [os.path.join(ROOT, 'include', 'acmi.h'), os.path.join(CSRC, 'acmi_common.h'),
-           os.path.join(CSRC, 'acmi_lm_internal.h')]
+           os.path.join(CSRC, 'acmi_lm_internal.h'), os.path.join(CSRC, 'acmi_attn_fused.h')]
 OUT = os.path.join(CSRC, 'libacmi.so')
 
 
@@ -25,7 +25,11 @@ def _hipcc() -> str:
     raise RuntimeError("hipcc not found (set HIPCC=...)")
 
 
-FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-Wno-pass-failed', '-ffp-contract=off']
+# -packed-fp32-ops: hipcc -O3 forms v_pk_add / mul / fma_f32 from ordinary float code by itself, and some of their forms have
+# given wrong results now and then on this hardware; scalar f32 instructions instead (the host pass warns that it does not know
+# the feature: harmless)
+FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-Wno-pass-failed', '-ffp-contract=off',
+         '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
 # Kernarg preload (gfx950): the leading scalar / pointer arguments of a kernel arrive in SGPRs at wave start (up to 14
 # dwords) instead of through scalar loads of a kernarg block that is cold on every launch of the decode chain; the
 # kernels of these files are written for it (acmi_gemm.hip: TlHot; acmi_attn.hip: attn_decode_kernel).  Firmware without the feature runs the compiler's

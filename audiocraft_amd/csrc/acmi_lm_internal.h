@@ -103,7 +103,7 @@ int acmi_launch_ln_tile(float* x, void* out, int wdtype, int M, int K, float eps
                         hipStream_t st);
 
 // ---- prefill (acmi_prefill.hip): MFMA-tiled GEMM on tiled operands + causal prefill attention
-enum { ACMI_BIG_F32 = 0, ACMI_BIG_RESID = 1, ACMI_BIG_TILED = 2, ACMI_BIG_QKV = 3 };
+enum { ACMI_BIG_F32 = 0, ACMI_BIG_RESID = 1, ACMI_BIG_TILED = 2, ACMI_BIG_QKV = 3, ACMI_BIG_I8 = 4 };
 
 struct BigArgs {
     const void* a; int a_rbs;   // tiled activation [M / 16][a_rbs][64 lanes][16 B]
@@ -118,8 +118,12 @@ struct BigArgs {
     // row / npos_pad (p = row % npos_pad < npos); V also time-minor into vt [rows, H, hd, vt_tcap]
     float* q_out; void* k_cache; void* v_cache; void* vt;
     int kv_bf16, H, hd, Tcap, d, npos, npos_pad, vt_tcap; const int* pos;
+    // I8 (int8 fragments, acmi_i8.hip): out = act(acc * a_scale[row] * w_scale[col] + bias) + residual, rows < `rows` stored,
+    // out row-major f32 / bf16 with pitch ldo64
+    const float* a_scale; const float* w_scale; const float* residual; long long ldo64; int out_bf16, rows;
 };
 int acmi_launch_big(BigArgs& a, int wdtype, hipStream_t st);
+int acmi_launch_big_i8(BigArgs& a, hipStream_t st);
 
 struct PrefillAttnArgs {
     const float* q;             // [rows * npos_pad, H * hd] f32, position-minor rows

@@ -28,6 +28,12 @@ __device__ __forceinline__ void big_mma(const u32x4& a, const u32x4& b, f32x4& a
     for (int e = 0; e < 4; ++e)
         acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[e]), __uint_as_float(b[e]), acc, 0, 0, 0);
 }
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ void big_mma(const u32x4& a, const u32x4& b, i32x4& acc, int8_t) {   // one fragment = 64 int8 columns
+    acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), acc, 0, 0, 0);
+}
+template <typename WT> struct BigAcc { typedef f32x4 v4; };
+template <> struct BigAcc<int8_t> { typedef i32x4 v4; };
 __device__ __forceinline__ float big_gelu(float x) { return 0.5f * x * (1.0f + erff(x * 0.70710678118654752440f)); }
 // GELU for a bf16 result: erfc(|x| / sqrt 2) by Abramowitz & Stegun 7.1.26 (|error| <= 1.5e-7: one v_rcp_f32, one v_exp_f32
 // and six FMAs against erff's ~45 instructions -- the exact form cost the FFN1 epilogue more than its K loop's MFMAs).
@@ -159,11 +165,12 @@ __global__ __launch_bounds__(BigTile<BIG>::NW * 64, BIG ? 1 : 2) void lin_big_ke
         sb[h] = reinterpret_cast<unsigned long long>(mine_a ? p.a : p.w) + blk * 1024 - (size_t)h * 1024;
     }
     const u32x4* lds = reinterpret_cast<const u32x4*>(smem);
-    f32x4 acc[WI][4];
+    typedef typename BigAcc<WT>::v4 acc4;
+    acc4 acc[WI][4];
 #pragma unroll
     for (int i = 0; i < WI; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int j = 0; j < 4; ++j) acc[i][j] = acc4{0, 0, 0, 0};
 
     const int nst = p.NKC;
     const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) void*)smem;
@@ -206,7 +213,7 @@ __global__ __launch_bounds__(BigTile<BIG>::NW * 64, BIG ? 1 : 2) void lin_big_ke
         // MFMAs are pure register arithmetic to the compiler, which otherwise sinks them past the barriers and the requests
         // (a half's 16 MFMAs were found behind the NEXT barrier): an empty volatile asm that "updates" a row block's four
         // accumulators keeps them where they are written
-        auto pin = [&](f32x4 (&c)[4]) { asm volatile("" : "+v"(c[0]), "+v"(c[1]), "+v"(c[2]), "+v"(c[3])); };
+        auto pin = [&](acc4 (&c)[4]) { asm volatile("" : "+v"(c[0]), "+v"(c[1]), "+v"(c[2]), "+v"(c[3])); };
         auto wait_vm = [&](int young) {   // this wave's requests but the `young` most recent stages have landed
             if (young >= 3) asm volatile("s_waitcnt vmcnt(12)" ::: "memory");
             else if (young == 2) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
@@ -271,6 +278,46 @@ __global__ __launch_bounds__(BigTile<BIG>::NW * 64, BIG ? 1 : 2) void lin_big_ke
     // ---- epilogue: lane (kg, nl) of accumulator (i, j) holds row i * 16 + nl, features j * 16 + kg * 4 + (0..3)
     const int nl = lane & 15, kg = lane >> 4;
     const int row0 = (tm << TS) + wm * (WI * 16) + nl, col0 = (tn << TS) + wn * 64 + kg * 4;
+    if constexpr (EPI == ACMI_BIG_I8) {
+        float sa[WI];
+#pragma unroll
+        for (int i = 0; i < WI; ++i) sa[i] = p.a_scale[min(row0 + i * 16, p.rows - 1)];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int col = col0 + j * 16;
+            if (col >= p.N) continue;
+            float sw[4], bi[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                sw[r] = p.w_scale[min(col + r, p.N - 1)];
+                bi[r] = p.bias != nullptr ? p.bias[min(col + r, p.N - 1)] : 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < WI; ++i) {
+                const int row = row0 + i * 16;
+                if (row >= p.rows) continue;
+                float v[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    v[r] = __builtin_fmaf((float)acc[i][j][r], sa[i] * sw[r], bi[r]);
+                    if (p.act == 1) v[r] = p.out_bf16 ? big_gelu_bf16(v[r]) : big_gelu(v[r]);
+                    if (p.residual != nullptr && col + r < p.N) v[r] += p.residual[(size_t)row * p.N + col + r];
+                }
+                const size_t at = (size_t)(row * p.ldo64) + col;
+                if (p.vec) {
+                    if (p.out_bf16) *reinterpret_cast<uint2*>(reinterpret_cast<bf16_t*>(p.out) + at) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+                    else *reinterpret_cast<f32x4*>(p.out + at) = f32x4{v[0], v[1], v[2], v[3]};
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        if (col + r >= p.N) break;
+                        if (p.out_bf16) reinterpret_cast<bf16_t*>(p.out)[at + r] = f32_to_bf16(v[r]);
+                        else p.out[at + r] = v[r];
+                    }
+                }
+            }
+        }
+    } else {
     // every operand of the epilogue is requested before the first one is used
     int pos0 = 0;
     if (EPI == ACMI_BIG_QKV) pos0 = *p.pos;
@@ -355,6 +402,7 @@ __global__ __launch_bounds__(BigTile<BIG>::NW * 64, BIG ? 1 : 2) void lin_big_ke
             }
         }
     }
+    }
 #ifdef ACMI_BIG_TRACE
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     ACMI_BT(t_end);
@@ -429,6 +477,19 @@ int acmi_launch_big(BigArgs& a, int wdtype, hipStream_t st) {
     ACMI_REQUIRE(a.epi != ACMI_BIG_QKV || (a.d % 16 == 0 && a.hd % 4 == 0 && a.N == 3 * a.d && (reinterpret_cast<size_t>(a.q_out) & 15) == 0),
                  "acmi_linear_big: the QKV epilogue needs d %% 16 == 0, hd %% 4 == 0 and N = 3 d (d=%d hd=%d N=%d)", a.d, a.hd, a.N);
     return wdtype == ACMI_BF16 ? launch_big_t<bf16_t>(a, st) : launch_big_t<float>(a, st);
+}
+
+// int8 fragments (acmi_linear_i8): the same tiles and ring, 64 columns per K step
+int acmi_launch_big_i8(BigArgs& a, hipStream_t st) {
+    a.NKC = (a.K + 63) / 64;
+    a.a_rbs = a.NKC;
+    a.epi = ACMI_BIG_I8;
+    const size_t align = a.out_bf16 ? 7 : 15;
+    a.vec = a.N % 4 == 0 && a.ldo64 % 4 == 0 && (reinterpret_cast<size_t>(a.out) & align) == 0;
+    const int t256 = ((a.M + 255) >> 8) * ((a.N + 255) >> 8), big = t256 >= 128;
+    const int tiles = big_grid(a.M, a.N, big ? 8 : 7);
+    const int rc = big ? launch_big_k<int8_t, ACMI_BIG_I8, 1>(a, tiles, st) : launch_big_k<int8_t, ACMI_BIG_I8, 0>(a, tiles, st);
+    return rc ? rc : acmi_check_launch("lin_big_kernel");
 }
 
 extern "C" int acmi_linear_big(const void* a, int a_rbs, const void* w, int wdtype, const float* bias, void* out, int out_mode,

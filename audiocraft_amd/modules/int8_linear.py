@@ -1,0 +1,62 @@
+"""A linear layer in 8-bit integers: int8 weight with one scale per output channel, activations quantised per token on the fly.
+
+    y[m, n] = act(sa[m] sw[n] sum_k a8[m, k] w8[n, k] + bias[n]) + residual[m, n]
+
+The counterpart of the `nn.Linear` projections of audiocraft/modules/transformer.py:362-399, 454-574 for serving: a quarter of
+the f32 weight's bytes and the int8 rate of the matrix cores.  No gradients.
+"""
+import typing as tp
+
+import torch
+from torch import nn
+
+from .. import _C
+
+_DTYPES = (torch.float32, torch.bfloat16)
+
+
+class Int8Linear:
+    """Built once from a weight [N, K] (nn.Linear layout, f32 or bf16, on the GPU) and an optional bias [N]; the int8 weight is laid
+    out for the matrix cores (include/acmi.h, "int8 fragments").  activation: 'none' or 'gelu' (exact).
+
+    A token (channel) that holds a NaN or an infinity gives NaN in its whole output row (column)."""
+
+    ACTIVATIONS = {'none': 0, 'gelu': 1}
+
+    def __init__(self, weight: torch.Tensor, bias: tp.Optional[torch.Tensor] = None, activation: str = 'none'):
+        if weight.dim() != 2 or weight.dtype not in _DTYPES or not weight.is_cuda or 0 in weight.shape:
+            raise ValueError(f"Int8Linear: weight {tuple(weight.shape)} {weight.dtype} on {weight.device}: [N, K] float32 or bfloat16 on the GPU")
+        if weight.shape[1] > 131072:
+            raise ValueError(f"Int8Linear: K {weight.shape[1]} (at most 131072: the 32-bit integer sums)")
+        if activation not in self.ACTIVATIONS:
+            raise ValueError(f"Int8Linear: activation {activation!r} ({', '.join(self.ACTIVATIONS)})")
+        self.out_features, self.in_features = weight.shape
+        self.activation = activation
+        w = weight.detach()
+        self.codes, self.scale = _C.quantize_rows_i8(w if w.stride(1) == 1 else w.contiguous())
+        self.bias = None
+        if bias is not None:
+            if bias.shape != (self.out_features,) or bias.device != weight.device:
+                raise ValueError(f"Int8Linear: bias {tuple(bias.shape)} on {bias.device}, expected [{self.out_features}] on {weight.device}")
+            self.bias = bias.detach().float().contiguous()
+
+    @classmethod
+    def from_linear(cls, linear: nn.Linear, activation: str = 'none') -> 'Int8Linear':
+        return cls(linear.weight, linear.bias, activation)
+
+    def __call__(self, x: torch.Tensor, residual: tp.Optional[torch.Tensor] = None) -> torch.Tensor:
+        """x [..., K] f32 or bf16 -> [..., N] in x's dtype; residual [..., N] f32 is added last."""
+        if x.shape[-1:] != (self.in_features,) or x.dtype not in _DTYPES or x.device != self.codes.device:
+            raise ValueError(f"Int8Linear: x {tuple(x.shape)} {x.dtype} on {x.device}: [..., {self.in_features}] float32 or bfloat16 on {self.codes.device}")
+        rows = x.reshape(-1, self.in_features)
+        if rows.stride(1) != 1 or (rows.shape[0] > 1 and rows.stride(0) < self.in_features):
+            rows = rows.contiguous()
+        out = torch.empty(rows.shape[0], self.out_features, device=x.device, dtype=x.dtype)
+        if residual is not None:
+            if residual.shape != x.shape[:-1] + (self.out_features,) or residual.dtype != torch.float32 or residual.device != x.device:
+                raise ValueError(f"Int8Linear: residual {tuple(residual.shape)} {residual.dtype}, expected float32 {tuple(x.shape[:-1]) + (self.out_features,)}")
+            residual = residual.contiguous()
+        if rows.shape[0]:
+            a, a_scale = _C.quantize_rows_i8(rows)
+            _C.linear_i8(a, a_scale, self.codes, self.scale, out, self.in_features, self.bias, residual, self.ACTIVATIONS[self.activation])
+        return out.view(x.shape[:-1] + (self.out_features,))

@@ -27,7 +27,7 @@
 extern "C" {
 #endif
 
-#define ACMI_VERSION 200 /* 0.2.0: acmi_lm_state.qkv_hand / hand_err (the decode step's QKV GEMM and self-attention as one launch with a per-(row, head) hand-off; opt-in per state).  0.1.9: post-norm layers (acmi_lm_model.post_norm, acmi_lm_layer.n1_g .. n2_b; acmi_ln_tile with eps < 0 = raw rows); score-folded cross-attention (acmi_cross_fold, acmi_lm_layer.w_qkvs .., acmi_lm_state.xs_rows).  0.1.8: acmi_ffn_engine (the tail of a decode layer as one persistent launch; measured slower than the launches, not used by
+#define ACMI_VERSION 300 /* 0.3.0: key / value cache in 8 bits (acmi_kv8_store, acmi_kv8_load, acmi_kv8_attn) and the int8 projection (acmi_quantize_rows_i8, acmi_linear_i8).  0.2.0: acmi_lm_state.qkv_hand / hand_err (the decode step's QKV GEMM and self-attention as one launch with a per-(row, head) hand-off; opt-in per state).  0.1.9: post-norm layers (acmi_lm_model.post_norm, acmi_lm_layer.n1_g .. n2_b; acmi_ln_tile with eps < 0 = raw rows); score-folded cross-attention (acmi_cross_fold, acmi_lm_layer.w_qkvs .., acmi_lm_state.xs_rows).  0.1.8: acmi_ffn_engine (the tail of a decode layer as one persistent launch; measured slower than the launches, not used by
                             acmi_lm_step), the decode step's cross-attention as a kernel of its own (cross_q_kernel, inside acmi_attn_decode_ex).  0.1.7: qk_layer_norm (acmi_lm_layer.q_ln_g .. cq_ln_b, acmi_layer_norm_rows), fuser 'sum' / 'input_interpolate'
                             (acmi_lm_state.input_add).  0.1.6: acmi_lstm_layer_ex / acmi_lstm_layer_work_floats (one recurrence per XCD at H = 1024).  0.1.5: folded LayerNorm with the row statistics taken from the activation fragments (acmi_linear_desc:
                             colsum without a_stats), left-padded streams (acmi_lm_state.row_off, acmi_attn_desc.start_rows: two_step_cfg
@@ -611,6 +611,97 @@ typedef struct {
  * active_rows and H at most 65535 -- larger values are rejected with ACMI_EINVAL.  acmi_linear_ex / acmi_linear_pair with a
  * tiled activation likewise: M, K tiles, a_rbs and ksplit at most 65535. */
 int acmi_attn_decode_ex(const acmi_attn_desc* desc, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Key / value cache in 8 bits (0.3.0)
+ * ------------------------------------------------------------------------------------------
+ * One attention layer's cache of `rows` streams.  A row's tokens stand in blocks of ACMI_KV8_BLOCK = 64:
+ *   - the NEWEST block of a row, partial or just completed, is kept as it was stored ("tail", f32 or bf16);
+ *   - every block before it is int8 codes with one f32 scale per (row, head, block), keys and values apart:
+ *         amax = max |x| over the block's 64 tokens x hd features;   scale = amax / 127;   code = rint(x * (127 / amax))
+ *     (each operation rounded to f32, ties to even; amax < 2^-120: codes and scale 0; a block that holds a NaN or an infinity
+ *     gets the scale NaN, so that all of it reads back as NaN).
+ * A block is quantised ONCE, from its exact tokens, by the call that stores its 64th token; that call also leaves it in the
+ * tail, which attention reads for the row's block (length - 1) / 64 until a token of the next block overwrites it.  So a token
+ * is exact while it is among the newest 1 .. 64 of its row, |error| <= scale / 2 afterwards, and never rounded twice.
+ * The caller zeroes the buffers once.  hd: 16, 32, 64 or 128.  A row holds nblk * 64 tokens; tokens past that are dropped.
+ * A row's length is the caller's (device int32), so every call here can be captured and replayed; nothing is kept in the
+ * library.  Lengths are clamped to [0, nblk * 64]. */
+#define ACMI_KV8_BLOCK 64
+typedef struct {
+    void* k_codes;          /* int8 [rows][H][nblk][64 tokens][hd] */
+    void* v_codes;          /* int8 [rows][H][nblk][hd][64], token t of the block at place ((t >> 2) & 3) * 16 + (t >> 4) * 4 + (t & 3):
+                               the order in which the probabilities leave the first matrix product */
+    float* k_scale; float* v_scale;   /* [rows][H][nblk] */
+    void* k_tail; void* v_tail;       /* [rows][H][64][hd] in tail_dtype */
+    int tail_dtype, rows, H, hd, nblk;
+} acmi_kv8_cache;
+
+/* Tokens start[r] .. start[r] + n[r] - 1 of every row r into the cache (n NULL: L each; start[r] = tokens the row holds
+ * already, which must have been stored in order).  k / v: `dtype` elements at row * *_row + token * *_tok + head * *_head
+ * (element strides), the hd features contiguous; tokens >= n[r] of a row are never read. */
+typedef struct {
+    const void* k; const void* v; int dtype;
+    long long k_row, k_tok, k_head, v_row, v_tok, v_head;
+    int L; const int* start; const int* n;
+} acmi_kv8_store_desc;
+int acmi_kv8_store(const acmi_kv8_cache* cache, const acmi_kv8_store_desc* desc, void* stream);
+
+/* The values the cache holds: k_out / v_out [rows][H][T][hd] in out_dtype, zeros at positions >= len[row]. */
+int acmi_kv8_load(const acmi_kv8_cache* cache, const int* len, int T, void* k_out, void* v_out, int out_dtype, void* stream);
+
+/* Attention over the cache (transformer.py:412-414 over what _complete_kv, :266-298, would hold): S queries per row,
+ * Hq = G * H query heads, query head h on cache head h / G.
+ *   length of row r = len[r * len_stride] + len_bias tokens (len_stride 0: one word for all rows);
+ *   causal: query i of a row sits at position length - q_len + i and sees positions <= its own, with past_context > 0 only the
+ *   last past_context before it; not causal: every query sees the whole row (cross-attention to states of another length).
+ *   q_len (or NULL = S): queries of every row; start_rows (or NULL): first position of a row that is seen (left padding).
+ *   A query that sees nothing, and queries >= q_len of a row, give zeros.
+ * k_new / v_new (S = 1; or NULL): the row's newest token, written at position length - 1 by this call before it is attended.
+ * With them, or with `complete` (the tail already holds the token), the call quantises a block that this token completes.
+ * out: out_mode ACMI_OUT_F32 / ACMI_OUT_BF16 = [rows][S][Hq][hd]; ACMI_OUT_TILED (S = 1) = tiled activation of `rows` rows in
+ * out_dtype with out_rbs K tiles per 16-row block, first column out_col0.
+ * The products of probabilities and values take f16 probabilities (2^-12 of each) for bf16 results, a pair of f16 for f32 ones;
+ * scores, softmax statistics and sums are f32.
+ * work: acmi_kv8_attn_work_floats(cache, S, Hq) floats of scratch of this call alone (NULL when that is 0). */
+typedef struct {
+    const void* q; int q_dtype; long long q_row, q_tok, q_head;
+    int S, Hq;
+    const int* len; int len_stride, len_bias;
+    const int* q_len; const int* start_rows;
+    int causal, past_context;
+    const void* k_new; const void* v_new; int new_dtype; long long kn_row, kn_head, vn_row, vn_head;
+    int complete;
+    void* out; int out_mode, out_dtype, out_rbs, out_col0;
+    float* work;
+} acmi_kv8_attn_desc;
+size_t acmi_kv8_attn_work_floats(const acmi_kv8_cache* cache, int S, int Hq);
+int acmi_kv8_attn(const acmi_kv8_cache* cache, const acmi_kv8_attn_desc* desc, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Projection in 8-bit integers (0.3.0)
+ * ------------------------------------------------------------------------------------------
+ * "int8 fragments" of a matrix X[R, K]: the tiled order of the decode step (above) with 16 one-byte elements per lane,
+ *     Xt[rt][kc][lane][j],  lane = kg * 16 + r,  holds  X[rt*16 + r][kc*64 + kg*16 + j],   kc < ceil(K / 64),
+ * columns past K zero, rows past R arbitrary (they only reach outputs that are not stored).  Weights (rows = output channels)
+ * and activations (rows = tokens) use the same order.
+ *
+ * One scale per row: scale = amax / 127, code = rint(x * (127 / amax)) with amax = max |x| of the row (amax < 2^-120: zeros;
+ * a row that holds a NaN or an infinity: scale NaN).  x: `dtype` (ACMI_F32 / ACMI_BF16), row pitch ldx elements.
+ * codes: ceil(R / 16) * ceil(K / 64) * 1024 bytes, 16-byte aligned. */
+int acmi_quantize_rows_i8(const void* x, int dtype, long long ldx, int R, int K, void* codes, float* scale, void* stream);
+
+/* out[M, N] = act(a_scale[m] * w_scale[n] * sum_k a[m, k] w[n, k] + bias[n]) + residual[m, n]: the sum exact in 32-bit integers
+ * (K <= 131072), one f32 product by a_scale * w_scale.  act: 0 none, 1 exact (erf) GELU.  bias [N] f32 or NULL; residual
+ * [M, N] f32 (pitch N) or NULL.  out: row-major, pitch ldo, out_dtype f32 / bf16. */
+typedef struct {
+    const void* a; const float* a_scale;
+    const void* w; const float* w_scale;
+    const float* bias; const float* residual;
+    void* out; int out_dtype; long long ldo;
+    int act, M, N, K;
+} acmi_linear_i8_desc;
+int acmi_linear_i8(const acmi_linear_i8_desc* desc, void* stream);
 
 /* ------------------------------------------------------------------------------------------
  * Prefill: the prompt / prepended-condition positions through ONE forward (reference lm.py:540-543,
