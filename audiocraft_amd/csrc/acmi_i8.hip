@@ -10,48 +10,110 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 // =====================================================================================================
 // rows -> int8 fragments + a scale each
 // =====================================================================================================
-struct QuantRowsArgs { const void* x; int bf16; long long ldx; int R, K, nkc; uint8_t* codes; float* scale; };
+struct RowSrc { const void* x; long long ldx; int bf16, vec, R, K; };   // vec: rows start on 4-element boundaries
 
-__device__ __forceinline__ float i8_ld(const void* p, size_t i, int bf16) {
-    return bf16 ? bf16_to_f32(reinterpret_cast<const bf16_t*>(p)[i]) : reinterpret_cast<const float*>(p)[i];
+// columns [col, col + 4) of a row; 0 past K
+__device__ __forceinline__ f32x4 row_ld4(const RowSrc& s, size_t base, int col) {
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (s.vec && col + 4 <= s.K) {
+        if (s.bf16) {
+            const uint2 w = *reinterpret_cast<const uint2*>(reinterpret_cast<const bf16_t*>(s.x) + base + col);
+            v = f32x4{__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u)};
+        } else {
+            v = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(s.x) + base + col);
+        }
+        return v;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (col + e < s.K) v[e] = s.bf16 ? bf16_to_f32(reinterpret_cast<const bf16_t*>(s.x)[base + col + e]) : reinterpret_cast<const float*>(s.x)[base + col + e];
+    return v;
 }
-__device__ __forceinline__ uint32_t i8_code(float x, float inv) { return (uint32_t)(uint8_t)(int8_t)(int)rintf(x * inv); }
+__device__ __forceinline__ float row_max4(const f32x4& v, float m) {   // +infinity for a NaN, which fmaxf would drop
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float a = fabsf(v[e]);
+        m = fmaxf(m, a <= 3.4028234663852886e38f ? a : INFINITY);
+    }
+    return m;
+}
+__device__ __forceinline__ void row_scale(float amax, float& scale, float& inv) {
+    if (amax == INFINITY) { scale = __uint_as_float(0x7fc00000u); inv = 0.f; }
+    else if (amax < 7.52316384526264e-37f) { scale = 0.f; inv = 0.f; }   // 2^-120: 127 / amax stays finite above
+    else { scale = __fdiv_rn(amax, 127.f); inv = __fdiv_rn(127.f, amax); }
+}
+// 4 codes: the product rounded to f32, then to the nearest integer by adding 1.5 * 2^23 (ties to even, |product| <= 127 (1 +
+// 2^-23)), whose low byte it then is.  (A row with a NaN has inv = 0; a NaN product gives some byte, its scale is NaN.)
+__device__ __forceinline__ uint32_t row_codes4(const f32x4& v, float inv) {
+    uint32_t b[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) b[e] = __float_as_uint(v[e] * inv + 12582912.f);
+    const uint32_t lo = __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(b[3], b[2], 0x04000c0cu);
+    return lo | hi;
+}
 
-// one workgroup per row; a thread owns chunks of 16 consecutive columns = the 16 bytes of one lane of a fragment
-__global__ __launch_bounds__(256) void quant_rows_kernel(const QuantRowsArgs p) {
-    __shared__ float red[4];
-    const int row = blockIdx.x, nch = p.nkc * 4;
-    const size_t xb = (size_t)(row * p.ldx);
+struct QuantRowsArgs { RowSrc s; int nkc, kchunk; uint8_t* codes; float* scale; };
+
+// One workgroup per 16 rows, a wave per row: the row is read once (NV x 256 columns of it stay in registers, longer ones are read
+// again from L2), its codes are laid down in LDS, and the 16 rows leave as whole fragments, 1 KB at a time.  (One workgroup per row
+// wrote 16-byte pieces 256 bytes apart: 38 us for 9600 x 1536 f32, now ~15; profiles: bound by the read.)
+template <int NV>
+__global__ __launch_bounds__(1024) void quant_rows_kernel(const QuantRowsArgs p) {
+    extern __shared__ __attribute__((aligned(16))) unsigned char sm[];   // [16][kchunk + 16]
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int row = blockIdx.x * 16 + wave, kpad = p.nkc * 64, pitch = p.kchunk + 16;
+    const bool live = row < p.s.R;
+    const size_t base = (size_t)((live ? row : 0) * p.s.ldx);
+    f32x4 v[NV];
     float amax = 0.f;
-    for (int k = threadIdx.x; k < p.K; k += 256) {
-        const float v = i8_ld(p.x, xb + k, p.bf16);
-        amax = fmaxf(amax, isfinite(v) ? fabsf(v) : INFINITY);   // (fmaxf would drop a NaN)
+    if (live) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) v[i] = row_ld4(p.s, base, (i * 64 + lane) * 4);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) amax = row_max4(v[i], amax);
+        for (int c = (NV * 64 + lane) * 4; c < p.s.K; c += 256) amax = row_max4(row_ld4(p.s, base, c), amax);
     }
     amax = wave_max(amax);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = amax;
-    __syncthreads();
-    amax = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
     float scale, inv;
-    if (amax == INFINITY) { scale = __uint_as_float(0x7fc00000u); inv = 0.f; }
-    else if (amax < 7.52316384526264e-37f) { scale = 0.f; inv = 0.f; }   // 2^-120
-    else { scale = __fdiv_rn(amax, 127.f); inv = __fdiv_rn(127.f, amax); }
-    if (threadIdx.x == 0) p.scale[row] = scale;
-    for (int ch = threadIdx.x; ch < nch; ch += 256) {
-        u32x4 w;
+    row_scale(amax, scale, inv);
+    if (live && lane == 0) p.scale[row] = scale;
+    for (int k0 = 0; k0 < kpad; k0 += p.kchunk) {   // (one round unless K > 8192)
+        const int k1 = min(kpad, k0 + p.kchunk);
+        if (k0 > 0) __syncthreads();
+        uint32_t* dst = reinterpret_cast<uint32_t*>(sm + wave * pitch);
+        if (!live) {
+            for (int c = k0 + lane * 4; c < k1; c += 256) dst[(c - k0) >> 2] = 0;
+        } else if (k0 == 0) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            uint32_t b = 0;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int col = ch * 16 + k * 4 + e;
-                const float v = col < p.K ? i8_ld(p.x, xb + col, p.bf16) : 0.f;
-                b |= i8_code(v, inv) << (8 * e);
+            for (int i = 0; i < NV; ++i) {
+                const int c = (i * 64 + lane) * 4;
+                if (c < k1) dst[c >> 2] = row_codes4(v[i], inv);
             }
-            w[k] = b;
+            for (int c = (NV * 64 + lane) * 4; c < k1; c += 256) dst[c >> 2] = row_codes4(row_ld4(p.s, base, c), inv);
+        } else {
+            for (int c = k0 + lane * 4; c < k1; c += 256) dst[(c - k0) >> 2] = row_codes4(row_ld4(p.s, base, c), inv);
         }
-        const size_t frag = (size_t)(row >> 4) * p.nkc + (ch >> 2);
-        *reinterpret_cast<u32x4*>(p.codes + frag * 1024 + ((ch & 3) * 16 + (row & 15)) * 16) = w;
+        __syncthreads();
+        u32x4* out = reinterpret_cast<u32x4*>(p.codes) + ((size_t)blockIdx.x * p.nkc + (k0 >> 6)) * 64 + lane;
+        for (int kc = wave; kc < (k1 - k0) >> 6; kc += 16)
+            out[(size_t)kc * 64] = *reinterpret_cast<const u32x4*>(sm + (lane & 15) * pitch + kc * 64 + (lane >> 4) * 16);
     }
+}
+
+static RowSrc row_src(const void* x, int dtype, long long ldx, int R, int K) {
+    const int bf16 = dtype == ACMI_BF16;
+    return RowSrc{x, ldx, bf16, (reinterpret_cast<size_t>(x) & (bf16 ? 7 : 15)) == 0 && ldx % 4 == 0, R, K};
+}
+static int launch_quant_rows(const RowSrc& s, uint8_t* codes, float* scale, hipStream_t st) {
+    QuantRowsArgs a = {s, (s.K + 63) / 64, 0, codes, scale};
+    a.kchunk = min(a.nkc * 64, 8192);
+    const size_t lds = (size_t)16 * (a.kchunk + 16);
+    static const bool ok = hipFuncSetAttribute(reinterpret_cast<const void*>(&quant_rows_kernel<8>), hipFuncAttributeMaxDynamicSharedMemorySize, 16 * (8192 + 16)) == hipSuccess &&
+                           hipFuncSetAttribute(reinterpret_cast<const void*>(&quant_rows_kernel<2>), hipFuncAttributeMaxDynamicSharedMemorySize, 16 * (8192 + 16)) == hipSuccess;
+    ACMI_REQUIRE(ok, "acmi_quantize_rows_i8: cannot set the dynamic LDS limit");
+    if (s.K <= 512) hipLaunchKernelGGL(quant_rows_kernel<2>, dim3((s.R + 15) / 16), dim3(1024), lds, st, a);
+    else hipLaunchKernelGGL(quant_rows_kernel<8>, dim3((s.R + 15) / 16), dim3(1024), lds, st, a);
+    return acmi_check_launch("quant_rows_kernel");
 }
 
 extern "C" int acmi_quantize_rows_i8(const void* x, int dtype, long long ldx, int R, int K, void* codes, float* scale, void* stream) {
@@ -60,9 +122,7 @@ extern "C" int acmi_quantize_rows_i8(const void* x, int dtype, long long ldx, in
     if (R == 0) return ACMI_OK;
     ACMI_REQUIRE(x && codes && scale && ldx >= K, "acmi_quantize_rows_i8: null buffer or ldx=%lld < K=%d", ldx, K);
     ACMI_REQUIRE((reinterpret_cast<size_t>(codes) & 15) == 0, "acmi_quantize_rows_i8: codes must be 16-byte aligned");
-    QuantRowsArgs a = {x, dtype == ACMI_BF16, ldx, R, K, (K + 63) / 64, reinterpret_cast<uint8_t*>(codes), scale};
-    hipLaunchKernelGGL(quant_rows_kernel, dim3(R), dim3(256), 0, (hipStream_t)stream, a);
-    return acmi_check_launch("quant_rows_kernel");
+    return launch_quant_rows(row_src(x, dtype, ldx, R, K), reinterpret_cast<uint8_t*>(codes), scale, (hipStream_t)stream);
 }
 
 // =====================================================================================================

@@ -28,6 +28,11 @@ __device__ __forceinline__ void big_mma(const u32x4& a, const u32x4& b, f32x4& a
     for (int e = 0; e < 4; ++e)
         acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[e]), __uint_as_float(b[e]), acc, 0, 0, 0);
 }
+typedef __bf16 hw_bf16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t pack_bf16x2_hw(float lo, float hi) {   // round to nearest even, like pack_bf16x2
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{lo, hi}, hw_bf16x2));
+}
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ void big_mma(const u32x4& a, const u32x4& b, i32x4& acc, int8_t) {   // one fragment = 64 int8 columns
     acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), acc, 0, 0, 0);
@@ -279,33 +284,56 @@ __global__ __launch_bounds__(BigTile<BIG>::NW * 64, BIG ? 1 : 2) void lin_big_ke
     const int nl = lane & 15, kg = lane >> 4;
     const int row0 = (tm << TS) + wm * (WI * 16) + nl, col0 = (tn << TS) + wn * 64 + kg * 4;
     if constexpr (EPI == ACMI_BIG_I8) {
-        float sa[WI];
+        // The finished sums go through LDS, half of every wave's rows at a time: straight from the registers a lane holds 4 features
+        // of a row (8 bytes of a bf16 output, 16 rows apart from its neighbours) and the scaling + GELU, unrolled over 128
+        // accumulators, spills; from LDS a wave takes whole rows of the tile, its column scales and biases loaded once.
+        constexpr int HI = WI / 2, PITCH = TC::T + 4, HR = 2 * HI * 16, CW = TC::T / 4;   // (two waves along m)
+        float* sm = reinterpret_cast<float*>(smem);
+        const int c4 = threadIdx.x % CW, col = (tn << TS) + c4 * 4;
+        float sw[4], bi[4];
 #pragma unroll
-        for (int i = 0; i < WI; ++i) sa[i] = p.a_scale[min(row0 + i * 16, p.rows - 1)];
+        for (int r = 0; r < 4; ++r) {
+            sw[r] = p.w_scale[min(col + r, p.N - 1)];
+            bi[r] = p.bias != nullptr ? p.bias[min(col + r, p.N - 1)] : 0.f;
+        }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int col = col0 + j * 16;
-            if (col >= p.N) continue;
-            float sw[4], bi[4];
+        for (int h = 0; h < 2; ++h) {
+            __syncthreads();
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                sw[r] = p.w_scale[min(col + r, p.N - 1)];
-                bi[r] = p.bias != nullptr ? p.bias[min(col + r, p.N - 1)] : 0.f;
-            }
+            for (int i = 0; i < HI; ++i)
 #pragma unroll
-            for (int i = 0; i < WI; ++i) {
-                const int row = row0 + i * 16;
-                if (row >= p.rows) continue;
+                for (int j = 0; j < 4; ++j) {
+                    const acc4 v = acc[h * HI + i][j];
+                    *reinterpret_cast<f32x4*>(sm + (wm * HI * 16 + i * 16 + nl) * PITCH + wn * 64 + j * 16 + kg * 4) =
+                        f32x4{(float)v[0], (float)v[1], (float)v[2], (float)v[3]};
+                }
+            __syncthreads();
+#pragma unroll 2
+            for (int rr = threadIdx.x / CW; rr < HR; rr += TC::NW * 64 / CW) {
+                const int row = (tm << TS) + (rr / (HI * 16)) * (WI * 16) + h * HI * 16 + rr % (HI * 16);
+                if (row >= p.rows || col >= p.N) continue;
+                const f32x4 x = *reinterpret_cast<const f32x4*>(sm + rr * PITCH + c4 * 4);
+                const float sa = p.a_scale[row];
                 float v[4];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    v[r] = __builtin_fmaf((float)acc[i][j][r], sa[i] * sw[r], bi[r]);
-                    if (p.act == 1) v[r] = p.out_bf16 ? big_gelu_bf16(v[r]) : big_gelu(v[r]);
-                    if (p.residual != nullptr && col + r < p.N) v[r] += p.residual[(size_t)row * p.N + col + r];
+                for (int r = 0; r < 4; ++r) v[r] = __builtin_fmaf(x[r], sa * sw[r], bi[r]);
+                if (p.act == 1) {
+                    if (p.out_bf16) {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) v[r] = big_gelu_bf16(v[r]);
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) v[r] = big_gelu(v[r]);
+                    }
+                }
+                if (p.residual != nullptr) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (col + r < p.N) v[r] += p.residual[(size_t)row * p.N + col + r];
                 }
                 const size_t at = (size_t)(row * p.ldo64) + col;
                 if (p.vec) {
-                    if (p.out_bf16) *reinterpret_cast<uint2*>(reinterpret_cast<bf16_t*>(p.out) + at) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+                    if (p.out_bf16) *reinterpret_cast<uint2*>(reinterpret_cast<bf16_t*>(p.out) + at) = make_uint2(pack_bf16x2_hw(v[0], v[1]), pack_bf16x2_hw(v[2], v[3]));
                     else *reinterpret_cast<f32x4*>(p.out + at) = f32x4{v[0], v[1], v[2], v[3]};
                 } else {
 #pragma unroll
@@ -416,7 +444,8 @@ __global__ __launch_bounds__(BigTile<BIG>::NW * 64, BIG ? 1 : 2) void lin_big_ke
 
 template <typename WT, int E, int BIG>
 static int launch_big_k(const BigArgs& a, int tiles, hipStream_t st) {
-    constexpr size_t lds = 4 * BigTile<BIG>::SLOT * 1024;
+    constexpr size_t ring = 4 * BigTile<BIG>::SLOT * 1024, joint = (size_t)BigTile<BIG>::WI * 16 * (BigTile<BIG>::T + 4) * 4;
+    constexpr size_t lds = E == ACMI_BIG_I8 && joint > ring ? joint : ring;   // the int8 epilogue's half tile of sums
     static const bool attr_ok = hipFuncSetAttribute(reinterpret_cast<const void*>(&lin_big_kernel<WT, E, BIG>),
                                                     hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) == hipSuccess;   // once, thread safe
     if (!attr_ok) {
@@ -486,7 +515,11 @@ int acmi_launch_big_i8(BigArgs& a, hipStream_t st) {
     a.epi = ACMI_BIG_I8;
     const size_t align = a.out_bf16 ? 7 : 15;
     a.vec = a.N % 4 == 0 && a.ldo64 % 4 == 0 && (reinterpret_cast<size_t>(a.out) & align) == 0;
-    const int t256 = ((a.M + 255) >> 8) * ((a.N + 255) >> 8), big = t256 >= 128;
+    // 256 x 256 tiles (one workgroup per CU) where they fill whole rounds of the 256 CUs to 85 %, else 128 x 128 (two per CU).
+    // Measured, us large / small, bf16 results: 9600 x 1536 x 6144 (228 tiles) 84.5 / 97.7; 2048 x 8192 x 2048 (256) 41.1 / 44.4;
+    // 9600 x 6144 x 1536 (912) 133 / 137; but 4800 x 4096 x 1024 (304) 49.1 / 38.4; 1000 x 4608 x 1536 (72) 28.3 / 17.8
+    const int t256 = ((a.M + 255) >> 8) * ((a.N + 255) >> 8), rounds = (t256 + 255) >> 8;
+    const int big = t256 * 100 >= rounds * 256 * 85;
     const int tiles = big_grid(a.M, a.N, big ? 8 : 7);
     const int rc = big ? launch_big_k<int8_t, ACMI_BIG_I8, 1>(a, tiles, st) : launch_big_k<int8_t, ACMI_BIG_I8, 0>(a, tiles, st);
     return rc ? rc : acmi_check_launch("lin_big_kernel");
@@ -530,11 +563,6 @@ extern "C" int acmi_linear_big(const void* a, int a_rbs, const void* w, int wdty
 // half of the time at two waves per SIMD, and requesting the next key block one iteration early did not change it:
 // r04_session26 / 27).
 // QB: 16-query blocks per wave (consecutive positions): a K / V^T fragment is fetched once and multiplied QB times.
-typedef __bf16 hw_bf16x2 __attribute__((ext_vector_type(2)));
-typedef float f32x2 __attribute__((ext_vector_type(2)));
-__device__ __forceinline__ uint32_t pack_bf16x2_hw(float lo, float hi) {   // round to nearest even, like pack_bf16x2
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{lo, hi}, hw_bf16x2));
-}
 
 template <typename KT, int HD, int QB>
 __global__ __launch_bounds__(256) void attn_prefill_kernel(const PrefillAttnArgs p) {
