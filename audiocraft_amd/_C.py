@@ -169,7 +169,8 @@ class KV8AttnDesc(C.Structure):
 
 class LinearI8Desc(C.Structure):
     _fields_ = [('a', vp), ('a_scale', vp), ('w', vp), ('w_scale', vp), ('bias', vp), ('residual', vp), ('out', vp),
-                ('out_dtype', i32), ('ldo', i64), ('act', i32), ('M', i32), ('N', i32), ('K', i32)]
+                ('out_dtype', i32), ('ldo', i64), ('act', i32), ('M', i32), ('N', i32), ('K', i32), ('x', vp), ('x_dtype', i32),
+                ('ldx', i64), ('work', vp)]
 
 
 KV8_BLOCK = 64
@@ -178,6 +179,7 @@ _kv8_load = _sig('acmi_kv8_load', [C.POINTER(KV8CacheDesc), vp, i32, vp, vp, i32
 _kv8_attn_work = _sig('acmi_kv8_attn_work_floats', [C.POINTER(KV8CacheDesc), i32, i32], C.c_size_t)
 _kv8_attn = _sig('acmi_kv8_attn', [C.POINTER(KV8CacheDesc), C.POINTER(KV8AttnDesc), vp])
 _quantize_rows_i8 = _sig('acmi_quantize_rows_i8', [vp, i32, i64, i32, i32, vp, vp, vp])
+_linear_i8_work = _sig('acmi_linear_i8_work_bytes', [i32, i32], C.c_size_t)
 _linear_i8 = _sig('acmi_linear_i8', [C.POINTER(LinearI8Desc), vp])
 
 _linear_ex = _sig('acmi_linear_ex', [C.POINTER(LinearDesc), vp])
@@ -215,7 +217,7 @@ EXPORTS = ['acmi_group_norm_work_floats', 'acmi_group_norm', 'acmi_channel_add',
            'acmi_conv1d', 'acmi_conv1d_gn', 'acmi_conv1d_tile_weights', 'acmi_conv1d_weight_floats', 'acmi_conv1d_work_floats', 'acmi_lstm_layer', 'acmi_lstm_work_floats', 'acmi_lstm_layer_ex', 'acmi_lstm_layer_work_floats', 'acmi_lstm_stack2', 'acmi_lstm_stack2_work_floats', 'acmi_lstm_stack2_supported', 'acmi_lm_step', 'acmi_linear',
            'acmi_attn_decode', 'acmi_kv_store', 'acmi_sample', 'acmi_pos_table', 'acmi_ln_tile', 'acmi_linear_ex', 'acmi_ln_tile_reduce', 'acmi_linear_pair', 'acmi_attn_decode_ex', 'acmi_layer_norm_rows',
            'acmi_ffn_engine', 'acmi_ffn_engine_supported', 'acmi_cross_fold', 'acmi_qkv_attn_launches',
-           'acmi_kv8_store', 'acmi_kv8_load', 'acmi_kv8_attn_work_floats', 'acmi_kv8_attn', 'acmi_quantize_rows_i8', 'acmi_linear_i8']
+           'acmi_kv8_store', 'acmi_kv8_load', 'acmi_kv8_attn_work_floats', 'acmi_kv8_attn', 'acmi_quantize_rows_i8', 'acmi_linear_i8_work_bytes', 'acmi_linear_i8']
 
 
 # ctypes mirror -> C type of include/acmi.h (tests/test_host_cpu.py compiles the header with gcc and compares every
@@ -662,40 +664,50 @@ def attn_prefill(q, k_cache, vt, out, npos, npos_pad, pos, past_context=0, out_r
 # ---------------------------------------------------------------------------------- 8-bit cache and projection
 # (the callers, modules/kv8_cache.py and modules/int8_linear.py, check shapes, types and devices)
 
-def on_device(t: torch.Tensor):
-    """The device guard of a call on `t`: kernels are launched on the current device's current stream."""
-    import contextlib
-    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+
+
+def launch(device: torch.device, what: str, fn, *args):
+    """fn(*args, stream) on `device` and its current stream, whatever the current device is."""
+    i = device.index
+    if _current_device() == i:
+        rc = fn(*args, _raw_stream(i))
+    else:
+        with torch.cuda.device(i):
+            rc = fn(*args, _raw_stream(i))
+    if rc != 0:
+        check(rc, what)
 
 
 def kv8_store(cache: KV8CacheDesc, k, v, start, n):
     """k / v [rows, L, H, hd] (any strides over the first three), start / n int32 [rows] (n None: L)."""
-    d = KV8StoreDesc(k.data_ptr(), v.data_ptr(), dtype_code(k.dtype), k.stride(0), k.stride(1), k.stride(2), v.stride(0),
-                     v.stride(1), v.stride(2), k.shape[1], start.data_ptr(), None if n is None else n.data_ptr())
-    with on_device(k):
-        check(_kv8_store(C.byref(cache), C.byref(d), stream()), 'acmi_kv8_store')
+    ks, vs = k.stride(), v.stride()
+    d = KV8StoreDesc(k.data_ptr(), v.data_ptr(), dtype_code(k.dtype), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], k.shape[1],
+                     start.data_ptr(), None if n is None else n.data_ptr())
+    launch(k.device, 'acmi_kv8_store', _kv8_store, C.byref(cache), C.byref(d))
 
 
 def kv8_load(cache: KV8CacheDesc, lens, T, k_out, v_out):
-    with on_device(k_out):
-        check(_kv8_load(C.byref(cache), lens.data_ptr(), T, k_out.data_ptr(), v_out.data_ptr(), dtype_code(k_out.dtype), stream()),
-              'acmi_kv8_load')
+    launch(k_out.device, 'acmi_kv8_load', _kv8_load, C.byref(cache), lens.data_ptr(), T, k_out.data_ptr(), v_out.data_ptr(),
+           dtype_code(k_out.dtype))
 
 
-def kv8_attn(cache: KV8CacheDesc, q, out, lens, len_bias=0, causal=True, past_context=0, q_lens=None, starts=None, k_new=None,
-             v_new=None):
-    """q [rows, S, Hq, hd] (any strides over the first three) -> out [rows, S, Hq, hd] dense; k_new / v_new [rows, H, hd]."""
-    S, Hq = q.shape[1], q.shape[2]
-    new = (None, None, 0, 0, 0, 0, 0) if k_new is None else (
-        k_new.data_ptr(), v_new.data_ptr(), dtype_code(k_new.dtype), k_new.stride(0), k_new.stride(1), v_new.stride(0), v_new.stride(1))
-    with on_device(q):
-        nw = _kv8_attn_work(C.byref(cache), S, Hq)
-        work = torch.empty(nw, device=q.device, dtype=torch.float32) if nw else None
-        d = KV8AttnDesc(q.data_ptr(), dtype_code(q.dtype), q.stride(0), q.stride(1), q.stride(2), S, Hq, lens.data_ptr(), 1, len_bias,
-                        None if q_lens is None else q_lens.data_ptr(), None if starts is None else starts.data_ptr(), int(causal),
-                        past_context, *new, 0, out.data_ptr(), OUT_BF16 if out.dtype == torch.bfloat16 else OUT_F32,
-                        dtype_code(out.dtype), 0, 0, None if work is None else work.data_ptr())
-        check(_kv8_attn(C.byref(cache), C.byref(d), stream()), 'acmi_kv8_attn')
+def kv8_attn(cache: KV8CacheDesc, q, q_strides, S, out, lens, len_bias=0, causal=True, past_context=0, q_lens=None, starts=None,
+             k_new=None, v_new=None):
+    """q [rows, (S,) Hq, hd] with strides (row, query, head) -> out [rows, (S,) Hq, hd] dense; k_new / v_new [rows, H, hd]."""
+    Hq = q.shape[-2]
+    if k_new is None:
+        new = (None, None, 0, 0, 0, 0, 0)
+    else:
+        kn, vn = k_new.stride(), v_new.stride()
+        new = (k_new.data_ptr(), v_new.data_ptr(), dtype_code(k_new.dtype), kn[0], kn[1], vn[0], vn[1])
+    nw = _kv8_attn_work(C.byref(cache), S, Hq)
+    work = torch.empty(nw, device=q.device, dtype=torch.float32) if nw else None
+    d = KV8AttnDesc(q.data_ptr(), dtype_code(q.dtype), *q_strides, S, Hq, lens.data_ptr(), 1, len_bias,
+                    None if q_lens is None else q_lens.data_ptr(), None if starts is None else starts.data_ptr(), int(causal),
+                    past_context, *new, 0, out.data_ptr(), OUT_BF16 if out.dtype == torch.bfloat16 else OUT_F32,
+                    dtype_code(out.dtype), 0, 0, None if work is None else work.data_ptr())
+    launch(q.device, 'acmi_kv8_attn', _kv8_attn, C.byref(cache), C.byref(d))
     return out
 
 
@@ -704,19 +716,28 @@ def quantize_rows_i8(x: torch.Tensor):
     R, K = x.shape
     codes = torch.empty(-(-R // 16) * -(-K // 64) * 1024, device=x.device, dtype=torch.int8)
     scale = torch.empty(R, device=x.device, dtype=torch.float32)
-    with on_device(x):
-        check(_quantize_rows_i8(x.data_ptr(), dtype_code(x.dtype), x.stride(0) if R > 1 else K, R, K, codes.data_ptr(), scale.data_ptr(),
-                                stream()), 'acmi_quantize_rows_i8')
+    launch(x.device, 'acmi_quantize_rows_i8', _quantize_rows_i8, x.data_ptr(), dtype_code(x.dtype), x.stride(0) if R > 1 else K, R, K,
+           codes.data_ptr(), scale.data_ptr())
     return codes, scale
 
 
-def linear_i8(a, a_scale, w, w_scale, out, K, bias=None, residual=None, act=0):
-    """out [M, N] = act(a_scale w_scale (a . w) + bias) + residual on int8 fragments (acmi_linear_i8)."""
+def linear_i8(x, w, w_scale, out, bias=None, residual=None, act=0, a_scale=None, K=None):
+    """out [M, N] = act(..) + residual (acmi_linear_i8): x [M, K] f32 / bf16 (rows contiguous, any pitch), or with a_scale the int8
+    fragments of an activation of K columns (quantize_rows_i8)."""
     M, N = out.shape
-    d = LinearI8Desc(a.data_ptr(), a_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(), None if bias is None else bias.data_ptr(),
-                     None if residual is None else residual.data_ptr(), out.data_ptr(), dtype_code(out.dtype), N, act, M, N, K)
-    with on_device(out):
-        check(_linear_i8(C.byref(d), stream()), 'acmi_linear_i8')
+    work = None
+    if a_scale is None:
+        K = x.shape[1]
+        nw = _linear_i8_work(M, K)
+        if nw:
+            work = torch.empty(nw, device=x.device, dtype=torch.uint8)
+        src = (x.data_ptr(), dtype_code(x.dtype), x.stride(0) if M > 1 else K, None if work is None else work.data_ptr())
+        act8 = (None, None)
+    else:
+        src, act8 = (None, 0, 0, None), (x.data_ptr(), a_scale.data_ptr())
+    d = LinearI8Desc(*act8, w.data_ptr(), w_scale.data_ptr(), None if bias is None else bias.data_ptr(),
+                     None if residual is None else residual.data_ptr(), out.data_ptr(), dtype_code(out.dtype), N, act, M, N, K, *src)
+    launch(out.device, 'acmi_linear_i8', _linear_i8, C.byref(d))
     return out
 
 

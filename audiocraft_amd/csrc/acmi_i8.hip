@@ -100,6 +100,48 @@ __global__ __launch_bounds__(1024) void quant_rows_kernel(const QuantRowsArgs p)
     }
 }
 
+// few rows: one workgroup of 8 waves per row, all of it in flight at once (8192 columns in registers); the 16-byte pieces it writes
+// lie 256 bytes apart, which costs nothing while there are few.  16 x 6144 f32: 9.5 -> 3.2 us
+__global__ __launch_bounds__(512) void quant_row_wide_kernel(const QuantRowsArgs p) {
+    constexpr int NV = 4, STEP = 512 * 4;
+    __shared__ float red[8];
+    extern __shared__ __attribute__((aligned(16))) unsigned char sm[];   // [kchunk]
+    const int row = blockIdx.x, kpad = p.nkc * 64;
+    const size_t base = (size_t)(row * p.s.ldx);
+    f32x4 v[NV];
+    float amax = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) v[i] = row_ld4(p.s, base, i * STEP + threadIdx.x * 4);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) amax = row_max4(v[i], amax);
+    for (int c = NV * STEP + threadIdx.x * 4; c < p.s.K; c += STEP) amax = row_max4(row_ld4(p.s, base, c), amax);
+    amax = wave_max(amax);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = amax;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 8; ++k) amax = fmaxf(amax, red[k]);
+    float scale, inv;
+    row_scale(amax, scale, inv);
+    if (threadIdx.x == 0) p.scale[row] = scale;
+    uint32_t* dst = reinterpret_cast<uint32_t*>(sm);
+    for (int k0 = 0; k0 < kpad; k0 += p.kchunk) {   // (one round unless K > 8192)
+        const int k1 = min(kpad, k0 + p.kchunk);
+        if (k0 > 0) __syncthreads();
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = i * STEP + threadIdx.x * 4;
+            if (k0 == 0) { if (c < k1) dst[c >> 2] = row_codes4(v[i], inv); }
+            else if (k0 + c < k1) dst[c >> 2] = row_codes4(row_ld4(p.s, base, k0 + c), inv);
+        }
+        __syncthreads();
+        for (int ch = threadIdx.x; ch < (k1 - k0) >> 4; ch += 512) {
+            const int g = (k0 >> 4) + ch;   // chunk of 16 columns = 16 bytes of one lane of fragment g / 4
+            const size_t frag = (size_t)(row >> 4) * p.nkc + (g >> 2);
+            *reinterpret_cast<u32x4*>(p.codes + frag * 1024 + ((g & 3) * 16 + (row & 15)) * 16) = *reinterpret_cast<const u32x4*>(sm + ch * 16);
+        }
+    }
+}
+
 static RowSrc row_src(const void* x, int dtype, long long ldx, int R, int K) {
     const int bf16 = dtype == ACMI_BF16;
     return RowSrc{x, ldx, bf16, (reinterpret_cast<size_t>(x) & (bf16 ? 7 : 15)) == 0 && ldx % 4 == 0, R, K};
@@ -107,6 +149,11 @@ static RowSrc row_src(const void* x, int dtype, long long ldx, int R, int K) {
 static int launch_quant_rows(const RowSrc& s, uint8_t* codes, float* scale, hipStream_t st) {
     QuantRowsArgs a = {s, (s.K + 63) / 64, 0, codes, scale};
     a.kchunk = min(a.nkc * 64, 8192);
+    // up to two workgroups per CU by rows; above, whole fragments (us: 384 x 1536 f32 3.9 against 4.3, 1000 x 1000 5.4 against 4.6)
+    if (s.R <= 512) {
+        hipLaunchKernelGGL(quant_row_wide_kernel, dim3(s.R), dim3(512), (size_t)a.kchunk, st, a);
+        return acmi_check_launch("quant_row_wide_kernel");
+    }
     const size_t lds = (size_t)16 * (a.kchunk + 16);
     static const bool ok = hipFuncSetAttribute(reinterpret_cast<const void*>(&quant_rows_kernel<8>), hipFuncAttributeMaxDynamicSharedMemorySize, 16 * (8192 + 16)) == hipSuccess &&
                            hipFuncSetAttribute(reinterpret_cast<const void*>(&quant_rows_kernel<2>), hipFuncAttributeMaxDynamicSharedMemorySize, 16 * (8192 + 16)) == hipSuccess;
@@ -128,59 +175,135 @@ extern "C" int acmi_quantize_rows_i8(const void* x, int dtype, long long ldx, in
 // =====================================================================================================
 // few rows: the weight is streamed once
 // =====================================================================================================
-// One workgroup per 16 output channels; its NW waves split K, every wave multiplies its weight fragments with MT 16-row blocks
-// of the activation, and the integer partial sums meet in LDS (exact, so their order does not matter).  Transposed like the
-// prefill GEMM: A operand = weight, so a lane ends with 4 consecutive channels of one row.
+// One workgroup per 16 output channels (and MT 16-row blocks); its NW waves split K, every wave multiplies its weight fragments
+// with MT row blocks of the activation, and the integer partial sums meet in LDS (exact, so their order does not matter).
+// Transposed like the prefill GEMM: A operand = weight, so a lane ends with 4 consecutive channels of one row.  The first WF
+// weight fragments of a wave (and, for one row block, its activation's) are requested before anything else: up to K = 4096 with 8
+// waves, 8192 with 16, a call is one round trip to memory.
+// FUSED (at most 16 rows): the workgroup quantises the activation itself, into LDS, while its weights arrive -- a launch less.
 struct I8Args {
     const u32x4* a; const float* a_scale; const u32x4* w; const float* w_scale; const float* bias; const float* residual;
     void* out; int out_bf16; long long ldo; int act, M, N, K, nkc;
+    RowSrc s;
 };
+constexpr int I8_WF = 8;
 
 __device__ __forceinline__ void i8_mma(const u32x4& a, const u32x4& b, i32x4& acc) {
     acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), acc, 0, 0, 0);
 }
 __device__ __forceinline__ float i8_gelu(float x) { return 0.5f * x * (1.0f + erff(x * 0.70710678118654752440f)); }
 
-template <int MT, int NW>
+template <int MT, int NW, bool FUSED>
 __global__ __launch_bounds__(NW * 64) void lin_i8_kernel(const I8Args p) {
+    constexpr int WF = I8_WF, NV = 4;
+    constexpr bool AF = MT == 1 && !FUSED;   // the activation's fragments are requested next to the weight's
     __shared__ i32x4 part[NW][MT][64];
+    __shared__ float red[FUSED ? NW : 1], fscale[FUSED ? 16 : 1];
+    extern __shared__ __attribute__((aligned(16))) unsigned char sm[];   // FUSED: [16][nkc * 64 + 16] codes
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int nt = blockIdx.x, mt0 = blockIdx.y * MT, mtiles = (p.M + 15) / 16;
     const u32x4* w = p.w + (size_t)nt * p.nkc * 64 + lane;
+    u32x4 wf[WF];
+#pragma unroll
+    for (int f = 0; f < WF; ++f) wf[f] = __builtin_nontemporal_load(w + (size_t)min(wave + f * NW, p.nkc - 1) * 64);
+    u32x4 apre[AF ? WF : 1];
+    if constexpr (AF) {
+#pragma unroll
+        for (int f = 0; f < WF; ++f) apre[f] = p.a[((size_t)min(mt0, mtiles - 1) * p.nkc + min(wave + f * NW, p.nkc - 1)) * 64 + lane];
+        __builtin_amdgcn_sched_barrier(0);   // (the scheduler sinks the requests to their uses)
+    }
+    const int pitch = p.nkc * 64 + 16;
+    if constexpr (FUSED) {
+        // NW / M waves to a row (a power of two), rows in rounds of NW / wpr
+        int wpr = 1;
+        while (wpr * 2 * p.M <= NW) wpr *= 2;
+        const int rpr = NW / wpr, mine = wave & (wpr - 1), step = wpr * 256;
+        for (int r0 = 0; r0 < p.M; r0 += rpr) {
+            const int row = r0 + wave / wpr;
+            const bool live = row < p.M;
+            const size_t base = (size_t)((live ? row : 0) * p.s.ldx);
+            f32x4 v[NV];
+            float amax = 0.f;
+            if (live) {
+#pragma unroll
+                for (int i = 0; i < NV; ++i) v[i] = row_ld4(p.s, base, i * step + (mine * 64 + lane) * 4);
+#pragma unroll
+                for (int i = 0; i < NV; ++i) amax = row_max4(v[i], amax);
+                for (int c = NV * step + (mine * 64 + lane) * 4; c < p.K; c += step) amax = row_max4(row_ld4(p.s, base, c), amax);
+            }
+            amax = wave_max(amax);
+            if (wpr > 1) {   // (one round only)
+                if (lane == 0) red[wave] = amax;
+                __syncthreads();
+                for (int k = 0; k < wpr; ++k) amax = fmaxf(amax, red[(wave & ~(wpr - 1)) + k]);
+            }
+            float scale, inv;
+            row_scale(amax, scale, inv);
+            if (live) {
+                if (mine == 0 && lane == 0) fscale[row] = scale;
+                uint32_t* dst = reinterpret_cast<uint32_t*>(sm + row * pitch);
+                const int kpad = p.nkc * 64;
+#pragma unroll
+                for (int i = 0; i < NV; ++i) {
+                    const int c = i * step + (mine * 64 + lane) * 4;
+                    if (c < kpad) dst[c >> 2] = row_codes4(v[i], inv);
+                }
+                for (int c = NV * step + (mine * 64 + lane) * 4; c < kpad; c += step) dst[c >> 2] = row_codes4(row_ld4(p.s, base, c), inv);
+            }
+        }
+        __syncthreads();
+    }
     i32x4 acc[MT];
 #pragma unroll
     for (int m = 0; m < MT; ++m) acc[m] = i32x4{0, 0, 0, 0};
-    for (int kc = wave; kc < p.nkc; kc += NW) {
-        const u32x4 wf = __builtin_nontemporal_load(w + (size_t)kc * 64);
+    auto mul = [&](int kc, const u32x4& wk) {
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
-            const int mt = min(mt0 + m, mtiles - 1);
-            const u32x4 af = p.a[((size_t)mt * p.nkc + kc) * 64 + lane];
-            i8_mma(wf, af, acc[m]);
+            u32x4 af;   // (a row that does not exist only reaches outputs that are not stored)
+            if constexpr (FUSED) af = *reinterpret_cast<const u32x4*>(sm + (lane & 15) * pitch + kc * 64 + (lane >> 4) * 16);
+            else af = p.a[((size_t)min(mt0 + m, mtiles - 1) * p.nkc + kc) * 64 + lane];
+            i8_mma(wk, af, acc[m]);
         }
+    };
+#pragma unroll
+    for (int f = 0; f < WF; ++f)
+        if (wave + f * NW < p.nkc) {
+            if constexpr (AF) i8_mma(wf[f], apre[f], acc[0]);
+            else mul(wave + f * NW, wf[f]);
+        }
+    for (int k0 = wave + WF * NW; k0 < p.nkc; k0 += WF * NW) {
+#pragma unroll
+        for (int f = 0; f < WF; ++f) wf[f] = __builtin_nontemporal_load(w + (size_t)min(k0 + f * NW, p.nkc - 1) * 64);
+#pragma unroll
+        for (int f = 0; f < WF; ++f)
+            if (k0 + f * NW < p.nkc) mul(k0 + f * NW, wf[f]);
     }
 #pragma unroll
     for (int m = 0; m < MT; ++m) part[wave][m][lane] = acc[m];
     __syncthreads();
-    for (int e = threadIdx.x; e < MT * 64; e += NW * 64) {
-        const int m = e >> 6, ln = e & 63, row = (mt0 + m) * 16 + (ln & 15), col = nt * 16 + (ln >> 4) * 4;
-        if (row >= p.M) continue;
-        i32x4 s = part[0][m][ln];
+    for (int e = threadIdx.x; e < MT * 256; e += NW * 64) {   // one output per thread
+        const int m = e >> 8, n = e & 15, rl = (e >> 4) & 15, row = (mt0 + m) * 16 + rl, c = nt * 16 + n;
+        if (row >= p.M || c >= p.N) continue;
+        int sum = 0;
 #pragma unroll
-        for (int k = 1; k < NW; ++k) s += part[k][m][ln];
-        const float sa = p.a_scale[row];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int c = col + r;
-            if (c >= p.N) break;
-            float y = fmaf((float)s[r], sa * p.w_scale[c], p.bias != nullptr ? p.bias[c] : 0.f);
-            if (p.act == 1) y = i8_gelu(y);
-            if (p.residual != nullptr) y += p.residual[(size_t)row * p.N + c];
-            const size_t at = (size_t)(row * p.ldo) + c;
-            if (p.out_bf16) reinterpret_cast<bf16_t*>(p.out)[at] = f32_to_bf16(y);
-            else reinterpret_cast<float*>(p.out)[at] = y;
-        }
+        for (int k = 0; k < NW; ++k) sum += reinterpret_cast<const int*>(&part[k][m][(n >> 2) * 16 + rl])[n & 3];
+        const float sa = FUSED ? fscale[FUSED ? rl : 0] : p.a_scale[row];
+        float y = fmaf((float)sum, sa * p.w_scale[c], p.bias != nullptr ? p.bias[c] : 0.f);
+        if (p.act == 1) y = i8_gelu(y);
+        if (p.residual != nullptr) y += p.residual[(size_t)row * p.N + c];
+        const size_t at = (size_t)(row * p.ldo) + c;
+        if (p.out_bf16) reinterpret_cast<bf16_t*>(p.out)[at] = f32_to_bf16(y);
+        else reinterpret_cast<float*>(p.out)[at] = y;
     }
+}
+
+// Every workgroup of the fused form quantises the whole activation: while that is little.  Measured, us fused / two launches:
+// 1 x 4096 x 1024 4.3 / 6.0, 8 x 1536 x 1536 4.8 / 7.0, 16 x 4096 x 1024 5.3 / 6.3; 16 x 4608 x 1536 8.0 / 7.2, 16 x 1536 x 6144 22 / 9.3
+static bool i8_fused(int M, int K) { return M <= 16 && (long long)M * K <= 20480 && K <= 8192; }
+static size_t i8_codes_bytes(int M, int K) { return (size_t)((M + 15) / 16) * ((K + 63) / 64) * 1024; }
+
+extern "C" size_t acmi_linear_i8_work_bytes(int M, int K) {
+    return M <= 0 || K <= 0 || i8_fused(M, K) ? 0 : i8_codes_bytes(M, K) + (size_t)M * sizeof(float);
 }
 
 extern "C" int acmi_linear_i8(const acmi_linear_i8_desc* desc, void* stream) {
@@ -190,23 +313,45 @@ extern "C" int acmi_linear_i8(const acmi_linear_i8_desc* desc, void* stream) {
     ACMI_REQUIRE(d.out_dtype == ACMI_F32 || d.out_dtype == ACMI_BF16, "acmi_linear_i8: out_dtype %d", d.out_dtype);
     ACMI_REQUIRE(d.act == 0 || d.act == 1, "acmi_linear_i8: act %d", d.act);
     if (d.M == 0) return ACMI_OK;
-    ACMI_REQUIRE(d.a && d.a_scale && d.w && d.w_scale && d.out && d.ldo >= d.N, "acmi_linear_i8: null operand or ldo=%lld < N=%d", d.ldo, d.N);
-    ACMI_REQUIRE(((reinterpret_cast<size_t>(d.a) | reinterpret_cast<size_t>(d.w)) & 15) == 0, "acmi_linear_i8: codes must be 16-byte aligned");
+    ACMI_REQUIRE(d.w && d.w_scale && d.out && d.ldo >= d.N, "acmi_linear_i8: null operand or ldo=%lld < N=%d", d.ldo, d.N);
+    ACMI_REQUIRE((d.x != nullptr) != (d.a != nullptr && d.a_scale != nullptr), "acmi_linear_i8: either x or the quantised a, a_scale");
+    ACMI_REQUIRE(((reinterpret_cast<size_t>(d.a) | reinterpret_cast<size_t>(d.w) | reinterpret_cast<size_t>(d.work)) & 15) == 0,
+                 "acmi_linear_i8: codes and work must be 16-byte aligned");
     I8Args a = {};
     a.a = reinterpret_cast<const u32x4*>(d.a); a.a_scale = d.a_scale; a.w = reinterpret_cast<const u32x4*>(d.w); a.w_scale = d.w_scale;
     a.bias = d.bias; a.residual = d.residual; a.out = d.out; a.out_bf16 = d.out_dtype == ACMI_BF16; a.ldo = d.ldo;
     a.act = d.act; a.M = d.M; a.N = d.N; a.K = d.K; a.nkc = (d.K + 63) / 64;
     const int nt = (d.N + 15) / 16, mt = (d.M + 15) / 16;
     hipStream_t st = (hipStream_t)stream;
-    if (d.M > 64) {
+    if (d.x != nullptr) {
+        ACMI_REQUIRE(d.x_dtype == ACMI_F32 || d.x_dtype == ACMI_BF16, "acmi_linear_i8: x_dtype %d", d.x_dtype);
+        ACMI_REQUIRE(d.ldx >= d.K, "acmi_linear_i8: ldx=%lld < K=%d", d.ldx, d.K);
+        a.s = row_src(d.x, d.x_dtype, d.ldx, d.M, d.K);
+        if (i8_fused(d.M, d.K)) {
+            static const bool ok = hipFuncSetAttribute(reinterpret_cast<const void*>(&lin_i8_kernel<1, 8, true>), hipFuncAttributeMaxDynamicSharedMemorySize, 16 * (8192 + 16)) == hipSuccess;
+            ACMI_REQUIRE(ok, "acmi_linear_i8: cannot set the dynamic LDS limit");
+            hipLaunchKernelGGL((lin_i8_kernel<1, 8, true>), dim3(nt, 1), dim3(512), (size_t)16 * (a.nkc * 64 + 16), st, a);
+            return acmi_check_launch("lin_i8_kernel");
+        }
+        ACMI_REQUIRE(d.work != nullptr, "acmi_linear_i8: needs acmi_linear_i8_work_bytes bytes of work");
+        uint8_t* codes = reinterpret_cast<uint8_t*>(d.work);
+        float* scale = reinterpret_cast<float*>(codes + i8_codes_bytes(d.M, d.K));
+        if (int rc = launch_quant_rows(a.s, codes, scale, st)) return rc;
+        a.a = reinterpret_cast<const u32x4*>(codes); a.a_scale = scale;
+    }
+    // the tiled form once its 128 x 128 tiles give 3 of 8 CUs one; below, 64-row groups of the streaming form.  Measured with the
+    // quantiser, us tiled / streamed: 256 x 4608 x 1536 (72 tiles) 17.8 / 15.9, 1000 x 1000 x 1000 (64) 17.2 / 14.9;
+    // 1024 x 1536 x 6144 (96) 44.6 / 59.7, 512 x 4096 x 1024 (128) 16.5 / 19.9, 600 x 6144 x 1536 (240) 19.9 / 41.3
+    if (((d.M + 127) / 128) * ((d.N + 127) / 128) >= 96) {
         BigArgs b = {};
-        b.a = d.a; b.w = d.w; b.bias = d.bias; b.M = mt * 16; b.N = d.N; b.K = d.K; b.epi = ACMI_BIG_I8; b.act = d.act;
-        b.a_scale = d.a_scale; b.w_scale = d.w_scale; b.residual = d.residual; b.rows = d.M;
+        b.a = a.a; b.w = d.w; b.bias = d.bias; b.M = mt * 16; b.N = d.N; b.K = d.K; b.act = d.act;
+        b.a_scale = a.a_scale; b.w_scale = d.w_scale; b.residual = d.residual; b.rows = d.M;
         b.out = reinterpret_cast<float*>(d.out); b.out_bf16 = a.out_bf16; b.ldo64 = d.ldo;
         return acmi_launch_big_i8(b, st);
     }
-    if (mt == 1) hipLaunchKernelGGL((lin_i8_kernel<1, 8>), dim3(nt, 1), dim3(512), 0, st, a);
-    else if (mt == 2) hipLaunchKernelGGL((lin_i8_kernel<2, 8>), dim3(nt, 1), dim3(512), 0, st, a);
-    else hipLaunchKernelGGL((lin_i8_kernel<4, 8>), dim3(nt, 1), dim3(512), 0, st, a);
+    if (mt == 1 && a.nkc > 64) hipLaunchKernelGGL((lin_i8_kernel<1, 16, false>), dim3(nt, 1), dim3(1024), 0, st, a);
+    else if (mt == 1) hipLaunchKernelGGL((lin_i8_kernel<1, 8, false>), dim3(nt, 1), dim3(512), 0, st, a);
+    else if (mt == 2) hipLaunchKernelGGL((lin_i8_kernel<2, 8, false>), dim3(nt, 1), dim3(512), 0, st, a);
+    else hipLaunchKernelGGL((lin_i8_kernel<4, 8, false>), dim3(nt, (mt + 3) / 4), dim3(512), 0, st, a);
     return acmi_check_launch("lin_i8_kernel");
 }

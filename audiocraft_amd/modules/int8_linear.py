@@ -31,7 +31,7 @@ class Int8Linear:
         if activation not in self.ACTIVATIONS:
             raise ValueError(f"Int8Linear: activation {activation!r} ({', '.join(self.ACTIVATIONS)})")
         self.out_features, self.in_features = weight.shape
-        self.activation = activation
+        self.activation, self._act = activation, self.ACTIVATIONS[activation]
         w = weight.detach()
         self.codes, self.scale = _C.quantize_rows_i8(w if w.stride(1) == 1 else w.contiguous())
         self.bias = None
@@ -48,15 +48,15 @@ class Int8Linear:
         """x [..., K] f32 or bf16 -> [..., N] in x's dtype; residual [..., N] f32 is added last."""
         if x.shape[-1:] != (self.in_features,) or x.dtype not in _DTYPES or x.device != self.codes.device:
             raise ValueError(f"Int8Linear: x {tuple(x.shape)} {x.dtype} on {x.device}: [..., {self.in_features}] float32 or bfloat16 on {self.codes.device}")
-        rows = x.reshape(-1, self.in_features)
-        if rows.stride(1) != 1 or (rows.shape[0] > 1 and rows.stride(0) < self.in_features):
+        rows = x if x.dim() == 2 else x.reshape(-1, self.in_features)
+        M = rows.shape[0]
+        if rows.stride(1) != 1 or (M > 1 and rows.stride(0) < self.in_features):
             rows = rows.contiguous()
-        out = torch.empty(rows.shape[0], self.out_features, device=x.device, dtype=x.dtype)
+        out = torch.empty(M, self.out_features, device=x.device, dtype=x.dtype)
         if residual is not None:
             if residual.shape != x.shape[:-1] + (self.out_features,) or residual.dtype != torch.float32 or residual.device != x.device:
                 raise ValueError(f"Int8Linear: residual {tuple(residual.shape)} {residual.dtype}, expected float32 {tuple(x.shape[:-1]) + (self.out_features,)}")
             residual = residual.contiguous()
-        if rows.shape[0]:
-            a, a_scale = _C.quantize_rows_i8(rows)
-            _C.linear_i8(a, a_scale, self.codes, self.scale, out, self.in_features, self.bias, residual, self.ACTIVATIONS[self.activation])
-        return out.view(x.shape[:-1] + (self.out_features,))
+        if M:
+            _C.linear_i8(rows, self.codes, self.scale, out, self.bias, residual, self._act)
+        return out if x.dim() == 2 else out.view(x.shape[:-1] + (self.out_features,))

@@ -113,7 +113,8 @@ class KV8Cache:
             raise ValueError(f"KV8Cache.decode: k is {k.dtype}, v is {v.dtype}")
         lens, starts = self._words('decode', 'lens', lens, True), self._words('decode', 'starts', starts, False)
         out = torch.empty(self.rows, Hq, self.head_dim, device=self.device, dtype=q.dtype)
-        _C.kv8_attn(self.desc, q[:, None], out, lens, 1, True, self._past('decode', past_context), None, starts, k, v)
+        qs = q.stride()
+        _C.kv8_attn(self.desc, q, (qs[0], 0, qs[1]), 1, out, lens, 1, True, self._past('decode', past_context), None, starts, k, v)
         return out
 
     def attend(self, q: torch.Tensor, lens: torch.Tensor, causal: bool = True, past_context: int = 0,
@@ -133,7 +134,7 @@ class KV8Cache:
         q_lens = self._words('attend', 'q_lens', q_lens, False)
         out = torch.empty(self.rows, S, Hq, self.head_dim, device=self.device, dtype=q.dtype)
         if S:
-            _C.kv8_attn(self.desc, q, out, lens, 0, bool(causal), past, q_lens, starts)
+            _C.kv8_attn(self.desc, q, q.stride()[:3], S, out, lens, 0, bool(causal), past, q_lens, starts)
         return out
 
     def _q_heads(self, who: str, q: torch.Tensor, dims: int) -> int:

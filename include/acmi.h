@@ -693,14 +693,20 @@ int acmi_quantize_rows_i8(const void* x, int dtype, long long ldx, int R, int K,
 
 /* out[M, N] = act(a_scale[m] * w_scale[n] * sum_k a[m, k] w[n, k] + bias[n]) + residual[m, n]: the sum exact in 32-bit integers
  * (K <= 131072), one f32 product by a_scale * w_scale.  act: 0 none, 1 exact (erf) GELU.  bias [N] f32 or NULL; residual
- * [M, N] f32 (pitch N) or NULL.  out: row-major, pitch ldo, out_dtype f32 / bf16. */
+ * [M, N] f32 (pitch N) or NULL.  out: row-major, pitch ldo, out_dtype f32 / bf16.
+ * The activation is given quantised (a, a_scale) or as it is (x [M, K] in x_dtype, pitch ldx; a, a_scale NULL): its rows are then
+ * quantised by the same rule within the call, with acmi_linear_i8_work_bytes(M, K) bytes of 16-byte aligned `work` of this call
+ * alone (NULL where that is 0). */
 typedef struct {
     const void* a; const float* a_scale;
     const void* w; const float* w_scale;
     const float* bias; const float* residual;
     void* out; int out_dtype; long long ldo;
     int act, M, N, K;
+    const void* x; int x_dtype; long long ldx;
+    void* work;
 } acmi_linear_i8_desc;
+size_t acmi_linear_i8_work_bytes(int M, int K);
 int acmi_linear_i8(const acmi_linear_i8_desc* desc, void* stream);
 
 /* ------------------------------------------------------------------------------------------
