@@ -19,74 +19,130 @@ __device__ __forceinline__ void kv8_st(void* p, size_t i, int bf16, float v) {
 }
 // what the tail makes of a value
 __device__ __forceinline__ float kv8_round(float v, int bf16) { return bf16 ? bf16_to_f32(f32_to_bf16(v)) : v; }
-// place of token t inside a block's 64 bytes of one value feature (include/acmi.h)
-__device__ __forceinline__ int kv8_vplace(int t) { return ((t >> 2) & 3) * 16 + (t >> 4) * 4 + (t & 3); }
+
+// 16 consecutive features (16-byte aligned) -> f32
+__device__ __forceinline__ void kv8_ld16(const void* p, size_t i, int bf16, float (&x)[16]) {
+    if (bf16) {
+        const u32x4* q = reinterpret_cast<const u32x4*>(reinterpret_cast<const bf16_t*>(p) + i);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const u32x4 w = q[h];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                x[h * 8 + e * 2] = __uint_as_float(w[e] << 16);
+                x[h * 8 + e * 2 + 1] = __uint_as_float(w[e] & 0xffff0000u);
+            }
+        }
+    } else {
+        const f32x4* q = reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(p) + i);
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+            const f32x4 w = q[h];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[h * 4 + e] = w[e];
+        }
+    }
+}
+__device__ __forceinline__ void kv8_st16(void* p, size_t i, int bf16, const float (&x)[16]) {
+    if (bf16) {
+        u32x4* q = reinterpret_cast<u32x4*>(reinterpret_cast<bf16_t*>(p) + i);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            q[h] = u32x4{pack_bf16x2(x[h * 8], x[h * 8 + 1]), pack_bf16x2(x[h * 8 + 2], x[h * 8 + 3]), pack_bf16x2(x[h * 8 + 4], x[h * 8 + 5]),
+                         pack_bf16x2(x[h * 8 + 6], x[h * 8 + 7])};
+    } else {
+        f32x4* q = reinterpret_cast<f32x4*>(reinterpret_cast<float*>(p) + i);
+#pragma unroll
+        for (int h = 0; h < 4; ++h) q[h] = f32x4{x[h * 4], x[h * 4 + 1], x[h * 4 + 2], x[h * 4 + 3]};
+    }
+}
 
 // =====================================================================================================
 // quantising a block
 // =====================================================================================================
-// 256 threads, hd / 16 rounds: thread chunk e = 16 consecutive features of a token (keys), resp. the 16 tokens of one lane group of
-// a feature (values), so that every code store is 16 bytes.  get(which, token, feature) returns the value as the tail holds it.
-__device__ __forceinline__ uint32_t kv8_code(float x, float inv) { return (uint32_t)(uint8_t)(int8_t)(int)rintf(x * inv); }
-
+// The first 256 threads of a workgroup: a thread takes chunks of 16 features of a token, so loads and key codes are 16 bytes
+// wide; the value codes are turned feature-major through LDS, 4 tokens x 4 features (words) at a time.
 struct Kv8Scale { float scale, inv; };
-__device__ __forceinline__ Kv8Scale kv8_scale(float amax, bool bad) {   // bad: a NaN or an infinity among the values
+__device__ __forceinline__ Kv8Scale kv8_scale(float amax) {   // +infinity: a NaN or an infinity among the values
     Kv8Scale s;
-    if (bad) { s.scale = __uint_as_float(0x7fc00000u); s.inv = 0.f; }
+    if (amax == INFINITY) { s.scale = __uint_as_float(0x7fc00000u); s.inv = 0.f; }
     else if (amax < 7.52316384526264e-37f) { s.scale = 0.f; s.inv = 0.f; }   // 2^-120: 127 / amax stays finite above
     else { s.scale = __fdiv_rn(amax, 127.f); s.inv = __fdiv_rn(127.f, amax); }
     return s;
 }
-// (amax, bad) over the workgroup of 256 threads: +infinity marks bad
-__device__ __forceinline__ float kv8_block_max(float v, float* red) {
-    v = wave_max(v);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    __syncthreads();
-    return v;
+__device__ __forceinline__ float kv8_amax(float m, float v) {   // fmaxf would drop a NaN
+    const float a = fabsf(v);
+    return fmaxf(m, a <= 3.4028234663852886e38f ? a : INFINITY);
+}
+// 4 codes: the product rounded to f32, then to the nearest integer by adding 1.5 * 2^23 (ties to even; |product| <= 127 (1 + 2^-23)),
+// whose low byte it then is
+__device__ __forceinline__ uint32_t kv8_codes4(const float* x, float inv) {
+    uint32_t b[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) b[e] = __float_as_uint(x[e] * inv + 12582912.f);
+    return __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u) | __builtin_amdgcn_perm(b[3], b[2], 0x04000c0cu);
+}
+// 4 x 4 bytes: out word j = byte j of the four words
+__device__ __forceinline__ void kv8_transpose4(const uint32_t (&w)[4], uint32_t (&o)[4]) {
+    const uint32_t a = __builtin_amdgcn_perm(w[1], w[0], 0x05010400u), b = __builtin_amdgcn_perm(w[3], w[2], 0x05010400u);
+    const uint32_t c = __builtin_amdgcn_perm(w[1], w[0], 0x07030602u), d = __builtin_amdgcn_perm(w[3], w[2], 0x07030602u);
+    o[0] = __builtin_amdgcn_perm(b, a, 0x05040100u); o[1] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+    o[2] = __builtin_amdgcn_perm(d, c, 0x05040100u); o[3] = __builtin_amdgcn_perm(d, c, 0x07060302u);
 }
 
+template <int HD> struct Kv8QuantLds { uint32_t v[BLK * (HD / 4 + 1)]; float red[2][4]; };
+
+// load(part, token, feature, x): 16 features as the tail holds them.  Every thread of the workgroup has to come here.
 template <int HD, typename G>
-__device__ __forceinline__ void kv8_quantise_block(const acmi_kv8_cache& c, int row, int h, int blk, float* red, const G& get) {
-    constexpr int RND = HD >= 64 ? HD / 64 : 1;            // rounds of 256 chunks of 16 elements
-    constexpr int NCH = HD * BLK / 16;                     // chunks
-    const size_t hb = ((size_t)row * c.H + h) * c.nblk + blk;
-    float x[RND][16];
+__device__ __forceinline__ void kv8_quantise_block(const acmi_kv8_cache& c, size_t hb, Kv8QuantLds<HD>& sm, const G& load) {
+    constexpr int NCH = HD * BLK / 16, RND = NCH > 256 ? NCH / 256 : 1, PW = HD / 4 + 1;
+    float x[2][RND][16], amax[2] = {0.f, 0.f};
+    const int tid = threadIdx.x;
+#pragma unroll
+    for (int part = 0; part < 2; ++part)
+#pragma unroll
+        for (int q = 0; q < RND; ++q) {
+            const int ch = q * 256 + tid;
+            if (tid < 256 && ch < NCH) load(part, ch / (HD / 16), ch % (HD / 16) * 16, x[part][q]);
+        }
 #pragma unroll
     for (int part = 0; part < 2; ++part) {
-        float amax = 0.f;
 #pragma unroll
-        for (int q = 0; q < RND; ++q) {
-            const int ch = q * 256 + threadIdx.x;
-            if (ch < NCH) {
+        for (int q = 0; q < RND; ++q)
+            if (tid < 256 && q * 256 + tid < NCH) {
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    if (part == 0) x[q][j] = get(0, ch / (HD / 16), ch % (HD / 16) * 16 + j);
-                    else x[q][j] = get(1, (j >> 2) * 16 + (ch / HD) * 4 + (j & 3), ch % HD);
-                    // NaN: fmaxf would drop it
-                    amax = fmaxf(amax, isfinite(x[q][j]) ? fabsf(x[q][j]) : INFINITY);
-                }
+                for (int j = 0; j < 16; ++j) amax[part] = kv8_amax(amax[part], x[part][q][j]);
             }
-        }
-        amax = kv8_block_max(amax, red);
-        const Kv8Scale s = kv8_scale(amax, amax == INFINITY);
-        if (threadIdx.x == 0) (part == 0 ? c.k_scale : c.v_scale)[hb] = s.scale;
-        uint8_t* dst = reinterpret_cast<uint8_t*>(part == 0 ? c.k_codes : c.v_codes) + hb * (size_t)(BLK * HD);
+        amax[part] = wave_max(amax[part]);
+        if ((tid & 63) == 0 && tid < 256) sm.red[part][tid >> 6] = amax[part];
+    }
+    __syncthreads();
+    Kv8Scale s[2];
 #pragma unroll
-        for (int q = 0; q < RND; ++q) {
-            const int ch = q * 256 + threadIdx.x;
-            if (ch < NCH) {
-                u32x4 w;
+    for (int part = 0; part < 2; ++part) s[part] = kv8_scale(fmaxf(fmaxf(sm.red[part][0], sm.red[part][1]), fmaxf(sm.red[part][2], sm.red[part][3])));
+    if (tid == 0) { c.k_scale[hb] = s[0].scale; c.v_scale[hb] = s[1].scale; }
+    u32x4* kd = reinterpret_cast<u32x4*>(reinterpret_cast<uint8_t*>(c.k_codes) + hb * (size_t)(BLK * HD));
+    uint32_t* vd = reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(c.v_codes) + hb * (size_t)(BLK * HD));
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    w[k] = kv8_code(x[q][4 * k], s.inv) | kv8_code(x[q][4 * k + 1], s.inv) << 8 |
-                           kv8_code(x[q][4 * k + 2], s.inv) << 16 | kv8_code(x[q][4 * k + 3], s.inv) << 24;
-                const size_t at = part == 0 ? (size_t)ch * 16 : (size_t)(ch % HD) * BLK + (ch / HD) * 16;
-                *reinterpret_cast<u32x4*>(dst + at) = w;
-            }
+    for (int q = 0; q < RND; ++q) {
+        const int ch = q * 256 + tid;
+        if (tid < 256 && ch < NCH) {
+            kd[ch] = u32x4{kv8_codes4(x[0][q], s[0].inv), kv8_codes4(x[0][q] + 4, s[0].inv), kv8_codes4(x[0][q] + 8, s[0].inv), kv8_codes4(x[0][q] + 12, s[0].inv)};
+            uint32_t* l = sm.v + ch / (HD / 16) * PW + ch % (HD / 16) * 4;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) l[k] = kv8_codes4(x[1][q] + 4 * k, s[1].inv);
         }
     }
+    __syncthreads();
+    if (tid < 256)
+        for (int e = tid; e < HD / 4 * 16; e += 256) {   // (4 features f4, word w of their 64 bytes: tokens (w & 3) * 16 + (w >> 2) * 4 ..)
+            const int w = e & 15, f4 = e >> 4, t = (w & 3) * 16 + (w >> 2) * 4;
+            const uint32_t in[4] = {sm.v[t * PW + f4], sm.v[(t + 1) * PW + f4], sm.v[(t + 2) * PW + f4], sm.v[(t + 3) * PW + f4]};
+            uint32_t o[4];
+            kv8_transpose4(in, o);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) vd[(f4 * 4 + j) * 16 + w] = o[j];
+        }
 }
 
 // =====================================================================================================
@@ -103,7 +159,7 @@ struct Kv8StoreArgs {
 
 template <int HD>
 __global__ __launch_bounds__(256) void kv8_store_kernel(const Kv8StoreArgs p) {
-    __shared__ float red[4];
+    __shared__ Kv8QuantLds<HD> sm;
     const int j = blockIdx.x, h = blockIdx.y, row = blockIdx.z;
     const int cap = p.c.nblk * BLK, tb = p.c.tail_dtype == ACMI_BF16;
     const int start = p.start[row];
@@ -111,24 +167,32 @@ __global__ __launch_bounds__(256) void kv8_store_kernel(const Kv8StoreArgs p) {
     if (start < 0 || start >= cap || n <= 0) return;
     const int end = (int)min((long long)start + n, (long long)cap);
     const int b0 = start / BLK, b1 = end / BLK, blk = b0 + j, last = (end - 1) / BLK;
-    const size_t tbase = ((size_t)row * p.c.H + h) * (BLK * HD);
+    const size_t rh = (size_t)row * p.c.H + h, tbase = rh * (BLK * HD);
     const size_t kb = (size_t)(row * p.k_row + h * p.k_head), vb = (size_t)(row * p.v_row + h * p.v_head);
-    if (blk < b1) {
-        kv8_quantise_block<HD>(p.c, row, h, blk, red, [&](int part, int t, int d) {
+    auto fresh = [&](int part, int pos, int d, float (&x)[16]) {   // a token of this call, as the tail will hold it
+        kv8_ld16(part == 0 ? p.k : p.v, (part == 0 ? kb : vb) + (size_t)(pos - start) * (part == 0 ? p.k_tok : p.v_tok) + d, p.bf16, x);
+        if (tb && !p.bf16) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[e] = kv8_round(x[e], 1);
+        }
+    };
+    if (blk < b1)
+        kv8_quantise_block<HD>(p.c, rh * p.c.nblk + blk, sm, [&](int part, int t, int d, float (&x)[16]) {
             const int pos = blk * BLK + t;
-            if (pos < start) return kv8_ld(part == 0 ? p.c.k_tail : p.c.v_tail, tbase + t * HD + d, tb);
-            const size_t i = (part == 0 ? kb : vb) + (size_t)(pos - start) * (part == 0 ? p.k_tok : p.v_tok) + d;
-            return kv8_round(kv8_ld(part == 0 ? p.k : p.v, i, p.bf16), tb);
+            if (pos < start) kv8_ld16(part == 0 ? p.c.k_tail : p.c.v_tail, tbase + t * HD + d, tb, x);
+            else fresh(part, pos, d, x);
         });
-    }
     if (j == 0) {
         __syncthreads();   // the old tail has been read
         const int first = max(start, last * BLK);
-        for (int e = threadIdx.x; e < (end - first) * HD; e += 256) {
-            const int pos = first + e / HD, d = e % HD;
+        for (int e = threadIdx.x; e < (end - first) * (HD / 16); e += 256) {
+            const int pos = first + e / (HD / 16), d = e % (HD / 16) * 16;
             const size_t at = tbase + (size_t)(pos % BLK) * HD + d;
-            kv8_st(p.c.k_tail, at, tb, kv8_ld(p.k, kb + (size_t)(pos - start) * p.k_tok + d, p.bf16));
-            kv8_st(p.c.v_tail, at, tb, kv8_ld(p.v, vb + (size_t)(pos - start) * p.v_tok + d, p.bf16));
+            float x[16];
+            fresh(0, pos, d, x);
+            kv8_st16(p.c.k_tail, at, tb, x);
+            fresh(1, pos, d, x);
+            kv8_st16(p.c.v_tail, at, tb, x);
         }
     }
 }
@@ -138,32 +202,61 @@ __global__ __launch_bounds__(256) void kv8_store_kernel(const Kv8StoreArgs p) {
 // =====================================================================================================
 struct Kv8LoadArgs { acmi_kv8_cache c; const int* len; int T; void* k; void* v; int bf16; };
 
+__device__ __forceinline__ void kv8_st4(void* p, size_t i, int bf16, const f32x4& v) {
+    if (bf16) *reinterpret_cast<uint2*>(reinterpret_cast<bf16_t*>(p) + i) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+    else *reinterpret_cast<f32x4*>(reinterpret_cast<float*>(p) + i) = v;
+}
+__device__ __forceinline__ f32x4 kv8_values4(uint32_t w, float scale) {
+    return f32x4{(float)(int8_t)w * scale, (float)(int8_t)(w >> 8) * scale, (float)(int8_t)(w >> 16) * scale, (float)(int8_t)(w >> 24) * scale};
+}
+
+// one workgroup per (row, head, block): a thread takes 4 features of 4 tokens, so every store of a wave is whole rows; the value
+// codes come through LDS (pitch 17 words: conflict free) and are turned 4 x 4
 template <int HD>
 __global__ __launch_bounds__(256) void kv8_load_kernel(const Kv8LoadArgs p) {
+    __shared__ uint32_t sv[HD * 17];
     const int blk = blockIdx.x, h = blockIdx.y, row = blockIdx.z;
     const int tb = p.c.tail_dtype == ACMI_BF16;
-    const int len = min(p.len[row], p.c.nblk * BLK), last = max(len - 1, 0) / BLK;
-    const size_t rh = (size_t)row * p.c.H + h, hb = rh * p.c.nblk + blk;
-    const bool coded = blk < last;
-    const float ks = coded ? p.c.k_scale[hb] : 0.f, vs = coded ? p.c.v_scale[hb] : 0.f;
-    const int8_t* kc = reinterpret_cast<const int8_t*>(p.c.k_codes) + hb * (size_t)(BLK * HD);
-    const int8_t* vc = reinterpret_cast<const int8_t*>(p.c.v_codes) + hb * (size_t)(BLK * HD);
-    for (int e = threadIdx.x; e < BLK * HD; e += 256) {
-        const int t = e / HD, d = e % HD, pos = blk * BLK + t;
-        if (pos >= p.T) break;
-        float k = 0.f, v = 0.f;
-        if (pos < len) {
-            if (coded) {
-                k = (float)kc[t * HD + d] * ks;
-                v = (float)vc[d * BLK + kv8_vplace(t)] * vs;
-            } else {
-                k = kv8_ld(p.c.k_tail, rh * (BLK * HD) + t * HD + d, tb);
-                v = kv8_ld(p.c.v_tail, rh * (BLK * HD) + t * HD + d, tb);
+    const int len = max(0, min(p.len[row], p.c.nblk * BLK)), last = max(len - 1, 0) / BLK;
+    const size_t rh = (size_t)row * p.c.H + h, hb = rh * p.c.nblk + blk, ob = rh * p.T * HD;
+    if (blk < last) {
+        const float ks = p.c.k_scale[hb], vs = p.c.v_scale[hb];
+        const uint32_t* kc = reinterpret_cast<const uint32_t*>(reinterpret_cast<const uint8_t*>(p.c.k_codes) + hb * (size_t)(BLK * HD));
+        const u32x4* vc = reinterpret_cast<const u32x4*>(reinterpret_cast<const uint8_t*>(p.c.v_codes) + hb * (size_t)(BLK * HD));
+        for (int e = threadIdx.x; e < HD * 4; e += 256) {
+            const u32x4 w = vc[e];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sv[(e >> 2) * 17 + (e & 3) * 4 + j] = w[j];
+        }
+        for (int e = threadIdx.x; e < BLK * HD / 4; e += 256) {
+            const int pos = blk * BLK + e / (HD / 4);
+            if (pos < p.T) kv8_st4(p.k, ob + (size_t)pos * HD + e % (HD / 4) * 4, p.bf16, kv8_values4(kc[e], ks));
+        }
+        __syncthreads();
+        for (int e = threadIdx.x; e < HD / 4 * 16; e += 256) {
+            const int f4 = e % (HD / 4), w = e / (HD / 4), t = (w & 3) * 16 + (w >> 2) * 4;
+            const uint32_t in[4] = {sv[(f4 * 4) * 17 + w], sv[(f4 * 4 + 1) * 17 + w], sv[(f4 * 4 + 2) * 17 + w], sv[(f4 * 4 + 3) * 17 + w]};
+            uint32_t o[4];
+            kv8_transpose4(in, o);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int pos = blk * BLK + t + j;
+                if (pos < p.T) kv8_st4(p.v, ob + (size_t)pos * HD + f4 * 4, p.bf16, kv8_values4(o[j], vs));
             }
         }
-        const size_t at = (rh * p.T + pos) * HD + d;
-        kv8_st(p.k, at, p.bf16, k);
-        kv8_st(p.v, at, p.bf16, v);
+        return;
+    }
+    for (int e = threadIdx.x; e < BLK * HD / 4; e += 256) {   // the newest block, and what lies past it
+        const int t = e / (HD / 4), d = e % (HD / 4) * 4, pos = blk * BLK + t;
+        if (pos >= p.T) break;
+        f32x4 k = {0.f, 0.f, 0.f, 0.f}, v = k;
+        if (pos < len) {
+            const size_t at = rh * (BLK * HD) + t * HD + d;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) { k[j] = kv8_ld(p.c.k_tail, at + j, tb); v[j] = kv8_ld(p.c.v_tail, at + j, tb); }
+        }
+        kv8_st4(p.k, ob + (size_t)pos * HD + d, p.bf16, k);
+        kv8_st4(p.v, ob + (size_t)pos * HD + d, p.bf16, v);
     }
 }
 
@@ -177,8 +270,9 @@ __global__ __launch_bounds__(256) void kv8_load_kernel(const Kv8LoadArgs p) {
 // probabilities are already the B operand of the second product, whose A operand is the 16 value codes of the lane (the order
 // the codes are stored in).  Codes become f16 exactly: byte u = code + 128 under 0x64 is the f16 number 1024 + u, minus 1152.
 // Queries are f16 relative to a power of two near the row's largest feature; an f32 query is a pair of f16 (22 bits).
-// The block's scales multiply the scores and the block's part of O.  Probabilities are carried as 2^14 p (f16 then resolves
-// p down to 2^-38).  The newest block comes from the tail in f32 through the f32 matrix instruction, 16 tokens per wave.
+// Per score the vector ALU does a maximum, one multiply-add (scale, running maximum), one exp2 and half a conversion: the value
+// block's scale, relative to the largest one met (vref), sits in the exponent too, and the row sums come out of the matrix
+// cores (a product with ones), from the very f16 numbers that multiply the values.  Probabilities are carried as 2^14 p.
 struct Kv8AttnArgs {
     acmi_kv8_cache c;
     const void* q; int q_bf16; long long q_row, q_tok, q_head;
@@ -188,7 +282,7 @@ struct Kv8AttnArgs {
     const void* kn; const void* vn; int n_bf16; long long kn_row, kn_head, vn_row, vn_head;
     int complete;
     void* out; int out_mode, out_bf16, out_rbs, out_col0;
-    float* work; int splits;
+    float* work; int splits, tiles;
     float scale;
 };
 
@@ -203,158 +297,183 @@ __device__ __forceinline__ f16x8 kv8_cvt(uint32_t w0, uint32_t w1) {
     return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 __device__ __forceinline__ f16x2 kv8_pk(float a, float b) { return __builtin_convertvector(kv8_f32x2{a, b}, f16x2); }   // nearest even
+__device__ __forceinline__ f32x4 kv8_mma(const f16x8& a, const f16x8& b, const f32x4& c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 
 template <int HD> struct Kv8Geo {
     static constexpr int KW = HD >= 64 ? HD / 16 : 2;     // 32-bit words of K codes per lane and 16 tokens
     static constexpr int NK = KW / 2;                     // products of 32 features
     static constexpr int ND = HD / 16;                    // 16-feature tiles of O^T
 };
-// the feature that element j of a lane's B operand of product c stands for (hd 16: lanes kg >= 2 hold nothing)
-template <int HD> __device__ __forceinline__ int kv8_qdim(int kg, int c, int j) {
-    if (HD >= 64) return (c >> 1) * 64 + kg * 16 + (c & 1) * 8 + j;
-    return kg * 8 + j;
+// first of the 8 features that a lane's B operand of product k stands for (hd 16: lanes kg >= 2 hold nothing)
+template <int HD> __device__ __forceinline__ int kv8_qdim(int kg, int k) {
+    return HD >= 64 ? (k >> 1) * 64 + kg * 16 + (k & 1) * 8 : kg * 8;
 }
-
-template <int HD> struct Kv8Raw { uint32_t k[4][Kv8Geo<HD>::KW]; u32x4 v[Kv8Geo<HD>::ND]; float ks, vs; };
-
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+// K codes of 16 tokens (lane: token nl), V codes of 16 features (lane: feature nl)
 template <int HD, bool NT>
-__device__ __forceinline__ void kv8_fetch(const uint8_t* kc, const uint8_t* vc, const float* ks, const float* vs, int blk, Kv8Raw<HD>& r) {
-    const int lane = threadIdx.x & 63, nl = lane & 15, kg = lane >> 4;
-    const uint8_t* kb = kc + (size_t)blk * (BLK * HD);
-    const uint8_t* vb = vc + (size_t)blk * (BLK * HD);
-    auto ld16 = [](const uint8_t* p) { return NT ? __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p)) : *reinterpret_cast<const u32x4*>(p); };
-    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-    auto ld8 = [](const uint8_t* p) { return NT ? __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(p)) : *reinterpret_cast<const u32x2*>(p); };
-    r.ks = ks[blk]; r.vs = vs[blk];
+__device__ __forceinline__ void kv8_fetch_k(const uint8_t* kb, int tt, int nl, int kg, uint32_t (&w)[Kv8Geo<HD>::KW]) {
+    const uint8_t* row = kb + (tt * 16 + nl) * HD;
+    if constexpr (HD >= 64) {
 #pragma unroll
-    for (int tt = 0; tt < 4; ++tt) {
-        const uint8_t* row = kb + (tt * 16 + nl) * HD;
-        if constexpr (HD >= 64) {
+        for (int l = 0; l < HD / 64; ++l) {
+            const u32x4* q = reinterpret_cast<const u32x4*>(row + l * 64 + kg * 16);
+            const u32x4 v = NT ? __builtin_nontemporal_load(q) : *q;
 #pragma unroll
-            for (int l = 0; l < HD / 64; ++l) {
-                const u32x4 w = ld16(row + l * 64 + kg * 16);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) r.k[tt][l * 4 + e] = w[e];
-            }
-        } else {
-            const u32x2 w = ld8(row + (HD == 32 ? kg : (kg & 1)) * 8);
-            // hd 16: lanes kg >= 2 have no feature; their queries are 0, any code will do
-            r.k[tt][0] = w[0]; r.k[tt][1] = w[1];
+            for (int e = 0; e < 4; ++e) w[l * 4 + e] = v[e];
         }
+    } else {   // hd 16: the queries of lanes kg >= 2 are 0, any code will do
+        const u32x2* q = reinterpret_cast<const u32x2*>(row + (HD == 32 ? kg : (kg & 1)) * 8);
+        const u32x2 v = NT ? __builtin_nontemporal_load(q) : *q;
+        w[0] = v[0]; w[1] = v[1];
     }
-#pragma unroll
-    for (int i = 0; i < Kv8Geo<HD>::ND; ++i) r.v[i] = ld16(vb + (i * 16 + nl) * BLK + kg * 16);
 }
+template <bool NT>
+__device__ __forceinline__ u32x4 kv8_fetch_v(const uint8_t* vb, int i, int nl, int kg) {
+    const u32x4* q = reinterpret_cast<const u32x4*>(vb + (i * 16 + nl) * BLK + kg * 16);
+    return NT ? __builtin_nontemporal_load(q) : *q;
+}
+
+constexpr float KV8_PSHIFT = 14.f;
 
 // one column tile's state: lane (kg, n) belongs to column n
 template <int HD, bool QHL> struct Kv8Col {
     f16x8 qh[Kv8Geo<HD>::NK], ql[QHL ? Kv8Geo<HD>::NK : 1];
     float sfac;          // score factor: softmax scale * log2(e) * the query's power of two
     int lo, lim;         // positions [lo, lim) are seen
-    float m, l;
-    f32x4 o[Kv8Geo<HD>::ND];
+    float m, l;          // running maximum (log2 units); sum of 2^14 p
+    f32x4 o[Kv8Geo<HD>::ND];   // sum of 2^14 p v, in units of the wave's vref
 };
 
-constexpr float KV8_PSHIFT = 14.f;
-
-// scores s (log2 units, masked) of 16 * NT tokens -> probabilities * 2^14; returns the factor of the old sums
-template <int NTT>
-__device__ __forceinline__ float kv8_softmax(f32x4 (&s)[NTT], float& m, float& l, bool& none) {
-    float cmax = -INFINITY;
-#pragma unroll
-    for (int tt = 0; tt < NTT; ++tt)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) cmax = fmaxf(cmax, s[tt][r]);
-    cmax = fmaxf(cmax, __shfl_xor(cmax, 16, 64));
-    cmax = fmaxf(cmax, __shfl_xor(cmax, 32, 64));
-    none = cmax == -INFINITY;
-    const float m_new = fmaxf(m, cmax);
-    const float m_use = m_new == -INFINITY ? 0.f : m_new;
-    const float alpha = __builtin_amdgcn_exp2f(m - m_use);
-    const float base = m_use - KV8_PSHIFT;
-    float sum = 0.f;
-#pragma unroll
-    for (int tt = 0; tt < NTT; ++tt)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) { s[tt][r] = __builtin_amdgcn_exp2f(s[tt][r] - base); sum += s[tt][r]; }
-    l = fmaf(l, alpha, sum);
-    m = m_new;
-    return alpha;
-}
-
-// a block of codes into one column tile
-template <int HD, bool QHL, bool PHL>
-__device__ __forceinline__ void kv8_block(Kv8Col<HD, QHL>& c, const f16x8 (&kf)[4][Kv8Geo<HD>::NK], const f16x8 (&vf)[Kv8Geo<HD>::ND][2],
-                                          float ks, float vs, int t0) {
+// A block of 64 tokens into QB column tiles.  K(tt, k) / V(i, u): the fragments (LO: KL / VL their f16 remainders, for a tail in
+// f32); ks, vs: the block's scales; t0 its first position; after_k(): called once the K fragments have been used.
+template <int HD, bool QHL, bool PHL, bool LO, int QB, typename FK, typename FV, typename FKL, typename FVL, typename FA, typename FS>
+__device__ __forceinline__ void kv8_block(Kv8Col<HD, QHL> (&c)[QB], float& vref, const FK& K, const FV& V, const FKL& KL, const FVL& VL,
+                                          float ks, float vs, int t0, const FA& after_k, const FS& fix_scores) {
     constexpr int NK = Kv8Geo<HD>::NK, ND = Kv8Geo<HD>::ND;
     const int kg = (threadIdx.x & 63) >> 4;
-    f32x4 s[4];
-#pragma unroll
-    for (int tt = 0; tt < 4; ++tt) {
-        s[tt] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int k = 0; k < NK; ++k) {
-            s[tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[tt][k], c.qh[k], s[tt], 0, 0, 0);
-            if constexpr (QHL) s[tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[tt][k], c.ql[k], s[tt], 0, 0, 0);
-        }
-    }
-    const float f = ks * c.sfac;
-    const bool all = c.lo <= t0 && c.lim >= t0 + BLK;
-    if (__all(all)) {
-#pragma unroll
-        for (int tt = 0; tt < 4; ++tt)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) s[tt][r] *= f;
-    } else {
-#pragma unroll
-        for (int tt = 0; tt < 4; ++tt)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int t = t0 + tt * 16 + kg * 4 + r;
-                s[tt][r] = (t >= c.lo && t < c.lim) ? s[tt][r] * f : -INFINITY;
-            }
-    }
-    bool none;
-    const float alpha = kv8_softmax<4>(s, c.m, c.l, none);
-    const float vse = none ? 0.f : vs;   // (a block poisoned by a NaN leaves columns that do not see it alone)
-    f16x8 ph[2], pl[2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float a = s[2 * u + (e >> 1)][(e & 1) * 2], b = s[2 * u + (e >> 1)][(e & 1) * 2 + 1];
-            const f16x2 h = kv8_pk(a, b);
-            ph[u][2 * e] = h[0]; ph[u][2 * e + 1] = h[1];
-            if constexpr (PHL) {
-                const f16x2 w = kv8_pk(a - (float)h[0], b - (float)h[1]);
-                pl[u][2 * e] = w[0]; pl[u][2 * e + 1] = w[1];
-            }
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < ND; ++i) {
-        f32x4 t = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            t = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[i][u], ph[u], t, 0, 0, 0);
-            if constexpr (PHL) t = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[i][u], pl[u], t, 0, 0, 0);
-        }
-#pragma unroll
-        for (int r = 0; r < 4; ++r) c.o[i][r] = fmaf(t[r], vse, c.o[i][r] * alpha);
-    }
-}
-
-template <int HD>
-__device__ __forceinline__ void kv8_convert(const Kv8Raw<HD>& r, f16x8 (&kf)[4][Kv8Geo<HD>::NK], f16x8 (&vf)[Kv8Geo<HD>::ND][2]) {
+    const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+    f32x4 s[QB][4];
 #pragma unroll
     for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
-        for (int k = 0; k < Kv8Geo<HD>::NK; ++k) kf[tt][k] = kv8_cvt(r.k[tt][2 * k], r.k[tt][2 * k + 1]);
+        for (int k = 0; k < NK; ++k) {
+            const f16x8 kf = K(tt, k);
 #pragma unroll
-    for (int i = 0; i < Kv8Geo<HD>::ND; ++i) {
-        vf[i][0] = kv8_cvt(r.v[i][0], r.v[i][1]);
-        vf[i][1] = kv8_cvt(r.v[i][2], r.v[i][3]);
+            for (int g = 0; g < QB; ++g) {
+                s[g][tt] = kv8_mma(kf, c[g].qh[k], k == 0 ? zero : s[g][tt]);
+                if constexpr (QHL) s[g][tt] = kv8_mma(kf, c[g].ql[k], s[g][tt]);
+            }
+            if constexpr (LO) {
+                const f16x8 kl = KL(tt, k);
+#pragma unroll
+                for (int g = 0; g < QB; ++g) s[g][tt] = kv8_mma(kl, c[g].qh[k], s[g][tt]);
+            }
+        }
+    after_k();
+    fix_scores(s);
+    // the block's value scale relative to the largest one met; a scale of 0 belongs to codes that are all 0
+    const bool vnan = !(vs == vs);
+    if (vs > vref) {
+        const float f = vref > 0.f ? vref / vs : 0.f;
+#pragma unroll
+        for (int g = 0; g < QB; ++g)
+#pragma unroll
+            for (int i = 0; i < ND; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) c[g].o[i][r] *= f;
+        vref = vs;
     }
+    const float lr = (vs > 0.f && vs < vref) ? __builtin_amdgcn_logf(vs / vref) : 0.f;   // log2
+    const float ie = __builtin_amdgcn_exp2f(-lr);
+    f16x8 ph[QB][2], pl[QB][PHL ? 2 : 1];
+    bool moved = false;
+    float alpha[QB];
+#pragma unroll
+    for (int g = 0; g < QB; ++g) {
+        const bool all = c[g].lo <= t0 && c[g].lim >= t0 + BLK;
+        if (!__all(all)) {
+#pragma unroll
+            for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int t = t0 + tt * 16 + kg * 4 + r;
+                    s[g][tt][r] = (t >= c[g].lo && t < c[g].lim) ? s[g][tt][r] : -INFINITY;
+                }
+        }
+        float cmax = -INFINITY;
+#pragma unroll
+        for (int tt = 0; tt < 4; ++tt) cmax = fmaxf(cmax, fmaxf(fmaxf(s[g][tt][0], s[g][tt][1]), fmaxf(s[g][tt][2], s[g][tt][3])));
+        cmax = fmaxf(cmax, __shfl_xor(cmax, 16, 64));
+        cmax = fmaxf(cmax, __shfl_xor(cmax, 32, 64));
+        const bool none = cmax == -INFINITY;
+        // a column that sees nothing here keeps clear of the block's scales (which a NaN may have poisoned); a key scale of 0
+        // belongs to scores that are all 0
+        float f = ks * c[g].sfac;
+        f = (none || f == 0.f) ? 1.f : f;
+        const float m_new = fmaxf(c[g].m, cmax * f);
+        const float m_use = m_new == -INFINITY ? 0.f : m_new;
+        alpha[g] = __builtin_amdgcn_exp2f(c[g].m - m_use);
+        c[g].m = m_new;
+        moved |= alpha[g] != 1.f;
+        float base = lr + KV8_PSHIFT - m_use, f2 = f;
+        if (__any(fabsf(m_use) > 1024.f)) {
+            // large scores: the multiply-add below subtracts the ROUNDED maximum from the exact product (and the shift drowns in it);
+            // scaled and shifted apart, the largest score gives exactly 0
+#pragma unroll
+            for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s[g][tt][r] = s[g][tt][r] * f - m_use;
+            f2 = 1.f;
+            base = lr + KV8_PSHIFT;
+        }
+#pragma unroll
+        for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[g][tt][r] = __builtin_amdgcn_exp2f(fmaf(s[g][tt][r], f2, base));
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float a = s[g][2 * u + (e >> 1)][(e & 1) * 2], b = s[g][2 * u + (e >> 1)][(e & 1) * 2 + 1];
+                const f16x2 h = kv8_pk(a, b);
+                ph[g][u][2 * e] = h[0]; ph[g][u][2 * e + 1] = h[1];
+                if constexpr (PHL) {
+                    const f16x2 w = kv8_pk(a - (float)h[0], b - (float)h[1]);
+                    pl[g][u][2 * e] = w[0]; pl[g][u][2 * e + 1] = w[1];
+                }
+            }
+        // the row sums: every row of (ones) P is the sum over the block's tokens
+        const _Float16 o1 = (_Float16)1.f;
+        const f16x8 ones = {o1, o1, o1, o1, o1, o1, o1, o1};
+        f32x4 sum = kv8_mma(ones, ph[g][1], kv8_mma(ones, ph[g][0], zero));
+        if constexpr (PHL) sum = kv8_mma(ones, pl[g][1], kv8_mma(ones, pl[g][0], sum));
+        c[g].l = fmaf(c[g].l, alpha[g], sum[0] * ie);
+        if (vnan && !none) c[g].l = __uint_as_float(0x7fc00000u);
+    }
+    if (__any(moved)) {
+#pragma unroll
+        for (int g = 0; g < QB; ++g)
+#pragma unroll
+            for (int i = 0; i < ND; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) c[g].o[i][r] *= alpha[g];
+    }
+#pragma unroll
+    for (int i = 0; i < ND; ++i)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const f16x8 vf = V(i, u);
+#pragma unroll
+            for (int g = 0; g < QB; ++g) {
+                c[g].o[i] = kv8_mma(vf, ph[g][u], c[g].o[i]);
+                if constexpr (PHL) c[g].o[i] = kv8_mma(vf, pl[g][u], c[g].o[i]);
+            }
+            if constexpr (LO) {
+                const f16x8 vl = VL(i, u);
+#pragma unroll
+                for (int g = 0; g < QB; ++g) c[g].o[i] = kv8_mma(vl, ph[g][u], c[g].o[i]);
+            }
+        }
 }
 
 // what a column is: row geometry shared by both kernels
@@ -369,11 +488,35 @@ __device__ __forceinline__ Kv8RowInfo kv8_row(const Kv8AttnArgs& p, int row) {
     return r;
 }
 
-// column c of (row, cache head): visible range and query; cidx may lie past the last column
+// the query features of a lane: x[k][j] = feature kv8_qdim(kg, k) + j of column cidx (past the last column: the last query)
+template <int HD>
+__device__ __forceinline__ void kv8_load_q(const Kv8AttnArgs& p, int row, int kvh, int cidx, int kg, float (&x)[Kv8Geo<HD>::NK][8]) {
+    const int s = min(cidx / p.G, p.S - 1), g = cidx % p.G;
+    const size_t qb = (size_t)(row * p.q_row + (long long)s * p.q_tok + (long long)(kvh * p.G + g) * p.q_head);
+#pragma unroll
+    for (int k = 0; k < Kv8Geo<HD>::NK; ++k) {
+        const size_t at = qb + (HD == 16 ? (kg & 1) * 8 : kv8_qdim<HD>(kg, k));
+        if (p.q_bf16) {
+            const u32x4 w = *reinterpret_cast<const u32x4*>(reinterpret_cast<const bf16_t*>(p.q) + at);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { x[k][2 * e] = __uint_as_float(w[e] << 16); x[k][2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u); }
+        } else {
+            const f32x4* q = reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(p.q) + at);
+            const f32x4 a = q[0], b = q[1];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { x[k][e] = a[e]; x[k][4 + e] = b[e]; }
+        }
+    }
+    if (HD == 16 && kg >= 2) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[0][j] = 0.f;
+    }
+}
+
+// column cidx of (row, cache head): visible range and operands from its features
 template <int HD, bool QHL>
-__device__ __forceinline__ void kv8_column(const Kv8AttnArgs& p, const Kv8RowInfo& ri, int row, int kvh, int cidx, Kv8Col<HD, QHL>& c) {
-    const int kg = (threadIdx.x & 63) >> 4;
-    const int s = cidx / p.G, g = cidx - s * p.G;
+__device__ __forceinline__ void kv8_column(const Kv8AttnArgs& p, const Kv8RowInfo& ri, int cidx, const float (&x)[Kv8Geo<HD>::NK][8], Kv8Col<HD, QHL>& c) {
+    const int s = cidx / p.G;
     const bool live = s < ri.qlen;
     const int pos = ri.len - ri.qlen + s;
     // (columns without a query are never stored: they see everything, so that they do not keep a block on the masked path)
@@ -384,21 +527,16 @@ __device__ __forceinline__ void kv8_column(const Kv8AttnArgs& p, const Kv8RowInf
     c.m = -INFINITY; c.l = 0.f;
 #pragma unroll
     for (int i = 0; i < Kv8Geo<HD>::ND; ++i) c.o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float x[Kv8Geo<HD>::NK][8], amax = 0.f;
-    const long long qb = row * p.q_row + (long long)s * p.q_tok + (long long)(kvh * p.G + g) * p.q_head;
+    float amax = 0.f;
 #pragma unroll
     for (int k = 0; k < Kv8Geo<HD>::NK; ++k)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int d = kv8_qdim<HD>(kg, k, j);
-            x[k][j] = (live && d < HD) ? kv8_ld(p.q, (size_t)(qb + d), p.q_bf16) : 0.f;
-            amax = fmaxf(amax, isfinite(x[k][j]) ? fabsf(x[k][j]) : INFINITY);
-        }
+        for (int j = 0; j < 8; ++j) amax = kv8_amax(amax, x[k][j]);
     amax = fmaxf(amax, __shfl_xor(amax, 16, 64));
     amax = fmaxf(amax, __shfl_xor(amax, 32, 64));
-    // x = xn * 2^(e - 14) with the largest |xn| in [2^14, 2^15); a query with a NaN or an infinity gives NaN
+    // features times a power of two that brings the largest into [2^14, 2^15); a query with a NaN or an infinity gives NaN
     const int e = (amax > 0.f && amax < INFINITY) ? ilogbf(amax) : 0;
-    const float down = ldexpf(1.f, 14 - e < 127 ? 14 - e : 127);   // (features below 2^-113 all over: the product below stays exact)
+    const float down = ldexpf(1.f, min(14 - e, 127));
     c.sfac = amax == INFINITY ? __uint_as_float(0x7fc00000u) : p.scale * 1.4426950408889634f / down;
 #pragma unroll
     for (int k = 0; k < Kv8Geo<HD>::NK; ++k)
@@ -409,78 +547,6 @@ __device__ __forceinline__ void kv8_column(const Kv8AttnArgs& p, const Kv8RowInf
             c.qh[k][j] = h;
             if constexpr (QHL) c.ql[k][j] = (_Float16)(y - (float)h);
         }
-}
-
-// 16 tokens (slot0 ..) of the tail into one column tile, in f32.  last: the tail's block
-template <int HD, bool QHL>
-__device__ __forceinline__ void kv8_tail(const Kv8AttnArgs& p, const Kv8RowInfo& ri, int row, int kvh, int cidx, int slot0, Kv8Col<HD, QHL>& c) {
-    constexpr int ND = Kv8Geo<HD>::ND;
-    const int lane = threadIdx.x & 63, nl = lane & 15, kg = lane >> 4;
-    const int last = (ri.len - 1) / BLK, t0 = last * BLK + slot0, tb = p.c.tail_dtype == ACMI_BF16;
-    if (t0 >= ri.len) return;   // (wave uniform)
-    const size_t base = ((size_t)row * p.c.H + kvh) * (BLK * HD);
-    const int s_ = cidx / p.G, g = cidx - s_ * p.G;
-    const bool live = s_ < ri.qlen;
-    const long long qb = row * p.q_row + (long long)s_ * p.q_tok + (long long)(kvh * p.G + g) * p.q_head;
-    auto val = [&](int part, int t, int d) {   // t: position; past the row's length: 0
-        if (t >= ri.len) return 0.f;
-        if (ri.fresh && t == ri.len - 1) {
-            const long long i = (part == 0 ? row * p.kn_row + kvh * p.kn_head : row * p.vn_row + kvh * p.vn_head) + d;
-            return kv8_round(kv8_ld(part == 0 ? p.kn : p.vn, (size_t)i, p.n_bf16), tb);
-        }
-        return kv8_ld(part == 0 ? p.c.k_tail : p.c.v_tail, base + (size_t)(t - last * BLK) * HD + d, tb);
-    };
-    f32x4 s[1] = {f32x4{0.f, 0.f, 0.f, 0.f}};
-#pragma unroll
-    for (int i = 0; i < ND; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int d = i * 16 + kg * 4 + j;
-            const float a = val(0, t0 + nl, d);
-            const float b = live ? kv8_ld(p.q, (size_t)(qb + d), p.q_bf16) : 0.f;
-            s[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, s[0], 0, 0, 0);
-        }
-    const float f = p.scale * 1.4426950408889634f;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        const int t = t0 + kg * 4 + r;
-        s[0][r] = (t >= c.lo && t < c.lim) ? s[0][r] * f : -INFINITY;
-    }
-    bool none;
-    const float alpha = kv8_softmax<1>(s, c.m, c.l, none);
-    bool bad = false;   // a NaN or an infinity among the values: it must not meet the probability 0 of a column that does not see it
-#pragma unroll
-    for (int i = 0; i < ND; ++i) {
-        f32x4 t = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const float v = val(1, t0 + kg * 4 + r, i * 16 + nl);
-            const bool fin = isfinite(v);
-            bad |= !fin;
-            t = __builtin_amdgcn_mfma_f32_16x16x4f32(fin ? v : 0.f, s[0][r], t, 0, 0, 0);
-        }
-#pragma unroll
-        for (int r = 0; r < 4; ++r) c.o[i][r] = fmaf(c.o[i][r], alpha, t[r]);
-    }
-    if (__any(bad)) {   // those values one by one, each column for itself
-        for (int tok = 0; tok < 16; ++tok) {
-            float pr = 0.f;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const float x = __shfl(s[0][r], (tok >> 2) * 16 + nl, 64);
-                if ((tok & 3) == r) pr = x;
-            }
-            const int t = t0 + tok;
-            const bool seen = t >= c.lo && t < c.lim;
-#pragma unroll
-            for (int i = 0; i < ND; ++i)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const float v = val(1, t, i * 16 + kg * 4 + r);
-                    if (seen && !isfinite(v)) c.o[i][r] = fmaf(pr, v, c.o[i][r]);
-                }
-        }
-    }
 }
 
 // the blocks of codes a column tile visits, and how many workgroups share them
@@ -517,55 +583,197 @@ __device__ __forceinline__ void kv8_put4(const Kv8AttnArgs& p, int row, int s, i
     }
 }
 
-// ---- few queries: one workgroup per (column tile, cache head, row, split); its four waves take the blocks in turn and 16 tokens
-// of the tail each, and are joined through LDS
+// ---- few queries: one workgroup per (split, column tile of a cache head, row); its 8 waves take the blocks in turn, four of them
+// 16 tokens of the tail each, and are joined through LDS.  A wave keeps one block in flight: the next block's K is requested as
+// soon as this block's K has been multiplied, its V likewise.
+constexpr int KV8_NW = 8;
+
+// The tail's 16 tokens slot0 .. in f32, through the f32 matrix instruction, before any block of codes.
+template <int HD, bool QHL>
+__device__ __forceinline__ void kv8_tail16(const Kv8AttnArgs& p, const Kv8RowInfo& ri, int row, int kvh, int slot0,
+                                           const float (&x)[Kv8Geo<HD>::NK][8], Kv8Col<HD, QHL>& c, float& vref) {
+    constexpr int NK = Kv8Geo<HD>::NK, ND = Kv8Geo<HD>::ND;
+    const int lane = threadIdx.x & 63, nl = lane & 15, kg = lane >> 4;
+    const int last = (ri.len - 1) / BLK, t0 = last * BLK + slot0, tb = p.c.tail_dtype == ACMI_BF16;
+    const size_t base = ((size_t)row * p.c.H + kvh) * (BLK * HD);
+    const size_t kn0 = (size_t)(row * p.kn_row + kvh * p.kn_head), vn0 = (size_t)(row * p.vn_row + kvh * p.vn_head);
+    // keys: lane (kg, nl) the features of its queries' lanes, of token t0 + nl
+    float kx[NK][8];
+    {
+        const int t = t0 + nl;
+        const bool isnew = ri.fresh && t == ri.len - 1;
+        const void* src = isnew ? p.kn : p.c.k_tail;
+        const int sb = isnew ? p.n_bf16 : tb;
+        const size_t at = isnew ? kn0 : base + (size_t)(slot0 + nl) * HD;
+#pragma unroll
+        for (int k = 0; k < NK; ++k) {
+            const size_t i = at + (HD == 16 ? (kg & 1) * 8 : kv8_qdim<HD>(kg, k));
+            if (sb) {
+                const u32x4 w = *reinterpret_cast<const u32x4*>(reinterpret_cast<const bf16_t*>(src) + i);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) { kx[k][2 * e] = __uint_as_float(w[e] << 16); kx[k][2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u); }
+            } else {
+                const f32x4* q = reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(src) + i);
+                const f32x4 a = q[0], b = q[1];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) { kx[k][e] = a[e]; kx[k][4 + e] = b[e]; }
+                if (tb && isnew) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) kx[k][e] = kv8_round(kx[k][e], 1);
+                }
+            }
+        }
+        // (a token past the row's length: whatever the tail holds there only reaches scores that are masked)
+    }
+    // values: lane (kg, nl) feature i * 16 + nl of tokens t0 + kg * 4 + r
+    float vx[ND][4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const int t = t0 + kg * 4 + r;
+        const bool isnew = ri.fresh && t == ri.len - 1;
+        const void* src = isnew ? p.vn : p.c.v_tail;
+        const int sb = isnew ? p.n_bf16 : tb;
+        const size_t at = isnew ? vn0 : base + (size_t)(slot0 + kg * 4 + r) * HD;
+#pragma unroll
+        for (int i = 0; i < ND; ++i) {
+            const float v = kv8_ld(src, at + i * 16 + nl, sb);
+            vx[i][r] = t < ri.len ? (isnew ? kv8_round(v, tb) : v) : 0.f;
+        }
+    }
+    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < NK; ++k)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s = __builtin_amdgcn_mfma_f32_16x16x4f32(HD == 16 && kg >= 2 ? 0.f : kx[k][j], x[k][j], s, 0, 0, 0);
+    const float f = p.scale * 1.4426950408889634f;
+    float cmax = -INFINITY, vmax = 0.f;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const int t = t0 + kg * 4 + r;
+        s[r] = (t >= c.lo && t < c.lim && t < ri.len) ? s[r] * f : -INFINITY;
+        cmax = fmaxf(cmax, s[r]);
+    }
+    cmax = fmaxf(cmax, __shfl_xor(cmax, 16, 64));
+    cmax = fmaxf(cmax, __shfl_xor(cmax, 32, 64));
+    c.m = cmax;
+    const float top = cmax == -INFINITY ? 0.f : cmax;
+    float sum = 0.f;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) { s[r] = __builtin_amdgcn_exp2f(s[r] - top + KV8_PSHIFT); sum += s[r]; }
+    sum += __shfl_xor(sum, 16, 64);
+    sum += __shfl_xor(sum, 32, 64);
+    c.l = sum;
+    bool bad = false;   // a NaN or an infinity among the values: it must not meet the probability 0 of a column that does not see it
+#pragma unroll
+    for (int i = 0; i < ND; ++i) {
+        f32x4 t = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const float a = fabsf(vx[i][r]);
+            const bool fin = a <= 3.4028234663852886e38f;
+            bad |= !fin;
+            vmax = fmaxf(vmax, fin ? a : 0.f);
+            t = __builtin_amdgcn_mfma_f32_16x16x4f32(fin ? vx[i][r] : 0.f, s[r], t, 0, 0, 0);
+        }
+        c.o[i] = t;
+    }
+    if (__any(bad)) {   // those values one by one, each column for itself
+        for (int tok = 0; tok < 16; ++tok) {
+            float pr = 0.f;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float y = __shfl(s[r], (tok >> 2) * 16 + nl, 64);
+                if ((tok & 3) == r) pr = y;
+            }
+            const int t = t0 + tok;
+            const bool seen = t >= c.lo && t < c.lim && t < ri.len, isnew = ri.fresh && t == ri.len - 1;
+#pragma unroll
+            for (int i = 0; i < ND; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int d = i * 16 + kg * 4 + r;
+                    float v = isnew ? kv8_round(kv8_ld(p.vn, vn0 + d, p.n_bf16), tb) : kv8_ld(p.c.v_tail, base + (size_t)(slot0 + tok) * HD + d, tb);
+                    if (seen && !(fabsf(v) <= 3.4028234663852886e38f)) c.o[i][r] = fmaf(pr, v, c.o[i][r]);
+                }
+        }
+    }
+    // in units of a scale like the blocks': largest value / 127
+    vref = wave_max(vmax) * (1.f / 127.f);
+    if (vref < 7.52316384526264e-37f) vref = 7.52316384526264e-37f;
+    const float iv = 1.f / vref;
+#pragma unroll
+    for (int i = 0; i < ND; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) c.o[i][r] *= iv;
+}
+
 template <int HD, bool QHL, bool PHL>
-__global__ __launch_bounds__(256) void kv8_attn_split_kernel(const Kv8AttnArgs p) {
-    constexpr int ND = Kv8Geo<HD>::ND, PITCH = HD + 4;
-    __shared__ __attribute__((aligned(16))) float sm_o[4][16][PITCH];
-    __shared__ float sm_m[4][16], sm_l[4][16], red[4];
+__global__ __launch_bounds__(KV8_NW * 64) void kv8_attn_split_kernel(const Kv8AttnArgs p) {
+    constexpr int NK = Kv8Geo<HD>::NK, ND = Kv8Geo<HD>::ND, KW = Kv8Geo<HD>::KW, PITCH = HD + 4, NW = KV8_NW;
+    __shared__ __attribute__((aligned(16))) float sm_o[NW][16][PITCH];
+    __shared__ float sm_m[NW][16], sm_l[NW][16];
+    __shared__ Kv8QuantLds<HD> sm_q;
     const int split = blockIdx.x, row = blockIdx.z;
-    const int qtiles = (p.S * p.G + 15) / 16, kvh = blockIdx.y / qtiles, qt = blockIdx.y - kvh * qtiles;
+    const int qtiles = p.tiles, kvh = blockIdx.y / qtiles, qt = blockIdx.y - kvh * qtiles;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int nl = lane & 15, kg = lane >> 4;
+    float x[NK][8];
+    kv8_load_q<HD>(p, row, kvh, qt * 16 + nl, kg, x);
     const Kv8RowInfo ri = kv8_row(p, row);
     const Kv8Span sp = kv8_span(p, ri, qt * 16, min(qt * 16 + 16, p.S * p.G));
     if (split >= sp.eff) return;
     const int per = (sp.bt - sp.bf + sp.eff - 1) / sp.eff;
     const int s0 = sp.bf + split * per, s1 = min(sp.bt, s0 + per);
     const size_t rh = (size_t)row * p.c.H + kvh, hb = rh * p.c.nblk;
-    const uint8_t* kc = reinterpret_cast<const uint8_t*>(p.c.k_codes) + hb * (BLK * HD);
-    const uint8_t* vc = reinterpret_cast<const uint8_t*>(p.c.v_codes) + hb * (BLK * HD);
+    const uint8_t* kc = reinterpret_cast<const uint8_t*>(p.c.k_codes) + hb * (size_t)(BLK * HD);
+    const uint8_t* vc = reinterpret_cast<const uint8_t*>(p.c.v_codes) + hb * (size_t)(BLK * HD);
     const float* ks = p.c.k_scale + hb; const float* vs = p.c.v_scale + hb;
 
-    Kv8Col<HD, QHL> c;
-    Kv8Raw<HD> ra, rb;
-    int b = s0 + wave;
-    if (b < s1) kv8_fetch<HD, true>(kc, vc, ks, vs, b, ra);
-    kv8_column<HD, QHL>(p, ri, row, kvh, qt * 16 + nl, c);
-    const bool mine = split == sp.eff - 1;   // the split that owns the tail
-    if (mine && sp.tail) kv8_tail<HD, QHL>(p, ri, row, kvh, qt * 16 + nl, wave * 16, c);
-    f16x8 kf[4][Kv8Geo<HD>::NK], vf[ND][2];
-    while (b < s1) {   // two raw blocks in flight
-        if (b + 4 < s1) kv8_fetch<HD, true>(kc, vc, ks, vs, b + 4, rb);
-        kv8_convert<HD>(ra, kf, vf);
-        kv8_block<HD, QHL, PHL>(c, kf, vf, ra.ks, ra.vs, b * BLK);
-        b += 4;
-        if (b >= s1) break;
-        if (b + 4 < s1) kv8_fetch<HD, true>(kc, vc, ks, vs, b + 4, ra);
-        kv8_convert<HD>(rb, kf, vf);
-        kv8_block<HD, QHL, PHL>(c, kf, vf, rb.ks, rb.vs, b * BLK);
-        b += 4;
-    }
-    float l = c.l;
-    l += __shfl_xor(l, 16, 64);
-    l += __shfl_xor(l, 32, 64);
+    uint32_t kr[4][KW];
+    u32x4 vr[ND];
+    float ksn = 0.f, vsn = 0.f;
+    auto get_k = [&](int b) {
+        const uint8_t* kb = kc + (size_t)b * (BLK * HD);
 #pragma unroll
-    for (int i = 0; i < ND; ++i) *reinterpret_cast<f32x4*>(&sm_o[wave][nl][i * 16 + kg * 4]) = c.o[i];
-    if (kg == 0) { sm_m[wave][nl] = c.m; sm_l[wave][nl] = l; }
+        for (int tt = 0; tt < 4; ++tt) kv8_fetch_k<HD, true>(kb, tt, nl, kg, kr[tt]);
+        ksn = ks[b];
+        __builtin_amdgcn_sched_barrier(0);   // (the scheduler sinks requests to their uses)
+    };
+    auto get_v = [&](int b) {
+        const uint8_t* vb = vc + (size_t)b * (BLK * HD);
+#pragma unroll
+        for (int i = 0; i < ND; ++i) vr[i] = kv8_fetch_v<true>(vb, i, nl, kg);
+        vsn = vs[b];
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    int b = s0 + wave;
+    if (b < s1) { get_k(b); get_v(b); }
+    Kv8Col<HD, QHL> c[1];
+    kv8_column<HD, QHL>(p, ri, qt * 16 + nl, x, c[0]);
+    const bool mine = split == sp.eff - 1;   // the split that owns the tail
+    float vref = 0.f;
+    if (mine && sp.tail && wave < 4 && (ri.len - 1) / BLK * BLK + wave * 16 < ri.len) kv8_tail16<HD, QHL>(p, ri, row, kvh, wave * 16, x, c[0], vref);
+    while (b < s1) {
+        const int nb = b + NW;
+        const float kcur = ksn, vcur = vsn;
+        kv8_block<HD, QHL, PHL, false, 1>(c, vref, [&](int tt, int k) { return kv8_cvt(kr[tt][2 * k], kr[tt][2 * k + 1]); },
+                                          [&](int i, int u) { return kv8_cvt(vr[i][2 * u], vr[i][2 * u + 1]); }, 0, 0, kcur, vcur, b * BLK,
+                                          [&] { if (nb < s1) get_k(nb); }, [](auto&) {});
+        if (nb < s1) get_v(nb);
+        b = nb;
+    }
+    const float unit = vref * (1.f / 16384.f);
+#pragma unroll
+    for (int i = 0; i < ND; ++i) {
+        f32x4 o = c[0].o[i];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[r] *= unit;
+        *reinterpret_cast<f32x4*>(&sm_o[wave][nl][i * 16 + kg * 4]) = o;
+    }
+    if (kg == 0) { sm_m[wave][nl] = c[0].m; sm_l[wave][nl] = c[0].l * (1.f / 16384.f); }
     // the row's newest token and a block it completes (column tile 0 alone)
     if (mine && qt == 0 && ri.len > 0 && (ri.fresh || p.complete)) {
-        const int last = (ri.len - 1) / BLK, tb = p.c.tail_dtype == ACMI_BF16;
+        const int tb = p.c.tail_dtype == ACMI_BF16;
         const size_t tbase = rh * (BLK * HD);
         auto newest = [&](int part, int d) {
             const long long i = (part == 0 ? row * p.kn_row + kvh * p.kn_head : row * p.vn_row + kvh * p.vn_head) + d;
@@ -576,29 +784,33 @@ __global__ __launch_bounds__(256) void kv8_attn_split_kernel(const Kv8AttnArgs p
             kv8_st(p.c.k_tail, at, tb, newest(0, threadIdx.x));
             kv8_st(p.c.v_tail, at, tb, newest(1, threadIdx.x));
         }
-        if (ri.len % BLK == 0)
-            kv8_quantise_block<HD>(p.c, row, kvh, last, red, [&](int part, int t, int d) {
-                if (t == BLK - 1 && ri.fresh) return kv8_round(newest(part, d), tb);
-                return kv8_ld(part == 0 ? p.c.k_tail : p.c.v_tail, tbase + t * HD + d, tb);
+        if (ri.len % BLK == 0)   // (workgroup uniform)
+            kv8_quantise_block<HD>(p.c, hb + (ri.len - 1) / BLK, sm_q, [&](int part, int t, int d, float (&y)[16]) {
+                if (t == BLK - 1 && ri.fresh) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) y[e] = kv8_round(newest(part, d + e), tb);
+                } else {
+                    kv8_ld16(part == 0 ? p.c.k_tail : p.c.v_tail, tbase + t * HD + d, tb, y);
+                }
             });
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < 16 * HD / 4; e += 256) {
+    for (int e = threadIdx.x; e < 16 * HD / 4; e += NW * 64) {
         const int n = e / (HD / 4), d = e % (HD / 4) * 4, cidx = qt * 16 + n;
         if (cidx >= p.S * p.G) continue;
         float M = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) M = fmaxf(M, sm_m[w][n]);
+        for (int w = 0; w < NW; ++w) M = fmaxf(M, sm_m[w][n]);
         const float Mu = M == -INFINITY ? 0.f : M;
         f32x4 o = {0.f, 0.f, 0.f, 0.f};
         float den = 0.f;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
+        for (int w = 0; w < NW; ++w) {
             const float f = __builtin_amdgcn_exp2f(sm_m[w][n] - Mu);
-            const f32x4 x = *reinterpret_cast<const f32x4*>(&sm_o[w][n][d]);
+            const f32x4 y = *reinterpret_cast<const f32x4*>(&sm_o[w][n][d]);
             den = fmaf(f, sm_l[w][n], den);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) o[r] = fmaf(f, x[r], o[r]);
+            for (int r = 0; r < 4; ++r) o[r] = fmaf(f, y[r], o[r]);
         }
         if (sp.eff == 1) {
             const int s = cidx / p.G, g = cidx - s * p.G;
@@ -606,91 +818,275 @@ __global__ __launch_bounds__(256) void kv8_attn_split_kernel(const Kv8AttnArgs p
 #pragma unroll
             for (int r = 0; r < 4; ++r) o[r] = none ? 0.f : o[r] / den;
             kv8_put4(p, row, s, kvh * p.G + g, HD, d, o);
-        } else {   // partial: [row][cache head x tile][split][column][features | max | sum]
-            float* w = p.work + ((((size_t)row * gridDim.y + blockIdx.y) * p.splits + split) * 16 + n) * (HD + 4);
+        } else {   // partial: [row][cache head x tile][column][split][features | max | sum]
+            float* w = p.work + ((((size_t)row * gridDim.y + blockIdx.y) * 16 + n) * p.splits + split) * (HD + 4);
             *reinterpret_cast<f32x4*>(w + d) = o;
             if (d == 0) { w[HD] = M; w[HD + 1] = den; }
         }
     }
 }
 
-// joins the splits, in their order
+// joins the splits of one column: 256 / (HD / 4) groups of threads take them in turn, then meet in LDS in a fixed order
 template <int HD>
 __global__ __launch_bounds__(256) void kv8_attn_join_kernel(const Kv8AttnArgs p) {
-    const int row = blockIdx.y, qtiles = (p.S * p.G + 15) / 16, kvh = blockIdx.x / qtiles, qt = blockIdx.x - kvh * qtiles;
+    constexpr int F4 = HD / 4, NG = 256 / F4;
+    __shared__ __attribute__((aligned(16))) f32x4 so[NG][F4];
+    __shared__ float sd[NG];
+    const int n = blockIdx.x, row = blockIdx.z, qtiles = p.tiles, kvh = blockIdx.y / qtiles, qt = blockIdx.y - kvh * qtiles;
+    const int cidx = qt * 16 + n;
+    if (cidx >= p.S * p.G) return;
     const Kv8RowInfo ri = kv8_row(p, row);
     const Kv8Span sp = kv8_span(p, ri, qt * 16, min(qt * 16 + 16, p.S * p.G));
     if (sp.eff == 1) return;   // the split kernel has written it
-    const float* base = p.work + ((size_t)row * gridDim.x + blockIdx.x) * p.splits * 16 * (HD + 4);
-    for (int e = threadIdx.x; e < 16 * HD / 4; e += 256) {
-        const int n = e / (HD / 4), d = e % (HD / 4) * 4, cidx = qt * 16 + n;
-        if (cidx >= p.S * p.G) continue;
-        const float* w = base + n * (HD + 4);
-        float M = -INFINITY;
-        for (int k = 0; k < sp.eff; ++k) M = fmaxf(M, w[(size_t)k * 16 * (HD + 4) + HD]);
-        const float Mu = M == -INFINITY ? 0.f : M;
-        f32x4 o = {0.f, 0.f, 0.f, 0.f};
-        float den = 0.f;
-        for (int k = 0; k < sp.eff; ++k) {
-            const float* x = w + (size_t)k * 16 * (HD + 4);
-            const float f = __builtin_amdgcn_exp2f(x[HD] - Mu);
-            const f32x4 v = *reinterpret_cast<const f32x4*>(x + d);
-            den = fmaf(f, x[HD + 1], den);
+    const float* w = p.work + (((size_t)row * gridDim.y + blockIdx.y) * 16 + n) * p.splits * (HD + 4);
+    const int f4 = threadIdx.x % F4, grp = threadIdx.x / F4;
+    float M = -INFINITY;
+    for (int k = 0; k < sp.eff; ++k) M = fmaxf(M, w[(size_t)k * (HD + 4) + HD]);
+    const float Mu = M == -INFINITY ? 0.f : M;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    float den = 0.f;
+    for (int k = grp; k < sp.eff; k += NG) {
+        const float* y = w + (size_t)k * (HD + 4);
+        const float f = __builtin_amdgcn_exp2f(y[HD] - Mu);
+        const f32x4 v = *reinterpret_cast<const f32x4*>(y + f4 * 4);
+        den = fmaf(f, y[HD + 1], den);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) o[r] = fmaf(f, v[r], o[r]);
-        }
-        const int s = cidx / p.G, g = cidx - s * p.G;
-        const bool none = s >= ri.qlen || den == 0.f;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) o[r] = none ? 0.f : o[r] / den;
-        kv8_put4(p, row, s, kvh * p.G + g, HD, d, o);
+        for (int r = 0; r < 4; ++r) o[r] = fmaf(f, v[r], o[r]);
     }
+    so[grp][f4] = o;
+    if (f4 == 0) sd[grp] = den;
+    __syncthreads();
+    if (grp != 0) return;
+    for (int k = 1; k < NG; ++k) {
+        den += sd[k];
+        const f32x4 v = so[k][f4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[r] += v[r];
+    }
+    const int s = cidx / p.G, g = cidx - s * p.G;
+    const bool none = s >= ri.qlen || den == 0.f;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) o[r] = none ? 0.f : o[r] / den;
+    kv8_put4(p, row, s, kvh * p.G + g, HD, f4 * 4, o);
 }
 
-// ---- many queries: a wave owns QB column tiles and walks every block they see
+// ---- many queries: a workgroup's 4 waves own QB column tiles each and walk the blocks together.  Every wave converts a quarter of
+// the next block's codes to f16 fragments in LDS while this block is multiplied (two buffers, one barrier per block).  The tail
+// is staged the same way, relative to a power of two, as f16 (bf16 tails: exact) or a pair of f16 (f32 tails).
+// All workgroups of a (row, cache head) run on one XCD (workgroup i on XCD i % 8), so its codes are read once into one L2;
+// the longest (last) tiles first.
+template <int HD> struct Kv8ManyLds {
+    f16x8 k[2][4 * Kv8Geo<HD>::NK][64], v[2][2 * Kv8Geo<HD>::ND][64];
+    float red[2][4];
+    unsigned long long kbad, vbad;   // tokens of the tail that hold a NaN or an infinity
+};
+
+#ifndef KV8_WPE
+#define KV8_WPE 3
+#endif
 template <int HD, bool QHL, bool PHL, int QB>
-__global__ __launch_bounds__(256) void kv8_attn_many_kernel(const Kv8AttnArgs p) {
-    constexpr int ND = Kv8Geo<HD>::ND;
+__global__ __launch_bounds__(256, KV8_WPE) void kv8_attn_many_kernel(const Kv8AttnArgs p) {
+    constexpr int NK = Kv8Geo<HD>::NK, ND = Kv8Geo<HD>::ND, KW = Kv8Geo<HD>::KW, VT = ND >= 4 ? ND / 4 : 1;
+    __shared__ Kv8ManyLds<HD> sm;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int nl = lane & 15, kg = lane >> 4;
-    const int kvh = blockIdx.y, row = blockIdx.z, cols = p.S * p.G;
-    const int c0 = (blockIdx.x * 4 + wave) * 16 * QB;
-    if (c0 >= cols) return;
+    const int nl = lane & 15, kg = lane >> 4, cols = p.S * p.G;
+    const int li = blockIdx.x >> 3, grp = (blockIdx.x & 7) + 8 * (li / p.tiles), tile = p.tiles - 1 - li % p.tiles;
+    if (grp >= p.c.rows * p.c.H) return;
+    const int row = grp / p.c.H, kvh = grp - row * p.c.H;
+    const int w0 = tile * 64 * QB, c0 = w0 + wave * 16 * QB;   // first column of the workgroup, of the wave
     const Kv8RowInfo ri = kv8_row(p, row);
-    const Kv8Span sp = kv8_span(p, ri, c0, min(c0 + 16 * QB, cols));
+    const Kv8Span sp = kv8_span(p, ri, w0, min(w0 + 64 * QB, cols));
+    Kv8Span me = kv8_span(p, ri, min(c0, cols - 1), min(c0 + 16 * QB, cols));
+    if (c0 >= cols) { me.live = me.tail = false; me.bf = me.bt = 0; }
     Kv8Col<HD, QHL> c[QB];
 #pragma unroll
-    for (int g = 0; g < QB; ++g) kv8_column<HD, QHL>(p, ri, row, kvh, c0 + g * 16 + nl, c[g]);
-    if (sp.live) {
-        const size_t rh = (size_t)row * p.c.H + kvh, hb = rh * p.c.nblk;
-        const uint8_t* kc = reinterpret_cast<const uint8_t*>(p.c.k_codes) + hb * (BLK * HD);
-        const uint8_t* vc = reinterpret_cast<const uint8_t*>(p.c.v_codes) + hb * (BLK * HD);
+    for (int g = 0; g < QB; ++g) {
+        float x[NK][8];
+        kv8_load_q<HD>(p, row, kvh, c0 + g * 16 + nl, kg, x);
+        kv8_column<HD, QHL>(p, ri, c0 + g * 16 + nl, x, c[g]);
+    }
+    float vref = 0.f;
+    const size_t rh = (size_t)row * p.c.H + kvh, hb = rh * p.c.nblk;
+    const uint8_t* kc = reinterpret_cast<const uint8_t*>(p.c.k_codes) + hb * (size_t)(BLK * HD);
+    const uint8_t* vc = reinterpret_cast<const uint8_t*>(p.c.v_codes) + hb * (size_t)(BLK * HD);
+    uint32_t kr[KW];
+    u32x4 vr[VT];
+    float ksn = 0.f, vsn = 0.f;
+    auto request = [&](int b) {   // this wave's quarter: 16 tokens of K, VT feature tiles of V; the block's scales
+        ksn = __builtin_nontemporal_load(p.c.k_scale + hb + b);
+        vsn = __builtin_nontemporal_load(p.c.v_scale + hb + b);
+        kv8_fetch_k<HD, false>(kc + (size_t)b * (BLK * HD), wave, nl, kg, kr);
+#pragma unroll
+        for (int q = 0; q < VT; ++q)
+            if (wave + q * 4 < ND) vr[q] = kv8_fetch_v<false>(vc + (size_t)b * (BLK * HD), wave + q * 4, nl, kg);
+    };
+    auto stage = [&](int buf) {
+#pragma unroll
+        for (int k = 0; k < NK; ++k) sm.k[buf][wave * NK + k][lane] = kv8_cvt(kr[2 * k], kr[2 * k + 1]);
+#pragma unroll
+        for (int q = 0; q < VT; ++q)
+            if (wave + q * 4 < ND) {
+                sm.v[buf][(wave + q * 4) * 2][lane] = kv8_cvt(vr[q][0], vr[q][1]);
+                sm.v[buf][(wave + q * 4) * 2 + 1][lane] = kv8_cvt(vr[q][2], vr[q][3]);
+            }
+    };
+    auto none = [] {};
+    auto keep = [](auto&) {};
+    int buf = 0;
+    if (sp.bf < sp.bt) {
+        request(sp.bf);
+        stage(0);
+        __syncthreads();
         for (int b = sp.bf; b < sp.bt; ++b) {
-            Kv8Raw<HD> r;
-            kv8_fetch<HD, false>(kc, vc, p.c.k_scale + hb, p.c.v_scale + hb, b, r);
-            f16x8 kf[4][Kv8Geo<HD>::NK], vf[ND][2];
-            kv8_convert<HD>(r, kf, vf);
-#pragma unroll
-            for (int g = 0; g < QB; ++g) kv8_block<HD, QHL, PHL>(c[g], kf, vf, r.ks, r.vs, b * BLK);
+            const bool more = b + 1 < sp.bt;
+            const float ks = ksn, vs = vsn;
+            if (more) request(b + 1);
+            __builtin_amdgcn_sched_barrier(0);
+            if (b >= me.bf && b < me.bt)
+                kv8_block<HD, QHL, PHL, false, QB>(c, vref, [&](int tt, int k) { return sm.k[buf][tt * NK + k][lane]; },
+                                                   [&](int i, int u) { return sm.v[buf][i * 2 + u][lane]; }, 0, 0,
+                                                   ks, vs, b * BLK, none, keep);
+            if (more) stage(buf ^ 1);
+            __syncthreads();
+            buf ^= 1;
         }
-        if (sp.tail)
-            for (int t = 0; t < 4; ++t)
+    }
+    if (sp.tail) {   // (workgroup uniform)
+        const int tb = p.c.tail_dtype == ACMI_BF16, t0 = (ri.len - 1) / BLK * BLK, nt = ri.len - t0;
+        const size_t base = rh * (BLK * HD);
+        float kx[NK][8], vx[VT][16], ka = 0.f, va = 0.f;
+        bool kb = false;
+        unsigned vb = 0;
+        if (threadIdx.x == 0) { sm.kbad = 0; sm.vbad = 0; }
+        const int tk = wave * 16 + nl;   // this lane's token of K
 #pragma unroll
-                for (int g = 0; g < QB; ++g) kv8_tail<HD, QHL>(p, ri, row, kvh, c0 + g * 16 + nl, t * 16, c[g]);
+        for (int k = 0; k < NK; ++k)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int d = HD == 16 ? (kg & 1) * 8 + j : kv8_qdim<HD>(kg, k) + j;
+                float v = tk < nt ? kv8_ld(p.c.k_tail, base + (size_t)tk * HD + d, tb) : 0.f;
+                const float a = fabsf(v);
+                if (!(a <= 3.4028234663852886e38f)) { kb = true; v = 0.f; }
+                kx[k][j] = v;
+                ka = fmaxf(ka, fabsf(v));
+            }
+#pragma unroll
+        for (int q = 0; q < VT; ++q)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const int t = (j >> 2) * 16 + kg * 4 + (j & 3), i = wave + q * 4;
+                float v = (i < ND && t < nt) ? kv8_ld(p.c.v_tail, base + (size_t)t * HD + i * 16 + nl, tb) : 0.f;
+                const float a = fabsf(v);
+                if (!(a <= 3.4028234663852886e38f)) { vb |= 1u << j; v = 0.f; }
+                vx[q][j] = v;
+                va = fmaxf(va, fabsf(v));
+            }
+        ka = wave_max(ka);
+        va = wave_max(va);
+        if (lane == 0) { sm.red[0][wave] = ka; sm.red[1][wave] = va; }
+        __syncthreads();
+        if (kb) atomicOr(&sm.kbad, 1ull << tk);
+        if (vb != 0) {
+            unsigned long long m = 0;
+            for (int j = 0; j < 16; ++j)
+                if (vb >> j & 1) m |= 1ull << ((j >> 2) * 16 + kg * 4 + (j & 3));
+            atomicOr(&sm.vbad, m);
+        }
+        ka = fmaxf(fmaxf(sm.red[0][0], sm.red[0][1]), fmaxf(sm.red[0][2], sm.red[0][3]));
+        va = fmaxf(fmaxf(sm.red[1][0], sm.red[1][1]), fmaxf(sm.red[1][2], sm.red[1][3]));
+        const float ku = ldexpf(1.f, min(14 - (ka > 0.f ? ilogbf(ka) : 0), 126)), vu = ldexpf(1.f, min(14 - (va > 0.f ? ilogbf(va) : 0), 126));
+#pragma unroll
+        for (int k = 0; k < NK; ++k) {
+            f16x8 h, l;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float y = kx[k][j] * ku;
+                h[j] = (_Float16)y;
+                l[j] = (_Float16)(y - (float)h[j]);
+            }
+            sm.k[0][wave * NK + k][lane] = h;
+            if (!tb) sm.k[1][wave * NK + k][lane] = l;
+        }
+#pragma unroll
+        for (int q = 0; q < VT; ++q)
+            if (wave + q * 4 < ND)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    f16x8 h, l;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float y = vx[q][u * 8 + j] * vu;
+                        h[j] = (_Float16)y;
+                        l[j] = (_Float16)(y - (float)h[j]);
+                    }
+                    sm.v[0][(wave + q * 4) * 2 + u][lane] = h;
+                    if (!tb) sm.v[1][(wave + q * 4) * 2 + u][lane] = l;
+                }
+        __syncthreads();
+        if (me.tail) {
+            // tokens past the row's length are masked for every stored column by its limit; a column without a query may count them
+            const unsigned long long kbad = sm.kbad, vbad = sm.vbad;
+            const float ks = 1.f / ku, vs = 1.f / vu;
+            // a score from the features themselves, for the tokens whose f16 fragments leave a value out
+            auto dot = [&](int g, int t) {
+                const int cidx = min(c0 + g * 16 + nl, cols - 1);
+                const size_t qb = (size_t)(row * p.q_row + (long long)(cidx / p.G) * p.q_tok + (long long)(kvh * p.G + cidx % p.G) * p.q_head);
+                float x = 0.f;
+#pragma unroll 1
+                for (int d = 0; d < HD; ++d) x = fmaf(kv8_ld(p.q, qb + d, p.q_bf16), kv8_ld(p.c.k_tail, base + (size_t)t * HD + d, tb), x);
+                return x;
+            };
+            auto fix = [&](f32x4 (&s)[QB][4]) {
+                if (kbad == 0) return;
+#pragma unroll 1
+                for (int t = 0; t < nt; ++t) {
+                    if (!(kbad >> t & 1)) continue;
+#pragma unroll
+                    for (int g = 0; g < QB; ++g) {
+                        const float x = dot(g, t);   // an infinity or a NaN, whatever its factor
+#pragma unroll
+                        for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r)
+                                if (tt * 16 + kg * 4 + r == t) s[g][tt][r] = x;
+                    }
+                }
+            };
+            auto K = [&](int tt, int k) { return sm.k[0][tt * NK + k][lane]; };
+            auto V = [&](int i, int u) { return sm.v[0][i * 2 + u][lane]; };
+            auto KL = [&](int tt, int k) { return sm.k[1][tt * NK + k][lane]; };
+            auto VL = [&](int i, int u) { return sm.v[1][i * 2 + u][lane]; };
+            if (tb) kv8_block<HD, QHL, PHL, false, QB>(c, vref, K, V, 0, 0, ks, vs, t0, none, fix);
+            else kv8_block<HD, QHL, PHL, true, QB>(c, vref, K, V, KL, VL, ks, vs, t0, none, fix);
+#pragma unroll 1
+            for (int t = 0; t < (vbad != 0 ? nt : 0); ++t) {   // values that are not finite one by one, each column for itself
+                if (!(vbad >> t & 1)) continue;
+#pragma unroll
+                for (int g = 0; g < QB; ++g) {
+                    const float pr = __builtin_amdgcn_exp2f(dot(g, t) * (p.scale * 1.4426950408889634f) - c[g].m + KV8_PSHIFT);
+                    const bool seen = t0 + t >= c[g].lo && t0 + t < c[g].lim;
+#pragma unroll
+                    for (int i = 0; i < ND; ++i)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const float v = kv8_ld(p.c.v_tail, base + (size_t)t * HD + i * 16 + kg * 4 + r, tb);
+                            if (seen && !(fabsf(v) <= 3.4028234663852886e38f)) c[g].o[i][r] = fmaf(pr, v, c[g].o[i][r]);
+                        }
+                }
+            }
+        }
     }
 #pragma unroll
     for (int g = 0; g < QB; ++g) {
-        float l = c[g].l;
-        l += __shfl_xor(l, 16, 64);
-        l += __shfl_xor(l, 32, 64);
         const int cidx = c0 + g * 16 + nl, s = cidx / p.G, h = cidx - s * p.G;
         if (cidx >= cols) continue;
-        const bool none = s >= ri.qlen || l == 0.f;
+        const bool zero = s >= ri.qlen || c[g].l == 0.f;
+        const float inv = vref / c[g].l;
 #pragma unroll
         for (int i = 0; i < ND; ++i) {
             f32x4 o;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) o[r] = none ? 0.f : c[g].o[i][r] / l;
+            for (int r = 0; r < 4; ++r) o[r] = zero ? 0.f : c[g].o[i][r] * inv;
             kv8_put4(p, row, s, kvh * p.G + h, HD, i * 16 + kg * 4, o);
         }
     }
@@ -709,6 +1105,9 @@ static int kv8_check(const acmi_kv8_cache* c, const char* who) {
     return ACMI_OK;
 }
 static bool kv8_dtype_ok(int d) { return d == ACMI_F32 || d == ACMI_BF16; }
+static bool kv8_rows_ok(const void* p, int es, long long a, long long b, long long c) {
+    return ((reinterpret_cast<size_t>(p) | (size_t)(a * es) | (size_t)(b * es) | (size_t)(c * es)) & 15) == 0;
+}
 
 #define KV8_HD_SWITCH(hd, CASE) \
     switch (hd) {               \
@@ -725,6 +1124,9 @@ extern "C" int acmi_kv8_store(const acmi_kv8_cache* cache, const acmi_kv8_store_
     ACMI_REQUIRE(desc->L >= 0 && desc->L <= (1 << 30) && kv8_dtype_ok(desc->dtype), "acmi_kv8_store: L=%d dtype=%d", desc->L, desc->dtype);
     if (desc->L == 0) return ACMI_OK;
     ACMI_REQUIRE(desc->k && desc->v, "acmi_kv8_store: null k or v");
+    const int es = desc->dtype == ACMI_BF16 ? 2 : 4;
+    ACMI_REQUIRE(kv8_rows_ok(desc->k, es, desc->k_row, desc->k_tok, desc->k_head) && kv8_rows_ok(desc->v, es, desc->v_row, desc->v_tok, desc->v_head),
+                 "acmi_kv8_store: k and v need 16-byte aligned rows");
     Kv8StoreArgs a = {};
     a.c = *cache; a.k = desc->k; a.v = desc->v; a.bf16 = desc->dtype == ACMI_BF16;
     a.k_row = desc->k_row; a.k_tok = desc->k_tok; a.k_head = desc->k_head;
@@ -784,6 +1186,10 @@ extern "C" int acmi_kv8_attn(const acmi_kv8_cache* cache, const acmi_kv8_attn_de
     ACMI_REQUIRE((d.k_new == nullptr) == (d.v_new == nullptr), "acmi_kv8_attn: k_new and v_new come together");
     ACMI_REQUIRE((d.k_new == nullptr && !d.complete) || (d.S == 1 && d.causal), "acmi_kv8_attn: a new token needs S = 1 and causal");
     ACMI_REQUIRE(d.k_new == nullptr || kv8_dtype_ok(d.new_dtype), "acmi_kv8_attn: new_dtype %d", d.new_dtype);
+    ACMI_REQUIRE(kv8_rows_ok(d.q, d.q_dtype == ACMI_BF16 ? 2 : 4, d.q_row, d.S > 1 ? d.q_tok : 0, d.q_head), "acmi_kv8_attn: q needs 16-byte aligned rows");
+    ACMI_REQUIRE(d.k_new == nullptr || (kv8_rows_ok(d.k_new, d.new_dtype == ACMI_BF16 ? 2 : 4, d.kn_row, d.kn_head, 0) &&
+                                        kv8_rows_ok(d.v_new, d.new_dtype == ACMI_BF16 ? 2 : 4, d.vn_row, d.vn_head, 0)),
+                 "acmi_kv8_attn: k_new and v_new need 16-byte aligned rows");
     ACMI_REQUIRE(d.past_context >= 0 && (d.past_context == 0 || d.causal), "acmi_kv8_attn: past_context=%d needs causal", d.past_context);
     Kv8AttnArgs a = {};
     a.c = *cache; a.q = d.q; a.q_bf16 = d.q_dtype == ACMI_BF16; a.q_row = d.q_row; a.q_tok = d.q_tok; a.q_head = d.q_head;
@@ -800,7 +1206,7 @@ extern "C" int acmi_kv8_attn(const acmi_kv8_cache* cache, const acmi_kv8_attn_de
                      "acmi_kv8_attn: tiled output placement col0=%d rbs=%d does not hold %d columns", d.out_col0, a.out_rbs, d.Hq * cache->hd);
     a.scale = 1.0f / sqrtf((float)cache->hd);
     const bool out_f32 = d.out_mode == ACMI_OUT_F32 || (d.out_mode == ACMI_OUT_TILED && d.out_dtype == ACMI_F32);
-    const bool qhl = d.q_dtype == ACMI_F32;   // (a bf16 query is one f16 exactly)
+    const bool qhl = d.q_dtype == ACMI_F32 || out_f32;   // (a bf16 query is one f16 exactly)
     hipStream_t st = (hipStream_t)stream;
     const int qtiles = (d.S * a.G + 15) / 16;
     if (kv8_few(d.S, a.G)) {
@@ -810,32 +1216,37 @@ extern "C" int acmi_kv8_attn(const acmi_kv8_cache* cache, const acmi_kv8_attn_de
                      "acmi_kv8_attn: needs acmi_kv8_attn_work_floats floats of 16-byte aligned work");
         ACMI_REQUIRE((long long)cache->H * qtiles <= 65535, "acmi_kv8_attn: %d heads x %d column tiles", cache->H, qtiles);
         const dim3 grid(a.splits, cache->H * qtiles, cache->rows);
-#define KV8_SPLIT(HDv, Q, P) hipLaunchKernelGGL((kv8_attn_split_kernel<HDv, Q, P>), grid, dim3(256), 0, st, a)
-#define KV8_CASE(HDv)                                                       \
-    case HDv:                                                               \
-        if (qhl) { if (out_f32) KV8_SPLIT(HDv, true, true); else KV8_SPLIT(HDv, true, false); }   \
-        else { if (out_f32) KV8_SPLIT(HDv, false, true); else KV8_SPLIT(HDv, false, false); }     \
+        a.tiles = qtiles;
+#define KV8_SPLIT(HDv, Q, P) hipLaunchKernelGGL((kv8_attn_split_kernel<HDv, Q, P>), grid, dim3(KV8_NW * 64), 0, st, a)
+#define KV8_CASE(HDv)                                            \
+    case HDv:                                                    \
+        if (out_f32) KV8_SPLIT(HDv, true, true);                 \
+        else if (qhl) KV8_SPLIT(HDv, true, false);               \
+        else KV8_SPLIT(HDv, false, false);                       \
         break;
         KV8_HD_SWITCH(cache->hd, KV8_CASE)
 #undef KV8_CASE
 #undef KV8_SPLIT
         if (int rc = acmi_check_launch("kv8_attn_split_kernel")) return rc;
         if (a.splits == 1) return ACMI_OK;
-        const dim3 jgrid(cache->H * qtiles, cache->rows);
+        const dim3 jgrid(min(d.S * a.G, 16), cache->H * qtiles, cache->rows);
 #define KV8_CASE(HDv) case HDv: hipLaunchKernelGGL((kv8_attn_join_kernel<HDv>), jgrid, dim3(256), 0, st, a); break;
         KV8_HD_SWITCH(cache->hd, KV8_CASE)
 #undef KV8_CASE
         return acmi_check_launch("kv8_attn_join_kernel");
     }
-#define KV8_MANY(HDv, Q, P, QBv)                                                                                             \
-    hipLaunchKernelGGL((kv8_attn_many_kernel<HDv, Q, P, QBv>), dim3((qtiles + 4 * QBv - 1) / (4 * QBv), cache->H, cache->rows), dim3(256), 0, st, a)
-#define KV8_CASE(HDv)                                                       \
-    case HDv: {                                                             \
-        constexpr int QBv = HDv <= 64 ? 2 : 1;                              \
-        if (qhl) { if (out_f32) KV8_MANY(HDv, true, true, QBv); else KV8_MANY(HDv, true, false, QBv); }   \
-        else { if (out_f32) KV8_MANY(HDv, false, true, QBv); else KV8_MANY(HDv, false, false, QBv); }     \
-        break;                                                              \
-    }
+    const int QB = cache->hd <= 64 ? 2 : 1;   // (hd 128: two column tiles do not fit the registers)
+    a.tiles = (qtiles + 4 * QB - 1) / (4 * QB);
+    const long long groups = ((long long)cache->rows * cache->H + 7) / 8 * 8;
+    ACMI_REQUIRE(groups * a.tiles <= 0x7fffffffLL, "acmi_kv8_attn: %lld workgroups", groups * a.tiles);
+    const dim3 mgrid((unsigned)(groups * a.tiles));
+#define KV8_MANY(HDv, Q, P) hipLaunchKernelGGL((kv8_attn_many_kernel<HDv, Q, P, (HDv <= 64 ? 2 : 1)>), mgrid, dim3(256), 0, st, a)
+#define KV8_CASE(HDv)                                            \
+    case HDv:                                                    \
+        if (out_f32) KV8_MANY(HDv, true, true);                  \
+        else if (qhl) KV8_MANY(HDv, true, false);                \
+        else KV8_MANY(HDv, false, false);                        \
+        break;
     KV8_HD_SWITCH(cache->hd, KV8_CASE)
 #undef KV8_CASE
 #undef KV8_MANY

@@ -65,7 +65,11 @@ class KV8Cache:
             raise ValueError(f"KV8Cache.{who}: {name} {tuple(getattr(t, 'shape', ()))}, expected {tuple(shape)}")
         if t.dtype not in _DTYPES or t.device != self.device:
             raise ValueError(f"KV8Cache.{who}: {name} is {t.dtype} on {t.device}, expected float32 or bfloat16 on {self.device}")
-        return t if t.stride(-1) == 1 else t.contiguous()
+        # the kernels read 16 bytes at a time: a view whose rows do not start on 16 bytes is copied
+        es, strides = t.element_size(), t.stride()
+        if strides[-1] != 1 or (t.data_ptr() | es * strides[0] | es * strides[1] | es * strides[-2]) & 15:
+            t = t.clone(memory_format=torch.contiguous_format)
+        return t
 
     def _words(self, who: str, name: str, t: tp.Optional[torch.Tensor], need: bool) -> tp.Optional[torch.Tensor]:
         if t is None and not need:

@@ -639,7 +639,7 @@ typedef struct {
 
 /* Tokens start[r] .. start[r] + n[r] - 1 of every row r into the cache (n NULL: L each; start[r] = tokens the row holds
  * already, which must have been stored in order).  k / v: `dtype` elements at row * *_row + token * *_tok + head * *_head
- * (element strides), the hd features contiguous; tokens >= n[r] of a row are never read. */
+ * (element strides), the hd features contiguous and every row 16-byte aligned; tokens >= n[r] of a row are never read. */
 typedef struct {
     const void* k; const void* v; int dtype;
     long long k_row, k_tok, k_head, v_row, v_tok, v_head;
@@ -661,6 +661,7 @@ int acmi_kv8_load(const acmi_kv8_cache* cache, const int* len, int T, void* k_ou
  * With them, or with `complete` (the tail already holds the token), the call quantises a block that this token completes.
  * out: out_mode ACMI_OUT_F32 / ACMI_OUT_BF16 = [rows][S][Hq][hd]; ACMI_OUT_TILED (S = 1) = tiled activation of `rows` rows in
  * out_dtype with out_rbs K tiles per 16-row block, first column out_col0.
+ * q, k_new and v_new rows are 16-byte aligned (element strides).
  * The products of probabilities and values take f16 probabilities (2^-12 of each) for bf16 results, a pair of f16 for f32 ones;
  * scores, softmax statistics and sums are f32.
  * work: acmi_kv8_attn_work_floats(cache, S, Hq) floats of scratch of this call alone (NULL when that is 0). */

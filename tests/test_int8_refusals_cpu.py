@@ -42,7 +42,8 @@ def test_null_descriptors(C):
         assert rc == -1
 
 
-@pytest.mark.parametrize('kw,word', [(dict(L=-1), 'L=-1'), (dict(dtype=2), 'dtype'), (dict(k=None), 'null'), (dict(start=None), 'null')])
+@pytest.mark.parametrize('kw,word', [(dict(L=-1), 'L=-1'), (dict(dtype=2), 'dtype'), (dict(k=None), 'null'), (dict(start=None), 'null'),
+                                     (dict(k=260), 'aligned rows'), (dict(v_tok=2), 'aligned rows')])
 def test_bad_stores(C, kw, word):
     d = C.KV8StoreDesc(**{**dict(k=256, v=256, dtype=0, L=1, start=256), **kw})
     refused(C, C._kv8_store(ctypes.byref(cache(C)), ctypes.byref(d), None), word)
@@ -59,7 +60,8 @@ def test_bad_loads(C, T, dt, k):
     (dict(k_new=256), 'together'), (dict(k_new=256, v_new=256, S=2), 'S = 1'), (dict(k_new=256, v_new=256, causal=0), 'causal'),
     (dict(complete=1, S=3), 'S = 1'), (dict(k_new=256, v_new=256, new_dtype=4), 'new_dtype'), (dict(past_context=-1), 'past_context'),
     (dict(causal=0, past_context=3), 'past_context'), (dict(out_mode=2, out_dtype=1, out_col0=16), 'placement'),
-    (dict(out_mode=2, out_dtype=1, out_rbs=1), 'placement')])
+    (dict(out_mode=2, out_dtype=1, out_rbs=1), 'placement'), (dict(q=260), 'aligned rows'), (dict(q_row=2), 'aligned rows'),
+    (dict(k_new=256, v_new=256, kn_row=3), 'aligned rows'), (dict(k_new=256, v_new=264), 'aligned rows')])
 def test_bad_attention(C, kw, word):
     d = C.KV8AttnDesc(**{**dict(q=256, q_dtype=0, S=1, Hq=2, len=256, len_stride=1, causal=1, out=256, out_mode=0), **kw})
     refused(C, C._kv8_attn(ctypes.byref(cache(C)), ctypes.byref(d), None), word)
