@@ -43,6 +43,8 @@ __device__ __forceinline__ void kv8_ld16(const void* p, size_t i, int bf16, floa
         }
     }
 }
+// 8 consecutive features (16-byte aligned) -> f32
+template <typename T> __device__ __forceinline__ void kv8_ld8(const T* p, float (&x)[8]) { ld8(p, x); }
 __device__ __forceinline__ void kv8_st16(void* p, size_t i, int bf16, const float (&x)[16]) {
     if (bf16) {
         u32x4* q = reinterpret_cast<u32x4*>(reinterpret_cast<bf16_t*>(p) + i);
@@ -272,7 +274,7 @@ __global__ __launch_bounds__(256) void kv8_load_kernel(const Kv8LoadArgs p) {
 // Queries are f16 relative to a power of two near the row's largest feature; an f32 query is a pair of f16 (22 bits).
 // Per score the vector ALU does a maximum, one multiply-add (scale, running maximum), one exp2 and half a conversion: the value
 // block's scale, relative to the largest one met (vref), sits in the exponent too, and the row sums come out of the matrix
-// cores (a product with ones), from the very f16 numbers that multiply the values.  Probabilities are carried as 2^14 p.
+// cores (a product with ones), from the very f16 numbers that multiply the values.
 struct Kv8AttnArgs {
     acmi_kv8_cache c;
     const void* q; int q_bf16; long long q_row, q_tok, q_head;
@@ -333,15 +335,18 @@ __device__ __forceinline__ u32x4 kv8_fetch_v(const uint8_t* vb, int i, int nl, i
     return NT ? __builtin_nontemporal_load(q) : *q;
 }
 
-constexpr float KV8_PSHIFT = 14.f;
+// Probabilities are carried as 2^8 p relative to a running maximum that lags: it moves only when a block's maximum passes it by
+// more than 2^7, so p <= 2^15 stays in f16's range and the sums are rescaled in the first block and almost never after.  f16
+// resolves them down to 2^-32 of the maximum.
+constexpr float KV8_PSHIFT = 8.f, KV8_LAG = 7.f;
 
 // one column tile's state: lane (kg, n) belongs to column n
 template <int HD, bool QHL> struct Kv8Col {
     f16x8 qh[Kv8Geo<HD>::NK], ql[QHL ? Kv8Geo<HD>::NK : 1];
     float sfac;          // score factor: softmax scale * log2(e) * the query's power of two
     int lo, lim;         // positions [lo, lim) are seen
-    float m, l;          // running maximum (log2 units); sum of 2^14 p
-    f32x4 o[Kv8Geo<HD>::ND];   // sum of 2^14 p v, in units of the wave's vref
+    float m, l;          // running maximum (log2 units, lagging); sum of 2^8 p
+    f32x4 o[Kv8Geo<HD>::ND];   // sum of 2^8 p v, in units of the wave's vref
 };
 
 // A block of 64 tokens into QB column tiles.  K(tt, k) / V(i, u): the fragments (LO: KL / VL their f16 remainders, for a tail in
@@ -373,20 +378,16 @@ __device__ __forceinline__ void kv8_block(Kv8Col<HD, QHL> (&c)[QB], float& vref,
     fix_scores(s);
     // the block's value scale relative to the largest one met; a scale of 0 belongs to codes that are all 0
     const bool vnan = !(vs == vs);
+    float rescale = 1.f;
+    bool moved = false;
     if (vs > vref) {
-        const float f = vref > 0.f ? vref / vs : 0.f;
-#pragma unroll
-        for (int g = 0; g < QB; ++g)
-#pragma unroll
-            for (int i = 0; i < ND; ++i)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) c[g].o[i][r] *= f;
+        rescale = vref > 0.f ? vref / vs : 0.f;
         vref = vs;
+        moved = true;
     }
     const float lr = (vs > 0.f && vs < vref) ? __builtin_amdgcn_logf(vs / vref) : 0.f;   // log2
     const float ie = __builtin_amdgcn_exp2f(-lr);
     f16x8 ph[QB][2], pl[QB][PHL ? 2 : 1];
-    bool moved = false;
     float alpha[QB];
 #pragma unroll
     for (int g = 0; g < QB; ++g) {
@@ -410,7 +411,8 @@ __device__ __forceinline__ void kv8_block(Kv8Col<HD, QHL> (&c)[QB], float& vref,
         // belongs to scores that are all 0
         float f = ks * c[g].sfac;
         f = (none || f == 0.f) ? 1.f : f;
-        const float m_new = fmaxf(c[g].m, cmax * f);
+        const float top = cmax * f;
+        const float m_new = top > c[g].m + KV8_LAG ? top : c[g].m;
         const float m_use = m_new == -INFINITY ? 0.f : m_new;
         alpha[g] = __builtin_amdgcn_exp2f(c[g].m - m_use);
         c[g].m = m_new;
@@ -456,7 +458,7 @@ __device__ __forceinline__ void kv8_block(Kv8Col<HD, QHL> (&c)[QB], float& vref,
 #pragma unroll
             for (int i = 0; i < ND; ++i)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) c[g].o[i][r] *= alpha[g];
+                for (int r = 0; r < 4; ++r) c[g].o[i][r] *= alpha[g] * rescale;
     }
 #pragma unroll
     for (int i = 0; i < ND; ++i)
@@ -588,6 +590,9 @@ __device__ __forceinline__ void kv8_put4(const Kv8AttnArgs& p, int row, int s, i
 // soon as this block's K has been multiplied, its V likewise.
 constexpr int KV8_NW = 8;
 
+__device__ __forceinline__ float raw8(bf16_t v) { return bf16_to_f32(v); }
+__device__ __forceinline__ float raw8(float v) { return v; }
+
 // The tail's 16 tokens slot0 .. in f32, through the f32 matrix instruction, before any block of codes.
 template <int HD, bool QHL>
 __device__ __forceinline__ void kv8_tail16(const Kv8AttnArgs& p, const Kv8RowInfo& ri, int row, int kvh, int slot0,
@@ -597,49 +602,44 @@ __device__ __forceinline__ void kv8_tail16(const Kv8AttnArgs& p, const Kv8RowInf
     const int last = (ri.len - 1) / BLK, t0 = last * BLK + slot0, tb = p.c.tail_dtype == ACMI_BF16;
     const size_t base = ((size_t)row * p.c.H + kvh) * (BLK * HD);
     const size_t kn0 = (size_t)(row * p.kn_row + kvh * p.kn_head), vn0 = (size_t)(row * p.vn_row + kvh * p.vn_head);
-    // keys: lane (kg, nl) the features of its queries' lanes, of token t0 + nl
-    float kx[NK][8];
-    {
-        const int t = t0 + nl;
-        const bool isnew = ri.fresh && t == ri.len - 1;
-        const void* src = isnew ? p.kn : p.c.k_tail;
-        const int sb = isnew ? p.n_bf16 : tb;
-        const size_t at = isnew ? kn0 : base + (size_t)(slot0 + nl) * HD;
+    // keys: lane (kg, nl) the features of its queries' lanes, of token t0 + nl; values: feature i * 16 + nl of tokens t0 + kg * 4 + r.
+    // The row's newest token, which the tail does not hold yet, is put in its place.  (A token past the row's length: whatever the
+    // tail holds there only reaches scores that are masked; its values are dropped.)
+    float kx[NK][8], vx[ND][4], kn[NK][8], vn[ND];
+    const bool hasnew = ri.fresh && ri.len - 1 < t0 + 16;   // (wave uniform; the newest token is never before t0)
+    auto from = [&](auto* kt, auto* vt) {
 #pragma unroll
-        for (int k = 0; k < NK; ++k) {
-            const size_t i = at + (HD == 16 ? (kg & 1) * 8 : kv8_qdim<HD>(kg, k));
-            if (sb) {
-                const u32x4 w = *reinterpret_cast<const u32x4*>(reinterpret_cast<const bf16_t*>(src) + i);
+        for (int k = 0; k < NK; ++k) kv8_ld8(kt + (size_t)nl * HD + (HD == 16 ? (kg & 1) * 8 : kv8_qdim<HD>(kg, k)), kx[k]);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) { kx[k][2 * e] = __uint_as_float(w[e] << 16); kx[k][2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u); }
-            } else {
-                const f32x4* q = reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(src) + i);
-                const f32x4 a = q[0], b = q[1];
+        for (int r = 0; r < 4; ++r)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) { kx[k][e] = a[e]; kx[k][4 + e] = b[e]; }
-                if (tb && isnew) {
+            for (int i = 0; i < ND; ++i) vx[i][r] = raw8(vt[(size_t)(kg * 4 + r) * HD + i * 16 + nl]);
+    };
+    auto from_new = [&](auto* k, auto* v) {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) kx[k][e] = kv8_round(kx[k][e], 1);
-                }
-            }
-        }
-        // (a token past the row's length: whatever the tail holds there only reaches scores that are masked)
+        for (int q = 0; q < NK; ++q) kv8_ld8(k + (HD == 16 ? (kg & 1) * 8 : kv8_qdim<HD>(kg, q)), kn[q]);
+#pragma unroll
+        for (int i = 0; i < ND; ++i) vn[i] = raw8(v[i * 16 + nl]);
+    };
+    if (tb) from(reinterpret_cast<const bf16_t*>(p.c.k_tail) + base + slot0 * HD, reinterpret_cast<const bf16_t*>(p.c.v_tail) + base + slot0 * HD);
+    else from(reinterpret_cast<const float*>(p.c.k_tail) + base + slot0 * HD, reinterpret_cast<const float*>(p.c.v_tail) + base + slot0 * HD);
+    if (hasnew) {
+        if (p.n_bf16) from_new(reinterpret_cast<const bf16_t*>(p.kn) + kn0, reinterpret_cast<const bf16_t*>(p.vn) + vn0);
+        else from_new(reinterpret_cast<const float*>(p.kn) + kn0, reinterpret_cast<const float*>(p.vn) + vn0);
+        const int at = ri.len - 1 - t0;
+#pragma unroll
+        for (int k = 0; k < NK; ++k)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) kx[k][j] = nl == at ? kv8_round(kn[k][j], tb) : kx[k][j];
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int i = 0; i < ND; ++i) vx[i][r] = kg * 4 + r == at ? kv8_round(vn[i], tb) : vx[i][r];
     }
-    // values: lane (kg, nl) feature i * 16 + nl of tokens t0 + kg * 4 + r
-    float vx[ND][4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        const int t = t0 + kg * 4 + r;
-        const bool isnew = ri.fresh && t == ri.len - 1;
-        const void* src = isnew ? p.vn : p.c.v_tail;
-        const int sb = isnew ? p.n_bf16 : tb;
-        const size_t at = isnew ? vn0 : base + (size_t)(slot0 + kg * 4 + r) * HD;
+    for (int r = 0; r < 4; ++r)
 #pragma unroll
-        for (int i = 0; i < ND; ++i) {
-            const float v = kv8_ld(src, at + i * 16 + nl, sb);
-            vx[i][r] = t < ri.len ? (isnew ? kv8_round(v, tb) : v) : 0.f;
-        }
-    }
+        for (int i = 0; i < ND; ++i) vx[i][r] = t0 + kg * 4 + r < ri.len ? vx[i][r] : 0.f;
     f32x4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int k = 0; k < NK; ++k)
@@ -762,7 +762,7 @@ __global__ __launch_bounds__(KV8_NW * 64) void kv8_attn_split_kernel(const Kv8At
         if (nb < s1) get_v(nb);
         b = nb;
     }
-    const float unit = vref * (1.f / 16384.f);
+    const float unit = vref * (1.f / 256.f);
 #pragma unroll
     for (int i = 0; i < ND; ++i) {
         f32x4 o = c[0].o[i];
@@ -770,7 +770,7 @@ __global__ __launch_bounds__(KV8_NW * 64) void kv8_attn_split_kernel(const Kv8At
         for (int r = 0; r < 4; ++r) o[r] *= unit;
         *reinterpret_cast<f32x4*>(&sm_o[wave][nl][i * 16 + kg * 4]) = o;
     }
-    if (kg == 0) { sm_m[wave][nl] = c[0].m; sm_l[wave][nl] = c[0].l * (1.f / 16384.f); }
+    if (kg == 0) { sm_m[wave][nl] = c[0].m; sm_l[wave][nl] = c[0].l * (1.f / 256.f); }
     // the row's newest token and a block it completes (column tile 0 alone)
     if (mine && qt == 0 && ri.len > 0 && (ri.fresh || p.complete)) {
         const int tb = p.c.tail_dtype == ACMI_BF16;
@@ -898,13 +898,6 @@ __global__ __launch_bounds__(256, KV8_WPE) void kv8_attn_many_kernel(const Kv8At
     const Kv8Span sp = kv8_span(p, ri, w0, min(w0 + 64 * QB, cols));
     Kv8Span me = kv8_span(p, ri, min(c0, cols - 1), min(c0 + 16 * QB, cols));
     if (c0 >= cols) { me.live = me.tail = false; me.bf = me.bt = 0; }
-    Kv8Col<HD, QHL> c[QB];
-#pragma unroll
-    for (int g = 0; g < QB; ++g) {
-        float x[NK][8];
-        kv8_load_q<HD>(p, row, kvh, c0 + g * 16 + nl, kg, x);
-        kv8_column<HD, QHL>(p, ri, c0 + g * 16 + nl, x, c[g]);
-    }
     float vref = 0.f;
     const size_t rh = (size_t)row * p.c.H + kvh, hb = rh * p.c.nblk;
     const uint8_t* kc = reinterpret_cast<const uint8_t*>(p.c.k_codes) + hb * (size_t)(BLK * HD);
@@ -933,8 +926,14 @@ __global__ __launch_bounds__(256, KV8_WPE) void kv8_attn_many_kernel(const Kv8At
     auto none = [] {};
     auto keep = [](auto&) {};
     int buf = 0;
+    float x[QB][NK][8];
+#pragma unroll
+    for (int g = 0; g < QB; ++g) kv8_load_q<HD>(p, row, kvh, c0 + g * 16 + nl, kg, x[g]);
+    if (sp.bf < sp.bt) request(sp.bf);
+    Kv8Col<HD, QHL> c[QB];
+#pragma unroll
+    for (int g = 0; g < QB; ++g) kv8_column<HD, QHL>(p, ri, c0 + g * 16 + nl, x[g], c[g]);
     if (sp.bf < sp.bt) {
-        request(sp.bf);
         stage(0);
         __syncthreads();
         for (int b = sp.bf; b < sp.bt; ++b) {
@@ -959,12 +958,22 @@ __global__ __launch_bounds__(256, KV8_WPE) void kv8_attn_many_kernel(const Kv8At
         unsigned vb = 0;
         if (threadIdx.x == 0) { sm.kbad = 0; sm.vbad = 0; }
         const int tk = wave * 16 + nl;   // this lane's token of K
+        auto from = [&](auto* kt, auto* vt) {   // every load of the tail in flight at once (places past the length are masked below)
+#pragma unroll
+            for (int k = 0; k < NK; ++k) kv8_ld8(kt + (size_t)tk * HD + (HD == 16 ? (kg & 1) * 8 : kv8_qdim<HD>(kg, k)), kx[k]);
+#pragma unroll
+            for (int q = 0; q < VT; ++q)
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                    vx[q][j] = raw8(vt[(size_t)((j >> 2) * 16 + kg * 4 + (j & 3)) * HD + min(wave + q * 4, ND - 1) * 16 + nl]);
+        };
+        if (tb) from(reinterpret_cast<const bf16_t*>(p.c.k_tail) + base, reinterpret_cast<const bf16_t*>(p.c.v_tail) + base);
+        else from(reinterpret_cast<const float*>(p.c.k_tail) + base, reinterpret_cast<const float*>(p.c.v_tail) + base);
 #pragma unroll
         for (int k = 0; k < NK; ++k)
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const int d = HD == 16 ? (kg & 1) * 8 + j : kv8_qdim<HD>(kg, k) + j;
-                float v = tk < nt ? kv8_ld(p.c.k_tail, base + (size_t)tk * HD + d, tb) : 0.f;
+                float v = tk < nt ? kx[k][j] : 0.f;
                 const float a = fabsf(v);
                 if (!(a <= 3.4028234663852886e38f)) { kb = true; v = 0.f; }
                 kx[k][j] = v;
@@ -974,8 +983,7 @@ __global__ __launch_bounds__(256, KV8_WPE) void kv8_attn_many_kernel(const Kv8At
         for (int q = 0; q < VT; ++q)
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
-                const int t = (j >> 2) * 16 + kg * 4 + (j & 3), i = wave + q * 4;
-                float v = (i < ND && t < nt) ? kv8_ld(p.c.v_tail, base + (size_t)t * HD + i * 16 + nl, tb) : 0.f;
+                float v = (j >> 2) * 16 + kg * 4 + (j & 3) < nt ? vx[q][j] : 0.f;
                 const float a = fabsf(v);
                 if (!(a <= 3.4028234663852886e38f)) { vb |= 1u << j; v = 0.f; }
                 vx[q][j] = v;
