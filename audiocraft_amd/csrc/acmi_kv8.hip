@@ -20,6 +20,14 @@ __device__ __forceinline__ void kv8_st(void* p, size_t i, int bf16, float v) {
 // what the tail makes of a value
 __device__ __forceinline__ float kv8_round(float v, int bf16) { return bf16 ? bf16_to_f32(f32_to_bf16(v)) : v; }
 
+// maximum over the four lanes of a column (xor 16, xor 32) without the LDS crossbar: a swap of a register with its own copy leaves
+// the two halves of every pair side by side
+__device__ __forceinline__ float kv8_xmax(float v) {
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
 // 16 consecutive features (16-byte aligned) -> f32
 __device__ __forceinline__ void kv8_ld16(const void* p, size_t i, int bf16, float (&x)[16]) {
     if (bf16) {
@@ -284,7 +292,7 @@ struct Kv8AttnArgs {
     const void* kn; const void* vn; int n_bf16; long long kn_row, kn_head, vn_row, vn_head;
     int complete;
     void* out; int out_mode, out_bf16, out_rbs, out_col0;
-    float* work; int splits, tiles;
+    float* work; int splits, chunk, tiles;   // a row's blocks in chunks of `chunk`, one workgroup each
     float scale;
 };
 
@@ -311,7 +319,8 @@ template <int HD> __device__ __forceinline__ int kv8_qdim(int kg, int k) {
     return HD >= 64 ? (k >> 1) * 64 + kg * 16 + (k & 1) * 8 : kg * 8;
 }
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-// K codes of 16 tokens (lane: token nl), V codes of 16 features (lane: feature nl)
+// K codes of 16 tokens (lane: token nl), V codes of 16 features (lane: feature nl).  NT: as a stream -- not for the keys of hd 128,
+// whose 128-byte rows take two requests: the line was gone before the second (decode over 32768 tokens: 70 -> 56 us)
 template <int HD, bool NT>
 __device__ __forceinline__ void kv8_fetch_k(const uint8_t* kb, int tt, int nl, int kg, uint32_t (&w)[Kv8Geo<HD>::KW]) {
     const uint8_t* row = kb + (tt * 16 + nl) * HD;
@@ -404,8 +413,7 @@ __device__ __forceinline__ void kv8_block(Kv8Col<HD, QHL> (&c)[QB], float& vref,
         float cmax = -INFINITY;
 #pragma unroll
         for (int tt = 0; tt < 4; ++tt) cmax = fmaxf(cmax, fmaxf(fmaxf(s[g][tt][0], s[g][tt][1]), fmaxf(s[g][tt][2], s[g][tt][3])));
-        cmax = fmaxf(cmax, __shfl_xor(cmax, 16, 64));
-        cmax = fmaxf(cmax, __shfl_xor(cmax, 32, 64));
+        cmax = kv8_xmax(cmax);
         const bool none = cmax == -INFINITY;
         // a column that sees nothing here keeps clear of the block's scales (which a NaN may have poisoned); a key scale of 0
         // belongs to scores that are all 0
@@ -534,8 +542,7 @@ __device__ __forceinline__ void kv8_column(const Kv8AttnArgs& p, const Kv8RowInf
     for (int k = 0; k < Kv8Geo<HD>::NK; ++k)
 #pragma unroll
         for (int j = 0; j < 8; ++j) amax = kv8_amax(amax, x[k][j]);
-    amax = fmaxf(amax, __shfl_xor(amax, 16, 64));
-    amax = fmaxf(amax, __shfl_xor(amax, 32, 64));
+    amax = kv8_xmax(amax);
     // features times a power of two that brings the largest into [2^14, 2^15); a query with a NaN or an infinity gives NaN
     const int e = (amax > 0.f && amax < INFINITY) ? ilogbf(amax) : 0;
     const float down = ldexpf(1.f, min(14 - e, 127));
@@ -554,6 +561,10 @@ __device__ __forceinline__ void kv8_column(const Kv8AttnArgs& p, const Kv8RowInf
 // the blocks of codes a column tile visits, and how many workgroups share them
 struct Kv8Span { int bf, bt, eff; bool live, tail; };
 constexpr int KV8_MIN_BLOCKS = 8;   // blocks per workgroup below which no further split is made
+constexpr int KV8_MAX_SPLITS = 64;
+#ifndef KV8_TARGET
+#define KV8_TARGET 512
+#endif
 __device__ __forceinline__ Kv8Span kv8_span(const Kv8AttnArgs& p, const Kv8RowInfo& ri, int c0, int c1) {   // columns [c0, c1)
     Kv8Span s;
     const int s0 = c0 / p.G, s1 = min((c1 - 1) / p.G, ri.qlen - 1);
@@ -565,7 +576,7 @@ __device__ __forceinline__ Kv8Span kv8_span(const Kv8AttnArgs& p, const Kv8RowIn
     const int lo = max(ri.start, (p.causal && p.past > 0) ? p0 - p.past : 0);
     s.bt = min(nf, (lim + BLK - 1) / BLK);
     s.bf = min(lo / BLK, s.bt);
-    s.eff = max(1, min(p.splits, (s.bt - s.bf) / KV8_MIN_BLOCKS));
+    s.eff = p.splits == 1 ? 1 : max(1, min(p.splits, (s.bt - s.bf + p.chunk - 1) / p.chunk));
     s.tail = lim > nf * BLK && lo < ri.len;
     return s;
 }
@@ -588,7 +599,20 @@ __device__ __forceinline__ void kv8_put4(const Kv8AttnArgs& p, int row, int s, i
 // ---- few queries: one workgroup per (split, column tile of a cache head, row); its 8 waves take the blocks in turn, four of them
 // 16 tokens of the tail each, and are joined through LDS.  A wave keeps one block in flight: the next block's K is requested as
 // soon as this block's K has been multiplied, its V likewise.
-constexpr int KV8_NW = 8;
+#ifndef KV8_NW64
+#define KV8_NW64 8
+#endif
+#ifndef KV8_NW128
+#define KV8_NW128 4
+#endif
+#ifndef KV8_B64
+#define KV8_B64 4
+#endif
+#ifndef KV8_B128
+#define KV8_B128 2
+#endif
+template <int HD> constexpr int kv8_nw() { return HD == 128 ? KV8_NW128 : KV8_NW64; }
+template <int HD> constexpr int kv8_wpe() { return HD == 128 ? KV8_B128 : KV8_B64; }
 
 __device__ __forceinline__ float raw8(bf16_t v) { return bf16_to_f32(v); }
 __device__ __forceinline__ float raw8(float v) { return v; }
@@ -653,8 +677,7 @@ __device__ __forceinline__ void kv8_tail16(const Kv8AttnArgs& p, const Kv8RowInf
         s[r] = (t >= c.lo && t < c.lim && t < ri.len) ? s[r] * f : -INFINITY;
         cmax = fmaxf(cmax, s[r]);
     }
-    cmax = fmaxf(cmax, __shfl_xor(cmax, 16, 64));
-    cmax = fmaxf(cmax, __shfl_xor(cmax, 32, 64));
+    cmax = kv8_xmax(cmax);
     c.m = cmax;
     const float top = cmax == -INFINITY ? 0.f : cmax;
     float sum = 0.f;
@@ -708,13 +731,14 @@ __device__ __forceinline__ void kv8_tail16(const Kv8AttnArgs& p, const Kv8RowInf
 }
 
 template <int HD, bool QHL, bool PHL>
-__global__ __launch_bounds__(KV8_NW * 64) void kv8_attn_split_kernel(const Kv8AttnArgs p) {
-    constexpr int NK = Kv8Geo<HD>::NK, ND = Kv8Geo<HD>::ND, KW = Kv8Geo<HD>::KW, PITCH = HD + 4, NW = KV8_NW;
+__global__ __launch_bounds__(kv8_nw<HD>() * 64, kv8_wpe<HD>()) void kv8_attn_split_kernel(const Kv8AttnArgs p) {
+    constexpr int NK = Kv8Geo<HD>::NK, ND = Kv8Geo<HD>::ND, KW = Kv8Geo<HD>::KW, PITCH = HD + 4, NW = kv8_nw<HD>();
     __shared__ __attribute__((aligned(16))) float sm_o[NW][16][PITCH];
     __shared__ float sm_m[NW][16], sm_l[NW][16];
     __shared__ Kv8QuantLds<HD> sm_q;
-    const int split = blockIdx.x, row = blockIdx.z;
-    const int qtiles = p.tiles, kvh = blockIdx.y / qtiles, qt = blockIdx.y - kvh * qtiles;
+    // (chunk slowest: the workgroups that a shorter row does not need come last, and leave at once)
+    const int split = blockIdx.z, row = blockIdx.y;
+    const int qtiles = p.tiles, kvh = blockIdx.x / qtiles, qt = blockIdx.x - kvh * qtiles;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int nl = lane & 15, kg = lane >> 4;
     float x[NK][8];
@@ -722,12 +746,13 @@ __global__ __launch_bounds__(KV8_NW * 64) void kv8_attn_split_kernel(const Kv8At
     const Kv8RowInfo ri = kv8_row(p, row);
     const Kv8Span sp = kv8_span(p, ri, qt * 16, min(qt * 16 + 16, p.S * p.G));
     if (split >= sp.eff) return;
-    const int per = (sp.bt - sp.bf + sp.eff - 1) / sp.eff;
-    const int s0 = sp.bf + split * per, s1 = min(sp.bt, s0 + per);
+    const int s0 = sp.bf + split * p.chunk, s1 = sp.eff == 1 ? sp.bt : min(sp.bt, s0 + p.chunk);
     const size_t rh = (size_t)row * p.c.H + kvh, hb = rh * p.c.nblk;
     const uint8_t* kc = reinterpret_cast<const uint8_t*>(p.c.k_codes) + hb * (size_t)(BLK * HD);
     const uint8_t* vc = reinterpret_cast<const uint8_t*>(p.c.v_codes) + hb * (size_t)(BLK * HD);
-    const float* ks = p.c.k_scale + hb; const float* vs = p.c.v_scale + hb;
+    int z = 0;   // an opaque lane offset of 0: the scales come as vector loads, in order with the codes (a scalar load shares its
+    asm volatile("" : "+v"(z));   // counter with the LDS and would be waited for early)
+    const float* ks = p.c.k_scale + hb + z; const float* vs = p.c.v_scale + hb + z;
 
     uint32_t kr[4][KW];
     u32x4 vr[ND];
@@ -735,15 +760,15 @@ __global__ __launch_bounds__(KV8_NW * 64) void kv8_attn_split_kernel(const Kv8At
     auto get_k = [&](int b) {
         const uint8_t* kb = kc + (size_t)b * (BLK * HD);
 #pragma unroll
-        for (int tt = 0; tt < 4; ++tt) kv8_fetch_k<HD, true>(kb, tt, nl, kg, kr[tt]);
-        ksn = ks[b];
+        for (int tt = 0; tt < 4; ++tt) kv8_fetch_k<HD, HD <= 64>(kb, tt, nl, kg, kr[tt]);
+        ksn = __builtin_nontemporal_load(ks + b);
         __builtin_amdgcn_sched_barrier(0);   // (the scheduler sinks requests to their uses)
     };
     auto get_v = [&](int b) {
         const uint8_t* vb = vc + (size_t)b * (BLK * HD);
 #pragma unroll
         for (int i = 0; i < ND; ++i) vr[i] = kv8_fetch_v<true>(vb, i, nl, kg);
-        vsn = vs[b];
+        vsn = __builtin_nontemporal_load(vs + b);
         __builtin_amdgcn_sched_barrier(0);
     };
     int b = s0 + wave;
@@ -754,12 +779,14 @@ __global__ __launch_bounds__(KV8_NW * 64) void kv8_attn_split_kernel(const Kv8At
     float vref = 0.f;
     if (mine && sp.tail && wave < 4 && (ri.len - 1) / BLK * BLK + wave * 16 < ri.len) kv8_tail16<HD, QHL>(p, ri, row, kvh, wave * 16, x, c[0], vref);
     while (b < s1) {
-        const int nb = b + NW;
+        // the next requests are not conditional (a wave's last ones read its last block again, from the cache): the waits of a
+        // straight line count them exactly, those behind a branch would wait for everything
+        const int nb = b + NW, rq = min(nb, s1 - 1);
         const float kcur = ksn, vcur = vsn;
         kv8_block<HD, QHL, PHL, false, 1>(c, vref, [&](int tt, int k) { return kv8_cvt(kr[tt][2 * k], kr[tt][2 * k + 1]); },
                                           [&](int i, int u) { return kv8_cvt(vr[i][2 * u], vr[i][2 * u + 1]); }, 0, 0, kcur, vcur, b * BLK,
-                                          [&] { if (nb < s1) get_k(nb); }, [](auto&) {});
-        if (nb < s1) get_v(nb);
+                                          [&] { get_k(rq); }, [](auto&) {});
+        get_v(rq);
         b = nb;
     }
     const float unit = vref * (1.f / 256.f);
@@ -819,7 +846,7 @@ __global__ __launch_bounds__(KV8_NW * 64) void kv8_attn_split_kernel(const Kv8At
             for (int r = 0; r < 4; ++r) o[r] = none ? 0.f : o[r] / den;
             kv8_put4(p, row, s, kvh * p.G + g, HD, d, o);
         } else {   // partial: [row][cache head x tile][column][split][features | max | sum]
-            float* w = p.work + ((((size_t)row * gridDim.y + blockIdx.y) * 16 + n) * p.splits + split) * (HD + 4);
+            float* w = p.work + ((((size_t)row * gridDim.x + blockIdx.x) * 16 + n) * p.splits + split) * (HD + 4);
             *reinterpret_cast<f32x4*>(w + d) = o;
             if (d == 0) { w[HD] = M; w[HD + 1] = den; }
         }
@@ -840,11 +867,12 @@ __global__ __launch_bounds__(256) void kv8_attn_join_kernel(const Kv8AttnArgs p)
     if (sp.eff == 1) return;   // the split kernel has written it
     const float* w = p.work + (((size_t)row * gridDim.y + blockIdx.y) * 16 + n) * p.splits * (HD + 4);
     const int f4 = threadIdx.x % F4, grp = threadIdx.x / F4;
-    float M = -INFINITY;
-    for (int k = 0; k < sp.eff; ++k) M = fmaxf(M, w[(size_t)k * (HD + 4) + HD]);
+    const int lane = threadIdx.x & 63;
+    const float M = wave_max(lane < sp.eff ? w[(size_t)lane * (HD + 4) + HD] : -INFINITY);   // (KV8_MAX_SPLITS = 64)
     const float Mu = M == -INFINITY ? 0.f : M;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
     float den = 0.f;
+#pragma unroll 4
     for (int k = grp; k < sp.eff; k += NG) {
         const float* y = w + (size_t)k * (HD + 4);
         const float f = __builtin_amdgcn_exp2f(y[HD] - Mu);
@@ -905,9 +933,11 @@ __global__ __launch_bounds__(256, KV8_WPE) void kv8_attn_many_kernel(const Kv8At
     uint32_t kr[KW];
     u32x4 vr[VT];
     float ksn = 0.f, vsn = 0.f;
+    int z = 0;   // an opaque lane offset of 0: vector loads, in order with the codes
+    asm volatile("" : "+v"(z));
     auto request = [&](int b) {   // this wave's quarter: 16 tokens of K, VT feature tiles of V; the block's scales
-        ksn = __builtin_nontemporal_load(p.c.k_scale + hb + b);
-        vsn = __builtin_nontemporal_load(p.c.v_scale + hb + b);
+        ksn = p.c.k_scale[hb + b + z];
+        vsn = p.c.v_scale[hb + b + z];
         kv8_fetch_k<HD, false>(kc + (size_t)b * (BLK * HD), wave, nl, kg, kr);
 #pragma unroll
         for (int q = 0; q < VT; ++q)
@@ -1166,17 +1196,23 @@ extern "C" int acmi_kv8_load(const acmi_kv8_cache* cache, const int* len, int T,
 // column tiles up to which the split form runs
 constexpr int KV8_SPLIT_TILES = 4;
 static bool kv8_few(int S, int G) { return (S * G + 15) / 16 <= KV8_SPLIT_TILES; }
-static int kv8_splits(const acmi_kv8_cache* c, int S, int G) {
-    const long long wgs = (long long)c->rows * c->H * ((S * G + 15) / 16);
-    const long long want = (1024 + wgs - 1) / wgs, most = c->nblk / KV8_MIN_BLOCKS;
-    return (int)max(1LL, min(min(want, most), 64LL));
+// Blocks per workgroup: the longest possible row in so many chunks that the call has about KV8_TARGET workgroups; one chunk (and
+// no second launch) when the tiles alone fill the chip.  The rows' lengths are not known here: shorter rows take fewer chunks of
+// the same size, so that all workgroups take equally long.
+static void kv8_split_plan(const acmi_kv8_cache* c, int S, int G, int* splits, int* chunk) {
+    const long long tiles = (long long)c->H * ((S * G + 15) / 16) * c->rows;
+    long long n = 1;
+    if (tiles * 4 <= KV8_TARGET) n = max(1LL, min(min(KV8_TARGET / tiles, (long long)(c->nblk / KV8_MIN_BLOCKS)), (long long)KV8_MAX_SPLITS));
+    *chunk = (int)((c->nblk + n - 1) / n);
+    *splits = (c->nblk + *chunk - 1) / *chunk;
 }
 
 extern "C" size_t acmi_kv8_attn_work_floats(const acmi_kv8_cache* cache, int S, int Hq) {
     if (kv8_check(cache, "acmi_kv8_attn_work_floats") || S <= 0 || Hq <= 0 || Hq % cache->H) return 0;
     const int G = Hq / cache->H;
     if (!kv8_few(S, G)) return 0;
-    const int sp = kv8_splits(cache, S, G);
+    int sp, chunk;
+    kv8_split_plan(cache, S, G, &sp, &chunk);
     return sp == 1 ? 0 : (size_t)cache->rows * cache->H * ((S * G + 15) / 16) * sp * 16 * (cache->hd + 4);
 }
 
@@ -1218,14 +1254,14 @@ extern "C" int acmi_kv8_attn(const acmi_kv8_cache* cache, const acmi_kv8_attn_de
     hipStream_t st = (hipStream_t)stream;
     const int qtiles = (d.S * a.G + 15) / 16;
     if (kv8_few(d.S, a.G)) {
-        a.splits = kv8_splits(cache, d.S, a.G);
+        kv8_split_plan(cache, d.S, a.G, &a.splits, &a.chunk);
         a.work = d.work;
         ACMI_REQUIRE(a.splits == 1 || (d.work != nullptr && (reinterpret_cast<size_t>(d.work) & 15) == 0),
                      "acmi_kv8_attn: needs acmi_kv8_attn_work_floats floats of 16-byte aligned work");
         ACMI_REQUIRE((long long)cache->H * qtiles <= 65535, "acmi_kv8_attn: %d heads x %d column tiles", cache->H, qtiles);
-        const dim3 grid(a.splits, cache->H * qtiles, cache->rows);
+        const dim3 grid(cache->H * qtiles, cache->rows, a.splits);
         a.tiles = qtiles;
-#define KV8_SPLIT(HDv, Q, P) hipLaunchKernelGGL((kv8_attn_split_kernel<HDv, Q, P>), grid, dim3(KV8_NW * 64), 0, st, a)
+#define KV8_SPLIT(HDv, Q, P) hipLaunchKernelGGL((kv8_attn_split_kernel<HDv, Q, P>), grid, dim3(kv8_nw<HDv>() * 64), 0, st, a)
 #define KV8_CASE(HDv)                                            \
     case HDv:                                                    \
         if (out_f32) KV8_SPLIT(HDv, true, true);                 \
