@@ -292,6 +292,7 @@ struct Kv8AttnArgs {
     const void* kn; const void* vn; int n_bf16; long long kn_row, kn_head, vn_row, vn_head;
     int complete;
     void* out; int out_mode, out_bf16, out_rbs, out_col0;
+    float rG;   // 1 / G
     float* work; int splits, chunk, tiles;   // a row's blocks in chunks of `chunk`, one workgroup each
     float scale;
 };
@@ -358,20 +359,33 @@ template <int HD, bool QHL> struct Kv8Col {
     f32x4 o[Kv8Geo<HD>::ND];   // sum of 2^8 p v, in units of the wave's vref
 };
 
+struct Kv8Ref { float v, inv; };   // largest value scale met, its reciprocal
+
 // A block of 64 tokens into QB column tiles.  K(tt, k) / V(i, u): the fragments (LO: KL / VL their f16 remainders, for a tail in
 // f32); ks, vs: the block's scales; t0 its first position; after_k(): called once the K fragments have been used.
 template <int HD, bool QHL, bool PHL, bool LO, int QB, typename FK, typename FV, typename FKL, typename FVL, typename FA, typename FS>
-__device__ __forceinline__ void kv8_block(Kv8Col<HD, QHL> (&c)[QB], float& vref, const FK& K, const FV& V, const FKL& KL, const FVL& VL,
+__device__ __forceinline__ void kv8_block(Kv8Col<HD, QHL> (&c)[QB], Kv8Ref& vref, const FK& K, const FV& V, const FKL& KL, const FVL& VL,
                                           float ks, float vs, int t0, const FA& after_k, const FS& fix_scores) {
     constexpr int NK = Kv8Geo<HD>::NK, ND = Kv8Geo<HD>::ND;
     const int kg = (threadIdx.x & 63) >> 4;
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
     f32x4 s[QB][4];
+    constexpr bool PRE = QB > 1 && NK <= 2;   // fragments from LDS: all requested at once, so that one latency is waited for
+    f16x8 pre[PRE ? 4 : 1][PRE ? NK : 1];
+    if constexpr (PRE) {
+#pragma unroll
+        for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+            for (int k = 0; k < NK; ++k) pre[tt][k] = K(tt, k);
+        __builtin_amdgcn_sched_barrier(0);
+    }
 #pragma unroll
     for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
         for (int k = 0; k < NK; ++k) {
-            const f16x8 kf = K(tt, k);
+            f16x8 kf;
+            if constexpr (PRE) kf = pre[tt][k];
+            else kf = K(tt, k);
 #pragma unroll
             for (int g = 0; g < QB; ++g) {
                 s[g][tt] = kv8_mma(kf, c[g].qh[k], k == 0 ? zero : s[g][tt]);
@@ -389,26 +403,30 @@ __device__ __forceinline__ void kv8_block(Kv8Col<HD, QHL> (&c)[QB], float& vref,
     const bool vnan = !(vs == vs);
     float rescale = 1.f;
     bool moved = false;
-    if (vs > vref) {
-        rescale = vref > 0.f ? vref / vs : 0.f;
-        vref = vs;
+    if (vs > vref.v) {
+        rescale = vref.v > 0.f ? vref.v / vs : 0.f;
+        vref.v = vs;
+        vref.inv = 1.f / vs;
         moved = true;
     }
-    const float lr = (vs > 0.f && vs < vref) ? __builtin_amdgcn_logf(vs / vref) : 0.f;   // log2
+    const float lr = (vs > 0.f && vs < vref.v) ? __builtin_amdgcn_logf(vs * vref.inv) : 0.f;   // log2
     const float ie = __builtin_amdgcn_exp2f(-lr);
     f16x8 ph[QB][2], pl[QB][PHL ? 2 : 1];
     float alpha[QB];
 #pragma unroll
     for (int g = 0; g < QB; ++g) {
-        const bool all = c[g].lo <= t0 && c[g].lim >= t0 + BLK;
-        if (!__all(all)) {
+        const int hi = c[g].lim - t0 - kg * 4, lo = c[g].lo - t0 - kg * 4;   // token tt * 16 + r of this lane is seen when lo <= it < hi
+        if (__any(c[g].lim < t0 + BLK)) {
 #pragma unroll
             for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int t = t0 + tt * 16 + kg * 4 + r;
-                    s[g][tt][r] = (t >= c[g].lo && t < c[g].lim) ? s[g][tt][r] : -INFINITY;
-                }
+                for (int r = 0; r < 4; ++r) s[g][tt][r] = tt * 16 + r < hi ? s[g][tt][r] : -INFINITY;
+        }
+        if (__any(c[g].lo > t0)) {
+#pragma unroll
+            for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s[g][tt][r] = tt * 16 + r >= lo ? s[g][tt][r] : -INFINITY;
         }
         float cmax = -INFINITY;
 #pragma unroll
@@ -487,21 +505,28 @@ __device__ __forceinline__ void kv8_block(Kv8Col<HD, QHL> (&c)[QB], float& vref,
 }
 
 // what a column is: row geometry shared by both kernels
+// column -> query: exact for columns below 2^21 (checked by the entry), since (c + 1/2) / G is at least 1 / (2 G) from an integer
+__device__ __forceinline__ int kv8_query(const Kv8AttnArgs& p, int c) { return (int)(((float)c + 0.5f) * p.rG); }
+
 struct Kv8RowInfo { int len, qlen, start; bool fresh; };   // fresh: the call brings the row's newest token (and it fits)
 __device__ __forceinline__ Kv8RowInfo kv8_row(const Kv8AttnArgs& p, int row) {
     Kv8RowInfo r;
-    const long long len = (long long)p.len[(size_t)row * p.len_stride] + p.len_bias;
+    // (every load at once, then into scalar registers: what follows from them is the same for the whole wave)
+    const int len0 = p.len[(size_t)row * p.len_stride];
+    const int ql = p.q_len != nullptr ? p.q_len[row] : p.S;
+    const int st = p.start_rows != nullptr ? p.start_rows[row] : 0;
+    const long long len = (long long)__builtin_amdgcn_readfirstlane(len0) + p.len_bias;
     r.len = (int)max(0LL, min(len, (long long)p.c.nblk * BLK));
     r.fresh = p.kn != nullptr && r.len == len && len > 0;
-    r.qlen = p.q_len != nullptr ? max(0, min(p.q_len[row], p.S)) : p.S;
-    r.start = p.start_rows != nullptr ? max(0, p.start_rows[row]) : 0;
+    r.qlen = max(0, min(__builtin_amdgcn_readfirstlane(ql), p.S));
+    r.start = max(0, __builtin_amdgcn_readfirstlane(st));
     return r;
 }
 
 // the query features of a lane: x[k][j] = feature kv8_qdim(kg, k) + j of column cidx (past the last column: the last query)
 template <int HD>
 __device__ __forceinline__ void kv8_load_q(const Kv8AttnArgs& p, int row, int kvh, int cidx, int kg, float (&x)[Kv8Geo<HD>::NK][8]) {
-    const int s = min(cidx / p.G, p.S - 1), g = cidx % p.G;
+    const int s0 = kv8_query(p, cidx), g = cidx - s0 * p.G, s = min(s0, p.S - 1);
     const size_t qb = (size_t)(row * p.q_row + (long long)s * p.q_tok + (long long)(kvh * p.G + g) * p.q_head);
 #pragma unroll
     for (int k = 0; k < Kv8Geo<HD>::NK; ++k) {
@@ -526,7 +551,7 @@ __device__ __forceinline__ void kv8_load_q(const Kv8AttnArgs& p, int row, int kv
 // column cidx of (row, cache head): visible range and operands from its features
 template <int HD, bool QHL>
 __device__ __forceinline__ void kv8_column(const Kv8AttnArgs& p, const Kv8RowInfo& ri, int cidx, const float (&x)[Kv8Geo<HD>::NK][8], Kv8Col<HD, QHL>& c) {
-    const int s = cidx / p.G;
+    const int s = kv8_query(p, cidx);
     const bool live = s < ri.qlen;
     const int pos = ri.len - ri.qlen + s;
     // (columns without a query are never stored: they see everything, so that they do not keep a block on the masked path)
@@ -537,12 +562,12 @@ __device__ __forceinline__ void kv8_column(const Kv8AttnArgs& p, const Kv8RowInf
     c.m = -INFINITY; c.l = 0.f;
 #pragma unroll
     for (int i = 0; i < Kv8Geo<HD>::ND; ++i) c.o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float amax = 0.f;
+    float amax = 0.f, bad = 0.f;   // bad: NaN as soon as a feature is not finite (which a maximum would not tell)
 #pragma unroll
     for (int k = 0; k < Kv8Geo<HD>::NK; ++k)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) amax = kv8_amax(amax, x[k][j]);
-    amax = kv8_xmax(amax);
+        for (int j = 0; j < 8; ++j) { amax = fmaxf(amax, fabsf(x[k][j])); bad = fmaf(x[k][j], 0.f, bad); }
+    amax = kv8_xmax(bad == 0.f ? amax : INFINITY);
     // features times a power of two that brings the largest into [2^14, 2^15); a query with a NaN or an infinity gives NaN
     const int e = (amax > 0.f && amax < INFINITY) ? ilogbf(amax) : 0;
     const float down = ldexpf(1.f, min(14 - e, 127));
@@ -581,17 +606,22 @@ __device__ __forceinline__ Kv8Span kv8_span(const Kv8AttnArgs& p, const Kv8RowIn
     return s;
 }
 
+typedef __bf16 kv8_bf16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t kv8_pack_bf16(float lo, float hi) {   // nearest even, one instruction
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(kv8_f32x2{lo, hi}, kv8_bf16x2));
+}
+
 // out of a finished column: 4 consecutive features
 __device__ __forceinline__ void kv8_put4(const Kv8AttnArgs& p, int row, int s, int head, int HD, int d, const f32x4& v) {
     const size_t at = (((size_t)row * p.S + s) * p.Hq + head) * HD + d;
     if (p.out_mode == ACMI_OUT_F32) *reinterpret_cast<f32x4*>(reinterpret_cast<float*>(p.out) + at) = v;
     else if (p.out_mode == ACMI_OUT_BF16)
-        *reinterpret_cast<uint2*>(reinterpret_cast<bf16_t*>(p.out) + at) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+        *reinterpret_cast<uint2*>(reinterpret_cast<bf16_t*>(p.out) + at) = make_uint2(kv8_pack_bf16(v[0], v[1]), kv8_pack_bf16(v[2], v[3]));
     else {
         const int col = p.out_col0 + head * HD + d;   // (a multiple of 4: the four features share a lane's 16 bytes)
         if (p.out_bf16)
             *reinterpret_cast<uint2*>(reinterpret_cast<bf16_t*>(p.out) + tiled_index<bf16_t>(row, col, p.out_rbs)) =
-                make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+                make_uint2(kv8_pack_bf16(v[0], v[1]), kv8_pack_bf16(v[2], v[3]));
         else *reinterpret_cast<f32x4*>(reinterpret_cast<float*>(p.out) + tiled_index<float>(row, col, p.out_rbs)) = v;
     }
 }
@@ -620,7 +650,7 @@ __device__ __forceinline__ float raw8(float v) { return v; }
 // The tail's 16 tokens slot0 .. in f32, through the f32 matrix instruction, before any block of codes.
 template <int HD, bool QHL>
 __device__ __forceinline__ void kv8_tail16(const Kv8AttnArgs& p, const Kv8RowInfo& ri, int row, int kvh, int slot0,
-                                           const float (&x)[Kv8Geo<HD>::NK][8], Kv8Col<HD, QHL>& c, float& vref) {
+                                           const float (&x)[Kv8Geo<HD>::NK][8], Kv8Col<HD, QHL>& c, Kv8Ref& vref) {
     constexpr int NK = Kv8Geo<HD>::NK, ND = Kv8Geo<HD>::ND;
     const int lane = threadIdx.x & 63, nl = lane & 15, kg = lane >> 4;
     const int last = (ri.len - 1) / BLK, t0 = last * BLK + slot0, tb = p.c.tail_dtype == ACMI_BF16;
@@ -721,13 +751,12 @@ __device__ __forceinline__ void kv8_tail16(const Kv8AttnArgs& p, const Kv8RowInf
         }
     }
     // in units of a scale like the blocks': largest value / 127
-    vref = wave_max(vmax) * (1.f / 127.f);
-    if (vref < 7.52316384526264e-37f) vref = 7.52316384526264e-37f;
-    const float iv = 1.f / vref;
+    vref.v = fmaxf(wave_max(vmax) * (1.f / 127.f), 7.52316384526264e-37f);
+    vref.inv = 1.f / vref.v;
 #pragma unroll
     for (int i = 0; i < ND; ++i)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) c.o[i][r] *= iv;
+        for (int r = 0; r < 4; ++r) c.o[i][r] *= vref.inv;
 }
 
 template <int HD, bool QHL, bool PHL>
@@ -776,7 +805,7 @@ __global__ __launch_bounds__(kv8_nw<HD>() * 64, kv8_wpe<HD>()) void kv8_attn_spl
     Kv8Col<HD, QHL> c[1];
     kv8_column<HD, QHL>(p, ri, qt * 16 + nl, x, c[0]);
     const bool mine = split == sp.eff - 1;   // the split that owns the tail
-    float vref = 0.f;
+    Kv8Ref vref = {0.f, 0.f};
     if (mine && sp.tail && wave < 4 && (ri.len - 1) / BLK * BLK + wave * 16 < ri.len) kv8_tail16<HD, QHL>(p, ri, row, kvh, wave * 16, x, c[0], vref);
     while (b < s1) {
         // the next requests are not conditional (a wave's last ones read its last block again, from the cache): the waits of a
@@ -789,7 +818,7 @@ __global__ __launch_bounds__(kv8_nw<HD>() * 64, kv8_wpe<HD>()) void kv8_attn_spl
         get_v(rq);
         b = nb;
     }
-    const float unit = vref * (1.f / 256.f);
+    const float unit = vref.v * (1.f / 256.f);
 #pragma unroll
     for (int i = 0; i < ND; ++i) {
         f32x4 o = c[0].o[i];
@@ -840,7 +869,7 @@ __global__ __launch_bounds__(kv8_nw<HD>() * 64, kv8_wpe<HD>()) void kv8_attn_spl
             for (int r = 0; r < 4; ++r) o[r] = fmaf(f, y[r], o[r]);
         }
         if (sp.eff == 1) {
-            const int s = cidx / p.G, g = cidx - s * p.G;
+            const int s = kv8_query(p, cidx), g = cidx - s * p.G;
             const bool none = s >= ri.qlen || den == 0.f;
 #pragma unroll
             for (int r = 0; r < 4; ++r) o[r] = none ? 0.f : o[r] / den;
@@ -891,7 +920,7 @@ __global__ __launch_bounds__(256) void kv8_attn_join_kernel(const Kv8AttnArgs p)
 #pragma unroll
         for (int r = 0; r < 4; ++r) o[r] += v[r];
     }
-    const int s = cidx / p.G, g = cidx - s * p.G;
+    const int s = kv8_query(p, cidx), g = cidx - s * p.G;
     const bool none = s >= ri.qlen || den == 0.f;
 #pragma unroll
     for (int r = 0; r < 4; ++r) o[r] = none ? 0.f : o[r] / den;
@@ -901,8 +930,8 @@ __global__ __launch_bounds__(256) void kv8_attn_join_kernel(const Kv8AttnArgs p)
 // ---- many queries: a workgroup's 4 waves own QB column tiles each and walk the blocks together.  Every wave converts a quarter of
 // the next block's codes to f16 fragments in LDS while this block is multiplied (two buffers, one barrier per block).  The tail
 // is staged the same way, relative to a power of two, as f16 (bf16 tails: exact) or a pair of f16 (f32 tails).
-// All workgroups of a (row, cache head) run on one XCD (workgroup i on XCD i % 8), so its codes are read once into one L2;
-// the longest (last) tiles first.
+// All workgroups of a (row, cache head) run on one XCD (workgroup i on XCD i % 8), whose L2 then holds its codes; the last (causal:
+// longest) tiles of all pairs go first, the short ones fill the end.
 template <int HD> struct Kv8ManyLds {
     f16x8 k[2][4 * Kv8Geo<HD>::NK][64], v[2][2 * Kv8Geo<HD>::ND][64];
     float red[2][4];
@@ -918,15 +947,16 @@ __global__ __launch_bounds__(256, KV8_WPE) void kv8_attn_many_kernel(const Kv8At
     __shared__ Kv8ManyLds<HD> sm;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int nl = lane & 15, kg = lane >> 4, cols = p.S * p.G;
-    const int li = blockIdx.x >> 3, grp = (blockIdx.x & 7) + 8 * (li / p.tiles), tile = p.tiles - 1 - li % p.tiles;
+    const int gpx = (p.c.rows * p.c.H + 7) >> 3, li = blockIdx.x >> 3, tq = li / gpx;   // (row, cache head) pairs per XCD
+    const int grp = (blockIdx.x & 7) + 8 * (li - tq * gpx), tile = p.tiles - 1 - tq;
     if (grp >= p.c.rows * p.c.H) return;
-    const int row = grp / p.c.H, kvh = grp - row * p.c.H;
+    const int row = __builtin_amdgcn_readfirstlane(grp / p.c.H), kvh = grp - row * p.c.H;
     const int w0 = tile * 64 * QB, c0 = w0 + wave * 16 * QB;   // first column of the workgroup, of the wave
     const Kv8RowInfo ri = kv8_row(p, row);
     const Kv8Span sp = kv8_span(p, ri, w0, min(w0 + 64 * QB, cols));
     Kv8Span me = kv8_span(p, ri, min(c0, cols - 1), min(c0 + 16 * QB, cols));
     if (c0 >= cols) { me.live = me.tail = false; me.bf = me.bt = 0; }
-    float vref = 0.f;
+    Kv8Ref vref = {0.f, 0.f};
     const size_t rh = (size_t)row * p.c.H + kvh, hb = rh * p.c.nblk;
     const uint8_t* kc = reinterpret_cast<const uint8_t*>(p.c.k_codes) + hb * (size_t)(BLK * HD);
     const uint8_t* vc = reinterpret_cast<const uint8_t*>(p.c.v_codes) + hb * (size_t)(BLK * HD);
@@ -1116,10 +1146,10 @@ __global__ __launch_bounds__(256, KV8_WPE) void kv8_attn_many_kernel(const Kv8At
     }
 #pragma unroll
     for (int g = 0; g < QB; ++g) {
-        const int cidx = c0 + g * 16 + nl, s = cidx / p.G, h = cidx - s * p.G;
+        const int cidx = c0 + g * 16 + nl, s = kv8_query(p, cidx), h = cidx - s * p.G;
         if (cidx >= cols) continue;
         const bool zero = s >= ri.qlen || c[g].l == 0.f;
-        const float inv = vref / c[g].l;
+        const float inv = vref.v / c[g].l;
 #pragma unroll
         for (int i = 0; i < ND; ++i) {
             f32x4 o;
@@ -1237,7 +1267,8 @@ extern "C" int acmi_kv8_attn(const acmi_kv8_cache* cache, const acmi_kv8_attn_de
     ACMI_REQUIRE(d.past_context >= 0 && (d.past_context == 0 || d.causal), "acmi_kv8_attn: past_context=%d needs causal", d.past_context);
     Kv8AttnArgs a = {};
     a.c = *cache; a.q = d.q; a.q_bf16 = d.q_dtype == ACMI_BF16; a.q_row = d.q_row; a.q_tok = d.q_tok; a.q_head = d.q_head;
-    a.S = d.S; a.Hq = d.Hq; a.G = d.Hq / cache->H;
+    a.S = d.S; a.Hq = d.Hq; a.G = d.Hq / cache->H; a.rG = 1.0f / (float)a.G;
+    ACMI_REQUIRE((long long)d.S * a.G <= (1 << 21), "acmi_kv8_attn: S=%d x %d query heads per cache head (at most 2^21)", d.S, a.G);
     a.len = d.len; a.len_stride = d.len_stride; a.len_bias = d.len_bias; a.q_len = d.q_len; a.start_rows = d.start_rows;
     a.causal = d.causal != 0; a.past = d.past_context;
     a.kn = d.k_new; a.vn = d.v_new; a.n_bf16 = d.new_dtype == ACMI_BF16;
