@@ -71,7 +71,8 @@ class LMLayer(C.Structure):
                 ('b_out', vp), ('b_cout', vp), ('b_ff2', vp), ('b_mq', vp), ('cvt_cache', vp),
                 ('q_ln_g', vp), ('q_ln_b', vp), ('k_ln_g', vp), ('k_ln_b', vp), ('cq_ln_g', vp), ('cq_ln_b', vp),
                 ('n1_g', vp), ('n1_b', vp), ('nc_g', vp), ('nc_b', vp), ('n2_g', vp), ('n2_b', vp),
-                ('w_qkvs', vp), ('b_qkvs', vp), ('cs_qkvs', vp), ('w_g2', vp), ('b_gs', vp), ('xs_u', vp), ('xs_cs', vp), ('xs_bs', vp)]
+                ('w_qkvs', vp), ('b_qkvs', vp), ('cs_qkvs', vp), ('w_g2', vp), ('b_gs', vp), ('xs_u', vp), ('xs_cs', vp), ('xs_bs', vp),
+                ('kv8', vp)]
 
 
 class LMModelDesc(C.Structure):
@@ -89,7 +90,8 @@ class LMState(C.Structure):
                 ('use_sampling', i32), ('temp', f32), ('top_k', i32), ('top_p', f32), ('cfg_coef', f32),
                 ('seed', u64), ('cfg_coef_beta', f32), ('cross_len_rows', vp), ('rope_first', i32), ('rope_shift', i32),
                 ('xshift', vp), ('cross_active_rows', i32), ('pf_xn', vp), ('pf_vt', vp), ('pf_tcap', i32), ('cvt_tcap', i32),
-                ('row_off', vp), ('input_add', vp), ('n_add', i32), ('xs_rows', i32), ('qkv_hand', vp), ('hand_err', vp)]
+                ('row_off', vp), ('input_add', vp), ('n_add', i32), ('xs_rows', i32), ('qkv_hand', vp), ('hand_err', vp),
+                ('pf_k', vp), ('pf_v', vp), ('kv8_work', vp)]
 
 
 def _sig(name, argtypes, restype=i32):
@@ -680,16 +682,20 @@ def launch(device: torch.device, what: str, fn, *args):
 
 
 def kv8_store(cache: KV8CacheDesc, k, v, start, n):
-    """k / v [rows, L, H, hd] (any strides over the first three), start / n int32 [rows] (n None: L)."""
+    """k / v [rows, L, H, hd] (any strides over the first three), start / n int32 [rows] (None: 0, L)."""
     ks, vs = k.stride(), v.stride()
     d = KV8StoreDesc(k.data_ptr(), v.data_ptr(), dtype_code(k.dtype), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], k.shape[1],
-                     start.data_ptr(), None if n is None else n.data_ptr())
+                     None if start is None else start.data_ptr(), None if n is None else n.data_ptr())
     launch(k.device, 'acmi_kv8_store', _kv8_store, C.byref(cache), C.byref(d))
 
 
 def kv8_load(cache: KV8CacheDesc, lens, T, k_out, v_out):
     launch(k_out.device, 'acmi_kv8_load', _kv8_load, C.byref(cache), lens.data_ptr(), T, k_out.data_ptr(), v_out.data_ptr(),
            dtype_code(k_out.dtype))
+
+
+def kv8_attn_work_floats(cache: KV8CacheDesc, S: int, Hq: int) -> int:
+    return int(_kv8_attn_work(C.byref(cache), S, Hq))
 
 
 def kv8_attn(cache: KV8CacheDesc, q, q_strides, S, out, lens, len_bias=0, causal=True, past_context=0, q_lens=None, starts=None,

@@ -172,7 +172,7 @@ __global__ __launch_bounds__(256) void kv8_store_kernel(const Kv8StoreArgs p) {
     __shared__ Kv8QuantLds<HD> sm;
     const int j = blockIdx.x, h = blockIdx.y, row = blockIdx.z;
     const int cap = p.c.nblk * BLK, tb = p.c.tail_dtype == ACMI_BF16;
-    const int start = p.start[row];
+    const int start = p.start != nullptr ? p.start[row] : 0;
     const int n = min(p.n != nullptr ? p.n[row] : p.L, p.L);
     if (start < 0 || start >= cap || n <= 0) return;
     const int end = (int)min((long long)start + n, (long long)cap);
@@ -585,7 +585,6 @@ __device__ __forceinline__ void kv8_column(const Kv8AttnArgs& p, const Kv8RowInf
 
 // the blocks of codes a column tile visits, and how many workgroups share them
 struct Kv8Span { int bf, bt, eff; bool live, tail; };
-constexpr int KV8_MIN_BLOCKS = 8;   // blocks per workgroup below which no further split is made
 constexpr int KV8_MAX_SPLITS = 64;
 #ifndef KV8_TARGET
 #define KV8_TARGET 512
@@ -1188,7 +1187,7 @@ static bool kv8_rows_ok(const void* p, int es, long long a, long long b, long lo
 
 extern "C" int acmi_kv8_store(const acmi_kv8_cache* cache, const acmi_kv8_store_desc* desc, void* stream) {
     if (int rc = kv8_check(cache, "acmi_kv8_store")) return rc;
-    ACMI_REQUIRE(desc != nullptr && desc->start != nullptr, "acmi_kv8_store: null descriptor or start");
+    ACMI_REQUIRE(desc != nullptr, "acmi_kv8_store: null descriptor");
     ACMI_REQUIRE(desc->L >= 0 && desc->L <= (1 << 30) && kv8_dtype_ok(desc->dtype), "acmi_kv8_store: L=%d dtype=%d", desc->L, desc->dtype);
     if (desc->L == 0) return ACMI_OK;
     ACMI_REQUIRE(desc->k && desc->v, "acmi_kv8_store: null k or v");
@@ -1232,7 +1231,8 @@ static bool kv8_few(int S, int G) { return (S * G + 15) / 16 <= KV8_SPLIT_TILES;
 static void kv8_split_plan(const acmi_kv8_cache* c, int S, int G, int* splits, int* chunk) {
     const long long tiles = (long long)c->H * ((S * G + 15) / 16) * c->rows;
     long long n = 1;
-    if (tiles * 4 <= KV8_TARGET) n = max(1LL, min(min(KV8_TARGET / tiles, (long long)(c->nblk / KV8_MIN_BLOCKS)), (long long)KV8_MAX_SPLITS));
+    const int least = 4 * (c->hd == 128 ? kv8_nw<128>() : kv8_nw<64>());   // four blocks per wave: below, the second launch costs more
+    if (tiles * 4 <= KV8_TARGET) n = max(1LL, min(min(KV8_TARGET / tiles, (long long)(c->nblk / least)), (long long)KV8_MAX_SPLITS));
     *chunk = (int)((c->nblk + n - 1) / n);
     *splits = (c->nblk + *chunk - 1) / *chunk;
 }

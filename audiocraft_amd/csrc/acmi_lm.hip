@@ -33,6 +33,7 @@ struct EmbedArgs {
     int npos_pad, npos; // > 0: position-minor rows of the MFMA-tiled prefill (row = cache row * npos_pad + position; pad
                         // rows repeat the last position: finite, never stored to the caches); 0: row = position * Beff + cache row
     const float* input_add; int n_add;   // ADD variant only: acmi_lm_state.input_add / n_add (fuser 'sum' / 'input_interpolate')
+    int* tail_pos;      // 8-bit cache: receives the position inside its newest block (acmi_lm_layer.kv8), or NULL
 };
 
 // BF16: element type of the tables; KQ >= n_q: codebook tables read per row (compile time, so that every load of a phase
@@ -48,6 +49,7 @@ __global__ __launch_bounds__(256) void embed_kernel(const EmbedArgs p) {
     if (p.npos_pad > 0) { m0 = m / p.npos_pad; pidx = min(m - m0 * p.npos_pad, p.npos - 1); }
     else { pidx = m / p.Beff; m0 = m - pidx * p.Beff; }
     const int g = *p.pos + pidx;
+    if (p.tail_pos != nullptr && m == 0 && threadIdx.x == 0) *p.tail_pos = g % ACMI_KV8_BLOCK;   // (one position per call)
     const int gpos = p.row_off != nullptr ? max(g - p.row_off[m0], 0) : g;   // the row's own position (left-padded streams)
     const int b = m0 % p.B;
     float loc[8];  // d <= 2048
@@ -780,11 +782,14 @@ static int lm_prefill_big(const acmi_lm_model* m, const acmi_lm_state* s, hipStr
     };
     for (int li = 0; li < m->num_layers; ++li) {
         const acmi_lm_layer& L = m->layers[li];
+        // 8-bit cache: the prompt attends to itself in kvdtype (one layer's keys and values in scratch), then enters the cache
+        void* const kc = L.kv8 ? s->pf_k : L.k_cache; void* const vc = L.kv8 ? s->pf_v : L.v_cache;
+        const int Tcap = L.kv8 ? s->pf_tcap : s->Tmax;
         if ((rc = acmi_launch_ln_tile(s->x, s->pf_xn, m->wdtype, M, d, tile_eps, nullptr, 0, st))) return rc;
         {
             BigArgs b = big(s->pf_xn, L.w_qkv, L.b_qkv, 3 * d, d, ACMI_BIG_QKV);
-            b.q_out = s->q; b.k_cache = L.k_cache; b.v_cache = L.v_cache; b.vt = s->pf_vt; b.kv_bf16 = kvbf;
-            b.H = H; b.hd = hd; b.Tcap = s->Tmax; b.d = d; b.npos = npos; b.npos_pad = npp; b.vt_tcap = s->pf_tcap; b.pos = s->pos;
+            b.q_out = s->q; b.k_cache = kc; b.v_cache = vc; b.vt = s->pf_vt; b.kv_bf16 = kvbf;
+            b.H = H; b.hd = hd; b.Tcap = Tcap; b.d = d; b.npos = npos; b.npos_pad = npp; b.vt_tcap = s->pf_tcap; b.pos = s->pos;
             if ((rc = acmi_launch_big(b, m->wdtype, st))) return rc;
         }
         if (L.q_ln_g != nullptr || L.k_ln_g != nullptr) {   // qk_layer_norm on the q rows and the K rows just stored (before the rotary positions)
@@ -804,11 +809,17 @@ static int lm_prefill_big(const acmi_lm_model* m, const acmi_lm_state* s, hipStr
             hipLaunchKernelGGL(rope_qk_kernel, dim3(M), dim3(d / 2), 0, st, ra);
             if ((rc = acmi_check_launch("rope_qk_kernel"))) return rc;
         }
+        if (L.kv8) {
+            acmi_kv8_store_desc ks = {};
+            ks.k = kc; ks.v = vc; ks.dtype = m->kvdtype; ks.L = npos;
+            ks.k_row = ks.v_row = (long long)H * Tcap * hd; ks.k_tok = ks.v_tok = hd; ks.k_head = ks.v_head = (long long)Tcap * hd;
+            if ((rc = acmi_kv8_store(reinterpret_cast<const acmi_kv8_cache*>(L.kv8), &ks, (void*)st))) return rc;
+        }
         if (li == m->num_layers - 1) break;   // the last layer only owes its K / V: no position of this call is sampled from
         {
             PrefillAttnArgs pa = {};
-            pa.q = s->q; pa.k_cache = L.k_cache; pa.vt = s->pf_vt; pa.out = s->att; pa.out_bf16 = wbf; pa.out_rbs = nkc_d;
-            pa.H = H; pa.Tcap = s->Tmax; pa.vt_tcap = s->pf_tcap; pa.npos = npos; pa.npos_pad = npp; pa.pos = s->pos;
+            pa.q = s->q; pa.k_cache = kc; pa.vt = s->pf_vt; pa.out = s->att; pa.out_bf16 = wbf; pa.out_rbs = nkc_d;
+            pa.H = H; pa.Tcap = Tcap; pa.vt_tcap = s->pf_tcap; pa.npos = npos; pa.npos_pad = npp; pa.pos = s->pos;
             pa.past_context = m->past_context; pa.causal = 1;
             if ((rc = acmi_launch_prefill_attn(pa, m->kvdtype, hd, s->Beff, st))) return rc;
         }
@@ -864,9 +875,29 @@ static int lm_prefill_big(const acmi_lm_model* m, const acmi_lm_state* s, hipStr
     return acmi_check_launch("advance_kernel");
 }
 
+// the 8-bit caches of a model (acmi_lm_layer.kv8): on every layer or none, of the step's geometry
+static int check_kv8(const acmi_lm_model* m, const acmi_lm_state* s, bool prefill) {
+    const bool on = m->layers[0].kv8 != nullptr;
+    for (int li = 0; li < m->num_layers; ++li) {
+        const acmi_lm_layer& L = m->layers[li];
+        ACMI_REQUIRE((L.kv8 != nullptr) == on, "acmi_lm_step: kv8 on every layer or none");
+        if (!on) continue;
+        const acmi_kv8_cache& c = *reinterpret_cast<const acmi_kv8_cache*>(L.kv8);
+        ACMI_REQUIRE(c.rows == s->Beff && c.H == m->num_heads && c.H * c.hd == m->dim && c.tail_dtype == m->kvdtype && c.nblk * ACMI_KV8_BLOCK >= s->Tmax,
+                     "acmi_lm_step: kv8 of layer %d does not fit (rows %d heads %d hd %d blocks %d)", li, c.rows, c.H, c.hd, c.nblk);
+        ACMI_REQUIRE(m->rope_freq == nullptr && L.q_ln_g == nullptr && L.k_ln_g == nullptr, "acmi_lm_step: kv8 with rotary positions or qk_layer_norm");
+    }
+    ACMI_REQUIRE(!on || (prefill ? s->pf_k != nullptr && s->pf_v != nullptr : s->n_pos <= 1),
+                 "acmi_lm_step: kv8 needs pf_k / pf_v in the one-forward prefill and one position per call elsewhere");
+    return ACMI_OK;
+}
+
 extern "C" int acmi_lm_step(const acmi_lm_model* m, const acmi_lm_state* s, int mode, void* stream) {
     hipStream_t st = (hipStream_t)stream;
     ACMI_REQUIRE(m && s, "acmi_lm_step: null argument");
+    ACMI_REQUIRE(m->num_layers > 0 && m->layers != nullptr, "acmi_lm_step: no layers");
+    if (int rc = check_kv8(m, s, mode == ACMI_STEP_PREFILL && s->pf_xn != nullptr && s->n_pos > 1)) return rc;
+    const bool kv8 = m->layers[0].kv8 != nullptr;
     if (mode == ACMI_STEP_PREFILL && s->pf_xn != nullptr && s->n_pos > 1) {
         ACMI_REQUIRE(s->row_off == nullptr, "acmi_lm_step: the one-forward prefill does not take left-padded streams (row_off)");
         ACMI_REQUIRE(m->dim % m->num_heads == 0 && m->n_q <= 16 && s->use_cfg >= ACMI_CFG_NONE && s->use_cfg <= ACMI_CFG_DOUBLE &&
@@ -936,7 +967,7 @@ extern "C" int acmi_lm_step(const acmi_lm_model* m, const acmi_lm_state* s, int 
     const bool fuse_qkv = mode == ACMI_STEP_DECODE && npos == 1 && s->qkv_hand != nullptr && s->hand_err != nullptr && wbf && kvbf &&
                           hd == 64 && c.lnm == LN_FOLD && c.gram && M <= fuse_rows && !post && !xs && m->rope_freq == nullptr &&
                           m->past_context <= 0 && s->row_off == nullptr && c.nkc_d % 4 == 0 && c.nkc_d / 4 <= 16 && s->Tmax <= 0xffff &&
-                          d % c.kt == 0;
+                          d % c.kt == 0 && !kv8;
 
     EmbedArgs e = {};
     for (int k = 0; k < m->n_q; ++k) e.emb[k] = m->emb[k];
@@ -944,6 +975,7 @@ extern "C" int acmi_lm_step(const acmi_lm_model* m, const acmi_lm_state* s, int 
     e.prepend = s->prepend; e.P = s->prepend ? s->n_prepend : 0; e.pos_table = m->pos_table;
     e.pos_scale = m->positional_scale; e.pos = s->pos; e.x = s->x; e.d = d; e.stats = s->stats; e.row_off = s->row_off;
     if (c.lnm == LN_FOLD) { e.xt_hi = c.xh; e.xt_lo = c.use_lo ? c.xl : nullptr; e.xt_nkc = c.rbs; e.xt_lo_nkc = c.nkc_d; }
+    e.tail_pos = kv8 ? s->pos + 2 : nullptr;
     e.input_add = s->input_add; e.n_add = s->n_add;
     if (shifted) { e.shift_out = shbuf[0]; c.xsh = shbuf[0]; }
 #define ACMI_EMBED_CASE(KQv)                                                                        \
@@ -986,6 +1018,10 @@ extern "C" int acmi_lm_step(const acmi_lm_model* m, const acmi_lm_state* s, int 
             a.mean_out = c.nsh;   // single-term mode: the row means of x0 = the shift of this layer's producers
             a.qkv = 1; a.q_out = s->q; a.k_cache = L.k_cache; a.v_cache = L.v_cache; a.kv_bf16 = kvbf;
             a.H = H; a.hd = hd; a.Tcap = s->Tmax; a.d = d; a.pos = s->pos; a.rpp = s->Beff;
+            if (kv8) {   // into the newest block, at the position inside it (embed_kernel has left it in pos[2])
+                const acmi_kv8_cache& c8 = *reinterpret_cast<const acmi_kv8_cache*>(L.kv8);
+                a.k_cache = c8.k_tail; a.v_cache = c8.v_tail; a.Tcap = ACMI_KV8_BLOCK; a.pos = s->pos + 2;
+            }
             if (xs) {     // + the x0 part of the folded cross-attention scores: R H Lc raw features -> r viewed as [M, R H Lc]
                 ACMI_REQUIRE(L.w_qkvs && L.b_qkvs && L.cs_qkvs && L.w_g2 && L.xs_u && L.xs_cs && L.xs_bs,
                              "acmi_lm_step: xs_rows > 0 needs the folded cross-attention tables on every layer");
@@ -1013,7 +1049,16 @@ extern "C" int acmi_lm_step(const acmi_lm_model* m, const acmi_lm_state* s, int 
         }
         // self attention over positions [0, g]; output in A-fragment order for the out projection: into `att`,
         // or next to x ([x | att], columns d_pad ..) when the out projection is paired with the cross query
-        {
+        if (kv8) {
+            acmi_kv8_attn_desc ka = {};
+            ka.q = s->q; ka.q_dtype = ACMI_F32; ka.q_row = d; ka.q_head = hd; ka.S = 1; ka.Hq = H;
+            ka.len = s->pos; ka.len_stride = 0; ka.len_bias = 1; ka.start_rows = s->row_off; ka.causal = 1;
+            ka.past_context = m->past_context > 0 ? m->past_context : 0; ka.complete = 1; ka.work = s->kv8_work;
+            ka.out_mode = ACMI_OUT_TILED; ka.out_dtype = m->wdtype;
+            if (pair) { ka.out = c.xh; ka.out_rbs = c.rbs; ka.out_col0 = c.nkc_d * c.kt; }
+            else { ka.out = s->att; ka.out_rbs = c.nkc_d; }
+            if ((rc = acmi_kv8_attn(reinterpret_cast<const acmi_kv8_cache*>(L.kv8), &ka, stream))) return rc;
+        } else {
         acmi_attn_desc sa = {};
         sa.q = s->q; sa.k_cache = L.k_cache; sa.v_cache = L.v_cache; sa.kvdtype = m->kvdtype;
         sa.out_mode = ACMI_OUT_TILED; sa.out_dtype = m->wdtype; sa.Beff = M; sa.H = H; sa.hd = hd; sa.Tcap = s->Tmax;

@@ -28,6 +28,7 @@ import torch
 from torch import nn
 
 from .. import _C
+from ..modules.kv8_cache import KV8Cache
 from ..modules.codebooks_patterns import CodebooksPatternProvider
 from ..modules.conditioners import (ClassifierFreeGuidanceDropout, ConditionFuser, ConditioningAttributes,
                                     ConditioningProvider, ConditionType, _drop_description_condition)
@@ -135,7 +136,9 @@ class LMModel(nn.Module):
 
     Args mirror `audiocraft.models.lm.LMModel.__init__` (lm.py:145-177) plus:
         weight_dtype: torch.bfloat16 (bench / serving) or torch.float32 (parity mode) for the packed matrices.
-        kv_dtype: dtype of the KV caches (defaults to weight_dtype).
+        kv_dtype: dtype of the KV caches (defaults to weight_dtype).  torch.int8: the self-attention cache in 8 bits with a scale
+            for each block of 64 positions and head (modules/kv8_cache.py: the newest 1 .. 64 positions exact in weight_dtype),
+            half the bytes that a decode step reads per past position; the cross-attention caches stay in weight_dtype.
     Beyond the MusicGen configuration the decode step also implements the transformer options no release uses
     (config/model/lm/default.yaml:25-46): positional_embedding 'rope' / 'sin_rope' (+ xpos), past_context, layer_scale,
     kv_repeat (the shared key / value heads are laid out per query head when the weights are packed: no kernel knows),
@@ -196,7 +199,12 @@ class LMModel(nn.Module):
         self.positional_scale = positional_scale
         self.has_cross_attention = cross_attention
         self.weight_dtype = weight_dtype
-        self.kv_dtype = kv_dtype or weight_dtype
+        # int8: the self-attention cache in 8 bits; its newest block and the cross-attention caches in weight_dtype
+        self.kv_int8 = kv_dtype == torch.int8
+        if self.kv_int8 and (positional_embedding != 'sin' or self.qk_layer_norm or dim // num_heads not in (16, 32, 64, 128)):
+            raise NotImplementedError("kv_dtype=torch.int8 with rotary positions or qk_layer_norm (both rewrite the appended key), or a "
+                                      "head size other than 16, 32, 64, 128")
+        self.kv_dtype = weight_dtype if kv_dtype is None or self.kv_int8 else kv_dtype
         self.emb = nn.ModuleList([nn.Embedding(card + 1, dim, device=device) for _ in range(n_q)])
         rope = None
         if positional_embedding in ('rope', 'sin_rope'):
@@ -543,8 +551,13 @@ class LMModel(nn.Module):
                              f"longer audio through MusicGen's windowed generation (extend_stride)")
         f32 = dict(device=dev, dtype=torch.float32)
         run: dict = {'key': key, 'Beff': Beff, 'graphs': {}}
-        run['k'] = torch.zeros(self.num_layers, Beff, H, Tmax, hd, device=dev, dtype=self.kv_dtype)
-        run['v'] = torch.zeros(self.num_layers, Beff, H, Tmax, hd, device=dev, dtype=self.kv_dtype)
+        if self.kv_int8:
+            run['kv8'] = [KV8Cache(Beff, H, hd, Tmax, dtype=self.kv_dtype, device=dev) for _ in range(self.num_layers)]
+            nw = _C.kv8_attn_work_floats(run['kv8'][0].desc, 1, H)
+            run['kv8_work'] = torch.empty(nw, **f32) if nw else None
+        else:
+            run['k'] = torch.zeros(self.num_layers, Beff, H, Tmax, hd, device=dev, dtype=self.kv_dtype)
+            run['v'] = torch.zeros(self.num_layers, Beff, H, Tmax, hd, device=dev, dtype=self.kv_dtype)
         if self.has_cross_attention:
             run['ck'] = torch.zeros(self.num_layers, Beff, H, max(Lc, 1), hd, device=dev, dtype=self.kv_dtype)
             run['cv'] = torch.zeros(self.num_layers, Beff, H, max(Lc, 1), hd, device=dev, dtype=self.kv_dtype)
@@ -553,7 +566,12 @@ class LMModel(nn.Module):
             run['cvt'] = torch.zeros(self.num_layers, Beff, H, hd, run['cvt_tcap'], device=dev, dtype=self.kv_dtype)
         for li in range(self.num_layers):
             L = pk['layers'][li]
-            L.k_cache, L.v_cache = run['k'][li].data_ptr(), run['v'][li].data_ptr()
+            if self.kv_int8:
+                L.k_cache = L.v_cache = None
+                L.kv8 = C.addressof(run['kv8'][li].desc)
+            else:
+                L.k_cache, L.v_cache = run['k'][li].data_ptr(), run['v'][li].data_ptr()
+                L.kv8 = None
             if self.has_cross_attention:
                 L.ck_cache, L.cv_cache = run['ck'][li].data_ptr(), run['cv'][li].data_ptr()
                 L.cvt_cache = run['cvt'][li].data_ptr()
@@ -661,6 +679,7 @@ class LMModel(nn.Module):
         st.cfg_coef, st.seed = float(cfg_coef), int(seed) & ((1 << 64) - 1)
         st.qkv_hand = run['qkv_hand'].data_ptr() if 'qkv_hand' in run else None
         st.hand_err = run['hand_err'].data_ptr() if 'qkv_hand' in run else None
+        st.kv8_work = run['kv8_work'].data_ptr() if run.get('kv8_work') is not None else None
         return st
 
     def _project_cross_kv(self, run, cross_src: torch.Tensor):
@@ -1045,17 +1064,22 @@ class LMModel(nn.Module):
                   'att': _C.tiled_activation_buffer(rows_a, d, self.weight_dtype, dev),
                   'hidden': _C.tiled_activation_buffer(rows_a, self.ffn_dim, self.weight_dtype, dev),
                   'vt': torch.zeros(Beff * H * (d // H) * tcap_a, device=dev, dtype=self.kv_dtype)}
+            if self.kv_int8:   # one layer's keys and values of the prompt (acmi_lm_state.pf_k)
+                pf['k'], pf['v'] = (torch.zeros(Beff * H * (d // H) * tcap_a, device=dev, dtype=self.kv_dtype) for _ in range(2))
             run['pf'] = pf
         saved = (state.x, state.q, state.stats, state.att, state.hidden)
         state.x, state.q, state.stats = pf['x'].data_ptr(), pf['q'].data_ptr(), pf['stats'].data_ptr()
         state.att, state.hidden = pf['att'].data_ptr(), pf['hidden'].data_ptr()
         state.pf_xn, state.pf_vt, state.pf_tcap = pf['xn'].data_ptr(), pf['vt'].data_ptr(), tcap
+        if self.kv_int8:
+            state.pf_k, state.pf_v = pf['k'].data_ptr(), pf['v'].data_ptr()
         state.n_pos = n_positions
         try:
             _C.lm_step(desc, state, _C.STEP_PREFILL)
         finally:
             state.x, state.q, state.stats, state.att, state.hidden = saved
             state.pf_xn, state.pf_vt, state.pf_tcap = None, None, 0
+            state.pf_k = state.pf_v = None
             state.n_pos = 1
 
     def _prefill(self, desc, state, n_positions: int, start: int = 0):
@@ -1068,7 +1092,7 @@ class LMModel(nn.Module):
             return self._prefill_big(desc, state, self._run, n_positions)
         done = 0
         while done < n_positions:
-            state.n_pos = min(self.PREFILL_CHUNK, n_positions - done)
+            state.n_pos = min(1 if self.kv_int8 else self.PREFILL_CHUNK, n_positions - done)   # (int8: a token at a time into the newest block)
             _C.lm_step(desc, state, _C.STEP_PREFILL)
             done += state.n_pos
         state.n_pos = 1
@@ -1151,7 +1175,9 @@ class LMModel(nn.Module):
 
     def get_streaming_state(self) -> tp.Dict[str, torch.Tensor]:
         """Key names of the reference (streaming.py:75-86): `transformer.offsets`,
-        `fuser.offsets`, `transformer.layers.{i}.self_attn.past_keys|past_values|offset`.  K / V: [B, H, t, hd] views."""
+        `fuser.offsets`, `transformer.layers.{i}.self_attn.past_keys|past_values|offset`.  K / V: [B, H, t, hd] views (with
+        kv_dtype=torch.int8 copies of the values the cache stands for: restoring them quantises again, to the same codes; a block
+        that was still exact when the state was taken and is rewound INTO later keeps the values of the state)."""
         st = getattr(self, '_stream', None)
         if st is None:
             return {}
@@ -1169,8 +1195,13 @@ class LMModel(nn.Module):
         for li in range(self.num_layers):
             pre = f'transformer.layers.{li}.self_attn.'
             # kv_repeat: the caches hold every shared head once per query head; the state lists the H / kv_repeat stored heads
-            state[pre + 'past_keys'] = run['k'][li][:, ::self.kv_repeat, :t]
-            state[pre + 'past_values'] = run['v'][li][:, ::self.kv_repeat, :t]
+            if self.kv_int8:   # copies, the values the 8-bit cache stands for
+                lens = torch.full((run['Beff'],), t, dtype=torch.int32, device=dev)
+                k, v = run['kv8'][li].load(lens, t, dtype=self.kv_dtype)
+            else:
+                k, v = run['k'][li][:, :, :t], run['v'][li][:, :, :t]
+            state[pre + 'past_keys'] = k[:, ::self.kv_repeat]
+            state[pre + 'past_values'] = v[:, ::self.kv_repeat]
             state[pre + 'offset'] = torch.tensor(dropped, dtype=torch.long, device=dev)
         return state
 
@@ -1189,6 +1220,18 @@ class LMModel(nn.Module):
         pc = self.past_context
         for li in range(self.num_layers):
             pre = f'transformer.layers.{li}.self_attn.'
+            if self.kv_int8:
+                kv = []
+                for name in ('past_keys', 'past_values'):
+                    src = state[pre + name]
+                    assert src.shape[2] == t, (src.shape, t)   # (a state trimmed to past_context does not say what its blocks held)
+                    if src.shape[1] != self.num_heads:
+                        src = src.repeat_interleave(self.kv_repeat, dim=1)
+                    kv.append(src.to(run['kv8'][li].device, self.kv_dtype).transpose(1, 2))
+                    known.add(pre + name)
+                run['kv8'][li].store(*kv)
+                known.add(pre + 'offset')
+                continue
             for name, cache in (('past_keys', run['k'][li]), ('past_values', run['v'][li])):
                 src = state[pre + name]
                 # full length (this class's own states) or trimmed to the last past_context keys (a reference-format state)

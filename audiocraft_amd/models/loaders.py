@@ -135,7 +135,7 @@ def lm_cfg_from_xp(cfg: dict) -> dict:
     return out
 
 
-def load_lm_model(file_or_id: str, device='cuda', weight_dtype=None):
+def load_lm_model(file_or_id: str, device='cuda', weight_dtype=None, kv_dtype=None):
     """reference loaders.py:111-126"""
     pkg = _get_state_dict(file_or_id, 'state_dict.bin')
     cfg = parse_cfg(pkg['xp.cfg'])
@@ -147,7 +147,7 @@ def load_lm_model(file_or_id: str, device='cuda', weight_dtype=None):
         w = state.get(f'condition_provider.conditioners.{name}.output_proj.weight')
         if w is not None and c['kind'] == 't5':
             c['dim'] = int(w.shape[1])
-    lm = builders.get_lm_model(lm_cfg, device, weight_dtype)
+    lm = builders.get_lm_model(lm_cfg, device, weight_dtype, kv_dtype)
     lm.load_state_dict(state)
     lm.cfg = cfg
     return lm

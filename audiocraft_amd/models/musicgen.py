@@ -42,10 +42,11 @@ class MusicGen(BaseGenModel):
 
     # ------------------------------------------------------------------------------------- construction
     @staticmethod
-    def get_pretrained(name: str = 'facebook/musicgen-melody', device=None, weight_dtype=None):
+    def get_pretrained(name: str = 'facebook/musicgen-melody', device=None, weight_dtype=None, kv_dtype=None):
         """'debug' builds the reference's debug geometry (musicgen.py:76-80).  Anything else is a released
         model name or a directory holding `state_dict.bin` + `compression_state_dict.bin` in the reference
-        export format, resolved on disk only (see `loaders.py`; there is no network here)."""
+        export format, resolved on disk only (see `loaders.py`; there is no network here).
+        kv_dtype: LMModel's (torch.int8: the self-attention cache in 8 bits)."""
         device = 'cuda' if device is None else device
         if name in _SHORT_NAMES:     # reference musicgen.py:83-87
             warnings.warn("MusicGen pretrained model relying on deprecated checkpoint mapping. "
@@ -55,20 +56,20 @@ class MusicGen(BaseGenModel):
             return MusicGen(name, builders.get_debug_compression_model(device), builders.get_debug_lm_model(device),
                             max_duration=30)
         from . import loaders
-        lm = loaders.load_lm_model(name, device=device, weight_dtype=weight_dtype)
+        lm = loaders.load_lm_model(name, device=device, weight_dtype=weight_dtype, kv_dtype=kv_dtype)
         # max_duration and the stereo codec wrapper come from the checkpoint's experiment config (BaseGenModel)
         return MusicGen(name, loaders.load_compression_model(name, device=device), lm)
 
     @staticmethod
     def get_random_init(name: str = 'facebook/musicgen-medium', device='cuda', weight_dtype=torch.bfloat16,
-                        text_len: int = 16, seed: int = 0):
+                        text_len: int = 16, seed: int = 0, kv_dtype=None):
         """Architecture of a released model with seeded random weights and synthetic conditioners: what
         bench.py runs, since neither checkpoints nor T5 weights exist offline."""
         scale, melody = _ARCH[name]
         stereo = '-stereo-' in name
         torch.manual_seed(seed)
         lm = builders.get_lm_model(builders.musicgen_lm_cfg(scale, melody, synthetic=True, text_len=text_len,
-                                                            stereo=stereo), device, weight_dtype)
+                                                            stereo=stereo), device, weight_dtype, kv_dtype)
         codec = builders.get_compression_model(builders.ENCODEC_32KHZ, device)
         if stereo:  # left / right through the mono codec, codebooks interleaved (reference encodec.py:397-506)
             codec = InterleaveStereoCompressionModel(codec)

@@ -79,15 +79,15 @@ class KV8Cache:
         return t if t.is_contiguous() else t.contiguous()
 
     # ------------------------------------------------------------------------------------- operators
-    def store(self, k: torch.Tensor, v: torch.Tensor, start: torch.Tensor, n: tp.Optional[torch.Tensor] = None) -> None:
+    def store(self, k: torch.Tensor, v: torch.Tensor, start: tp.Optional[torch.Tensor] = None, n: tp.Optional[torch.Tensor] = None) -> None:
         """Keys and values [rows, L, heads, head_dim] of the tokens start[r] .. start[r] + n[r] - 1 of every row (n None: all L;
-        start[r]: how many the row holds already).  Tokens past n[r] are padding and never read."""
+        start[r]: how many the row holds already, None: none).  Tokens past n[r] are padding and never read."""
         L = k.shape[1] if k.dim() == 4 else -1
         k = self._data('store', 'k', k, (self.rows, L, self.heads, self.head_dim))
         v = self._data('store', 'v', v, k.shape)
         if k.dtype != v.dtype:
             raise ValueError(f"KV8Cache.store: k is {k.dtype}, v is {v.dtype}")
-        start, n = self._words('store', 'start', start, True), self._words('store', 'n', n, False)
+        start, n = self._words('store', 'start', start, False), self._words('store', 'n', n, False)
         if L:
             _C.kv8_store(self.desc, k, v, start, n)
 

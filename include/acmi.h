@@ -234,6 +234,12 @@ typedef struct {
      * launch and the cross-out GEMM of the layer are gone.  All NULL = off. */
     const void* w_qkvs; const float* b_qkvs; const float* cs_qkvs; const void* w_g2; const float* b_gs;
     const void* xs_u; const float* xs_cs; const float* xs_bs;
+    /* 0.3.0: self-attention cache in 8 bits: host pointer to an acmi_kv8_cache of Beff rows, num_heads heads and tail_dtype ==
+     * kvdtype, or NULL (on every layer or none).  k_cache / v_cache are then unused; the step's QKV launch appends to the tail
+     * and its attention (acmi_kv8_attn) quantises a block that the position completes.  One position per call, or the one-forward
+     * prefill (which stores the whole prompt, acmi_kv8_store, after attending to it in kvdtype); no rotary positions, no
+     * qk_layer_norm (both rewrite the appended key), head size 16 .. 128. */
+    const void* kv8;
 } acmi_lm_layer;
 
 typedef struct {
@@ -286,7 +292,7 @@ typedef struct {
     int64_t* gen_sequence;  /* [B, K, S] int64; -1 = not generated yet (lm.py:523-534) */
     const uint8_t* seq_mask;/* [K, S] pattern validity mask (codebooks_patterns.py:138-151) */
     const float* prepend;   /* [Beff, P, d] f32 prepended condition rows (conditioners.py:1739-1741) or NULL */
-    int* pos;               /* device int[4]: pos[0] = current position index g (advanced by the step),
+    int* pos;               /* device int[4]: pos[0] = current position index g (advanced by the step), pos[2] = scratch (g % 64 with kv8),
                                pos[1] = scratch ticket counter (must be 0 between steps) */
     float* x;               /* [Beff, d] f32 residual stream */
     float* q;               /* [Beff, d] f32 */
@@ -363,6 +369,9 @@ typedef struct {
                                launch consume and re-arm them */
     int* hand_err;          /* [1]: number of hand-off polls that gave up (bounded spin); non-zero = the step's result is not to
                                be trusted (the caller checks it once per generate), and later launches do not spin again */
+    void* pf_k; void* pf_v; /* 0.3.0, one-forward prefill with acmi_lm_layer.kv8: [Beff, H, pf_tcap, hd] in kvdtype each, zero-initialised: the
+                               prompt's keys and values of one layer at a time */
+    float* kv8_work;        /* with acmi_lm_layer.kv8: acmi_kv8_attn_work_floats(kv8, 1, num_heads) floats (NULL where that is 0) */
 } acmi_lm_state;
 
 #define ACMI_CFG_NONE 0
@@ -638,7 +647,7 @@ typedef struct {
 } acmi_kv8_cache;
 
 /* Tokens start[r] .. start[r] + n[r] - 1 of every row r into the cache (n NULL: L each; start[r] = tokens the row holds
- * already, which must have been stored in order).  k / v: `dtype` elements at row * *_row + token * *_tok + head * *_head
+ * already, which must have been stored in order; start NULL: 0).  k / v: `dtype` elements at row * *_row + token * *_tok + head * *_head
  * (element strides), the hd features contiguous and every row 16-byte aligned; tokens >= n[r] of a row are never read. */
 typedef struct {
     const void* k; const void* v; int dtype;

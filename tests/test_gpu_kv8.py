@@ -404,6 +404,32 @@ def test_a_generation_captured_and_replayed(KV8Cache):
             assert torch.equal(a, b)
 
 
+def test_tiled_output_and_one_length_word(KV8Cache):
+    """The form the LM's decode step calls: the new token already in the tail, one length word for all rows, f32 queries, the
+    result as the next GEMM's tiled bf16 operand at a column offset; the block that the token completes is quantised."""
+    import ctypes
+    from audiocraft_amd import _C
+    R, H, hd, n = 5, 3, 64, 128
+    k, v = make(R, n, H, hd, torch.bfloat16, 30)
+    whole, c = KV8Cache(R, H, hd, n), KV8Cache(R, H, hd, n)
+    whole.store(k.cuda(), v.cuda())
+    c.store(k[:, :n - 1].cuda(), v[:, :n - 1].cuda())
+    c.k_tail[:, :, 63], c.v_tail[:, :, 63] = k[:, n - 1].cuda(), v[:, n - 1].cuda()
+    q = torch.randn(R, H * hd, generator=torch.Generator().manual_seed(5))
+    qd, pos, d = q.cuda(), words(n - 1), H * hd
+    out = _C.tiled_activation_buffer(R, 2 * d, torch.bfloat16, 'cuda')
+    desc = _C.KV8AttnDesc(q=qd.data_ptr(), q_dtype=_C.F32, q_row=d, q_head=hd, S=1, Hq=H, len=pos.data_ptr(), len_stride=0, len_bias=1,
+                          causal=1, complete=1, out=out.data_ptr(), out_mode=_C.OUT_TILED, out_dtype=_C.BF16, out_rbs=2 * d // 32, out_col0=d)
+    _C.check(_C._kv8_attn(ctypes.byref(c.desc), ctypes.byref(desc), _C.stream()), 'acmi_kv8_attn')
+    got = _C.untile_matrix(out, R, 2 * d)
+    assert (got[:, :d] == 0).all()
+    for r in range(R):
+        ref = attention(q[r].view(1, H, hd).double(), held(k[r].float()), held(v[r].float()), True, 1, 0, 0)
+        check(got[r, d:].view(1, H, hd), ref, torch.bfloat16, v[r].float().abs().max().item())
+    for name in ('k_codes', 'v_codes', 'k_scale', 'v_scale'):
+        assert torch.equal(getattr(c, name), getattr(whole, name))
+
+
 def test_another_stream(KV8Cache):
     c, k, v = filled(KV8Cache, [700], 2, 64, torch.float32, 14)
     q = torch.randn(1, 1, 2, 64, device='cuda')
@@ -436,7 +462,7 @@ def test_refusals(KV8Cache):
     z, z64 = words(0, 0), torch.zeros(2, dtype=torch.int64, device='cuda')
     x = torch.zeros(2, 5, 2, 64, device='cuda')
     for args in ((x, x, z64), (x, x, z.cpu()), (x, x, z[:1]), (x[:1], x[:1], z), (x, x[:, :4], z), (x, x.bfloat16(), z), (x.half(), x.half(), z),
-                 (x[:, :, :1], x[:, :, :1], z), (x[..., :32], x[..., :32], z), (x.cpu(), x.cpu(), z), (x[0], x[0], z), (x, x, z, z64), (x, x, None)):
+                 (x[:, :, :1], x[:, :, :1], z), (x[..., :32], x[..., :32], z), (x.cpu(), x.cpu(), z), (x[0], x[0], z), (x, x, z, z64)):
         with pytest.raises(ValueError):
             c.store(*args)
     for args, kw in (((z,), dict(T=129)), ((z,), dict(T=-1)), ((z,), dict(dtype=torch.float16)), ((z64,), {}), ((None,), {})):

@@ -42,7 +42,7 @@ def test_null_descriptors(C):
         assert rc == -1
 
 
-@pytest.mark.parametrize('kw,word', [(dict(L=-1), 'L=-1'), (dict(dtype=2), 'dtype'), (dict(k=None), 'null'), (dict(start=None), 'null'),
+@pytest.mark.parametrize('kw,word', [(dict(L=-1), 'L=-1'), (dict(dtype=2), 'dtype'), (dict(k=None), 'null'), (dict(v=None), 'null'),
                                      (dict(k=260), 'aligned rows'), (dict(v_tok=2), 'aligned rows')])
 def test_bad_stores(C, kw, word):
     d = C.KV8StoreDesc(**{**dict(k=256, v=256, dtype=0, L=1, start=256), **kw})
