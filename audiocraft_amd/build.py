@@ -35,7 +35,7 @@ FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-Wno-pass-faile
 # kernels of these files are written for it (acmi_gemm.hip: TlHot; acmi_attn.hip: attn_decode_kernel).  Firmware without the feature runs the compiler's
 # compatibility prologue, which loads the same registers.
 _PRELOAD = ['-mllvm', '-amdgpu-kernarg-preload-count=14']
-FILE_FLAGS = {'acmi_gemm.hip': _PRELOAD, 'acmi_gemm_f32.hip': _PRELOAD, 'acmi_attn.hip': _PRELOAD}
+FILE_FLAGS = {'acmi_gemm.hip': _PRELOAD, 'acmi_gemm_f32.hip': _PRELOAD, 'acmi_attn.hip': _PRELOAD, 'acmi_kv8.hip': _PRELOAD}
 OBJDIR = os.path.join(CSRC, 'build')
 FILE_DEPS = {'acmi_gemm_f32.hip': ['acmi_gemm.hip']}   # sources a translation unit #includes
 

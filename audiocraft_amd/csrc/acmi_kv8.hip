@@ -509,10 +509,9 @@ __device__ __forceinline__ void kv8_block(Kv8Col<HD, QHL> (&c)[QB], Kv8Ref& vref
 __device__ __forceinline__ int kv8_query(const Kv8AttnArgs& p, int c) { return (int)(((float)c + 0.5f) * p.rG); }
 
 struct Kv8RowInfo { int len, qlen, start; bool fresh; };   // fresh: the call brings the row's newest token (and it fits)
-__device__ __forceinline__ Kv8RowInfo kv8_row(const Kv8AttnArgs& p, int row) {
+__device__ __forceinline__ Kv8RowInfo kv8_row_of(const Kv8AttnArgs& p, int row, int len0) {
     Kv8RowInfo r;
     // (every load at once, then into scalar registers: what follows from them is the same for the whole wave)
-    const int len0 = p.len[(size_t)row * p.len_stride];
     const int ql = p.q_len != nullptr ? p.q_len[row] : p.S;
     const int st = p.start_rows != nullptr ? p.start_rows[row] : 0;
     const long long len = (long long)__builtin_amdgcn_readfirstlane(len0) + p.len_bias;
@@ -522,30 +521,39 @@ __device__ __forceinline__ Kv8RowInfo kv8_row(const Kv8AttnArgs& p, int row) {
     r.start = max(0, __builtin_amdgcn_readfirstlane(st));
     return r;
 }
+__device__ __forceinline__ Kv8RowInfo kv8_row(const Kv8AttnArgs& p, int row) { return kv8_row_of(p, row, p.len[(size_t)row * p.len_stride]); }
 
-// the query features of a lane: x[k][j] = feature kv8_qdim(kg, k) + j of column cidx (past the last column: the last query)
+// 8 NK query features of a lane at q + at: x[k][j] = feature kv8_qdim(kg, k) + j
 template <int HD>
-__device__ __forceinline__ void kv8_load_q(const Kv8AttnArgs& p, int row, int kvh, int cidx, int kg, float (&x)[Kv8Geo<HD>::NK][8]) {
-    const int s0 = kv8_query(p, cidx), g = cidx - s0 * p.G, s = min(s0, p.S - 1);
-    const size_t qb = (size_t)(row * p.q_row + (long long)s * p.q_tok + (long long)(kvh * p.G + g) * p.q_head);
+__device__ __forceinline__ void kv8_load_q(const void* q, size_t qb, int bf16, int kg, float (&x)[Kv8Geo<HD>::NK][8]) {
+    u32x4 w[Kv8Geo<HD>::NK][2];
+    if (bf16) {   // (requests only: a conversion here would wait for them)
 #pragma unroll
-    for (int k = 0; k < Kv8Geo<HD>::NK; ++k) {
-        const size_t at = qb + (HD == 16 ? (kg & 1) * 8 : kv8_qdim<HD>(kg, k));
-        if (p.q_bf16) {
-            const u32x4 w = *reinterpret_cast<const u32x4*>(reinterpret_cast<const bf16_t*>(p.q) + at);
+        for (int k = 0; k < Kv8Geo<HD>::NK; ++k)
+            w[k][0] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const bf16_t*>(q) + qb + (HD == 16 ? (kg & 1) * 8 : kv8_qdim<HD>(kg, k)));
+    } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) { x[k][2 * e] = __uint_as_float(w[e] << 16); x[k][2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u); }
-        } else {
-            const f32x4* q = reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(p.q) + at);
-            const f32x4 a = q[0], b = q[1];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) { x[k][e] = a[e]; x[k][4 + e] = b[e]; }
+        for (int k = 0; k < Kv8Geo<HD>::NK; ++k) {
+            const u32x4* s = reinterpret_cast<const u32x4*>(reinterpret_cast<const float*>(q) + qb + (HD == 16 ? (kg & 1) * 8 : kv8_qdim<HD>(kg, k)));
+            w[k][0] = s[0]; w[k][1] = s[1];
         }
     }
+#pragma unroll
+    for (int k = 0; k < Kv8Geo<HD>::NK; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (bf16) { x[k][2 * e] = __uint_as_float(w[k][0][e] << 16); x[k][2 * e + 1] = __uint_as_float(w[k][0][e] & 0xffff0000u); }
+            else { x[k][e] = __uint_as_float(w[k][0][e]); x[k][4 + e] = __uint_as_float(w[k][1][e]); }
+        }
     if (HD == 16 && kg >= 2) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[0][j] = 0.f;
     }
+}
+// where column cidx's query lies (past the last column: some query)
+__device__ __forceinline__ size_t kv8_query_at(const Kv8AttnArgs& p, int row, int kvh, int cidx) {
+    const int s0 = kv8_query(p, cidx), g = cidx - s0 * p.G, s = min(s0, p.S - 1);
+    return (size_t)(row * p.q_row + (long long)s * p.q_tok + (long long)(kvh * p.G + g) * p.q_head);
 }
 
 // column cidx of (row, cache head): visible range and operands from its features
@@ -646,37 +654,66 @@ template <int HD> constexpr int kv8_wpe() { return HD == 128 ? KV8_B128 : KV8_B6
 __device__ __forceinline__ float raw8(bf16_t v) { return bf16_to_f32(v); }
 __device__ __forceinline__ float raw8(float v) { return v; }
 
+// 16 places of the tail as they are in memory: requested before anything else is known of the row (the places do not depend on
+// its length), made into numbers when they are used.  Keys: lane (kg, nl) the features of its queries' lanes, of place nl;
+// values: feature i * 16 + nl of places kg * 4 + r.
+template <int HD> struct Kv8TailRaw { u32x4 k[Kv8Geo<HD>::NK][2]; uint32_t v[Kv8Geo<HD>::ND][4]; };
+template <int HD>
+__device__ __forceinline__ void kv8_tail_request(const void* kt, const void* vt, size_t base, int bf16, int nl, int kg, Kv8TailRaw<HD>& t) {
+    constexpr int NK = Kv8Geo<HD>::NK, ND = Kv8Geo<HD>::ND;
+    const size_t kb = base + (size_t)nl * HD, vb = base + (size_t)kg * 4 * HD + nl;
+    if (bf16) {
+#pragma unroll
+        for (int k = 0; k < NK; ++k) t.k[k][0] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const bf16_t*>(kt) + kb + (HD == 16 ? (kg & 1) * 8 : kv8_qdim<HD>(kg, k)));
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int i = 0; i < ND; ++i) t.v[i][r] = reinterpret_cast<const bf16_t*>(vt)[vb + r * HD + i * 16];
+    } else {
+#pragma unroll
+        for (int k = 0; k < NK; ++k) {
+            const u32x4* q = reinterpret_cast<const u32x4*>(reinterpret_cast<const float*>(kt) + kb + (HD == 16 ? (kg & 1) * 8 : kv8_qdim<HD>(kg, k)));
+            t.k[k][0] = q[0]; t.k[k][1] = q[1];
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int i = 0; i < ND; ++i) t.v[i][r] = reinterpret_cast<const uint32_t*>(vt)[vb + r * HD + i * 16];
+    }
+}
+
 // The tail's 16 tokens slot0 .. in f32, through the f32 matrix instruction, before any block of codes.
 template <int HD, bool QHL>
-__device__ __forceinline__ void kv8_tail16(const Kv8AttnArgs& p, const Kv8RowInfo& ri, int row, int kvh, int slot0,
+__device__ __forceinline__ void kv8_tail16(const Kv8AttnArgs& p, const Kv8RowInfo& ri, int row, int kvh, int slot0, const Kv8TailRaw<HD>& raw,
                                            const float (&x)[Kv8Geo<HD>::NK][8], Kv8Col<HD, QHL>& c, Kv8Ref& vref) {
     constexpr int NK = Kv8Geo<HD>::NK, ND = Kv8Geo<HD>::ND;
     const int lane = threadIdx.x & 63, nl = lane & 15, kg = lane >> 4;
     const int last = (ri.len - 1) / BLK, t0 = last * BLK + slot0, tb = p.c.tail_dtype == ACMI_BF16;
     const size_t base = ((size_t)row * p.c.H + kvh) * (BLK * HD);
     const size_t kn0 = (size_t)(row * p.kn_row + kvh * p.kn_head), vn0 = (size_t)(row * p.vn_row + kvh * p.vn_head);
-    // keys: lane (kg, nl) the features of its queries' lanes, of token t0 + nl; values: feature i * 16 + nl of tokens t0 + kg * 4 + r.
+    float kx[NK][8], vx[ND][4];
+    const int sh = tb ? 16 : 0;   // bf16 bits are the upper half of the f32
+#pragma unroll
+    for (int k = 0; k < NK; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (tb) { kx[k][2 * e] = __uint_as_float(raw.k[k][0][e] << 16); kx[k][2 * e + 1] = __uint_as_float(raw.k[k][0][e] & 0xffff0000u); }
+            else { kx[k][e] = __uint_as_float(raw.k[k][0][e]); kx[k][4 + e] = __uint_as_float(raw.k[k][1][e]); }
+        }
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int i = 0; i < ND; ++i) vx[i][r] = __uint_as_float(raw.v[i][r] << sh);
     // The row's newest token, which the tail does not hold yet, is put in its place.  (A token past the row's length: whatever the
     // tail holds there only reaches scores that are masked; its values are dropped.)
-    float kx[NK][8], vx[ND][4], kn[NK][8], vn[ND];
-    const bool hasnew = ri.fresh && ri.len - 1 < t0 + 16;   // (wave uniform; the newest token is never before t0)
-    auto from = [&](auto* kt, auto* vt) {
+    if (ri.fresh && ri.len - 1 < t0 + 16) {   // (wave uniform; the newest token is never before t0)
+        float kn[NK][8], vn[ND];
+        auto from_new = [&](auto* k, auto* v) {
 #pragma unroll
-        for (int k = 0; k < NK; ++k) kv8_ld8(kt + (size_t)nl * HD + (HD == 16 ? (kg & 1) * 8 : kv8_qdim<HD>(kg, k)), kx[k]);
+            for (int q = 0; q < NK; ++q) kv8_ld8(k + (HD == 16 ? (kg & 1) * 8 : kv8_qdim<HD>(kg, q)), kn[q]);
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int i = 0; i < ND; ++i) vx[i][r] = raw8(vt[(size_t)(kg * 4 + r) * HD + i * 16 + nl]);
-    };
-    auto from_new = [&](auto* k, auto* v) {
-#pragma unroll
-        for (int q = 0; q < NK; ++q) kv8_ld8(k + (HD == 16 ? (kg & 1) * 8 : kv8_qdim<HD>(kg, q)), kn[q]);
-#pragma unroll
-        for (int i = 0; i < ND; ++i) vn[i] = raw8(v[i * 16 + nl]);
-    };
-    if (tb) from(reinterpret_cast<const bf16_t*>(p.c.k_tail) + base + slot0 * HD, reinterpret_cast<const bf16_t*>(p.c.v_tail) + base + slot0 * HD);
-    else from(reinterpret_cast<const float*>(p.c.k_tail) + base + slot0 * HD, reinterpret_cast<const float*>(p.c.v_tail) + base + slot0 * HD);
-    if (hasnew) {
+            for (int i = 0; i < ND; ++i) vn[i] = raw8(v[i * 16 + nl]);
+        };
         if (p.n_bf16) from_new(reinterpret_cast<const bf16_t*>(p.kn) + kn0, reinterpret_cast<const bf16_t*>(p.vn) + vn0);
         else from_new(reinterpret_cast<const float*>(p.kn) + kn0, reinterpret_cast<const float*>(p.vn) + vn0);
         const int at = ri.len - 1 - t0;
@@ -758,20 +795,35 @@ __device__ __forceinline__ void kv8_tail16(const Kv8AttnArgs& p, const Kv8RowInf
         for (int r = 0; r < 4; ++r) c.o[i][r] *= vref.inv;
 }
 
+// The leading arguments are what the first requests need -- query, length word, tail -- and arrive in scalar registers at wave
+// start (kernarg preload); the rest of the descriptor is fetched behind those requests.
+//   g0 = H | G << 16   g1 = column tiles | q bf16 << 16 | tail bf16 << 17 | length per row << 18   query strides in elements
 template <int HD, bool QHL, bool PHL>
-__global__ __launch_bounds__(kv8_nw<HD>() * 64, kv8_wpe<HD>()) void kv8_attn_split_kernel(const Kv8AttnArgs p) {
+__global__ __launch_bounds__(kv8_nw<HD>() * 64, kv8_wpe<HD>()) void kv8_attn_split_kernel(const void* hq, const int* hlen, const void* hkt, const void* hvt,
+                                                                                          unsigned g0, unsigned g1, int q_row, int q_tok, int q_head, int S,
+                                                                                          const Kv8AttnArgs p) {
     constexpr int NK = Kv8Geo<HD>::NK, ND = Kv8Geo<HD>::ND, KW = Kv8Geo<HD>::KW, PITCH = HD + 4, NW = kv8_nw<HD>();
     __shared__ __attribute__((aligned(16))) float sm_o[NW][16][PITCH];
     __shared__ float sm_m[NW][16], sm_l[NW][16];
     __shared__ Kv8QuantLds<HD> sm_q;
     // (chunk slowest: the workgroups that a shorter row does not need come last, and leave at once)
     const int split = blockIdx.z, row = blockIdx.y;
-    const int qtiles = p.tiles, kvh = blockIdx.x / qtiles, qt = blockIdx.x - kvh * qtiles;
+    const int H = (int)(g0 & 0xffffu), G = (int)(g0 >> 16), qtiles = (int)(g1 & 0xffffu);
+    const int kvh = blockIdx.x / qtiles, qt = blockIdx.x - kvh * qtiles;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int nl = lane & 15, kg = lane >> 4;
+    const int len0 = hlen[(g1 >> 18 & 1) ? row : 0];
     float x[NK][8];
-    kv8_load_q<HD>(p, row, kvh, qt * 16 + nl, kg, x);
-    const Kv8RowInfo ri = kv8_row(p, row);
+    Kv8TailRaw<HD> raw;
+    const int tw = wave - (NW - 4);   // the last four waves take 16 places of the tail each (they have the fewer blocks)
+    {
+        // column -> query and head (a column past the last one reads some query of the call)
+        const int cidx = qt * 16 + nl, sq = (int)(((float)cidx + 0.5f) * __builtin_amdgcn_rcpf((float)G)), g = cidx - sq * G;
+        const size_t qb = (size_t)((long long)row * q_row + (long long)min(sq, S - 1) * q_tok + (long long)(kvh * G + g) * q_head);
+        if (tw >= 0) kv8_tail_request<HD>(hkt, hvt, (((size_t)row * H + kvh) * BLK + tw * 16) * HD, g1 >> 17 & 1, nl, kg, raw);
+        kv8_load_q<HD>(hq, qb, g1 >> 16 & 1, kg, x);
+    }
+    const Kv8RowInfo ri = kv8_row_of(p, row, len0);
     const Kv8Span sp = kv8_span(p, ri, qt * 16, min(qt * 16 + 16, p.S * p.G));
     if (split >= sp.eff) return;
     const int s0 = sp.bf + split * p.chunk, s1 = sp.eff == 1 ? sp.bt : min(sp.bt, s0 + p.chunk);
@@ -805,7 +857,7 @@ __global__ __launch_bounds__(kv8_nw<HD>() * 64, kv8_wpe<HD>()) void kv8_attn_spl
     kv8_column<HD, QHL>(p, ri, qt * 16 + nl, x, c[0]);
     const bool mine = split == sp.eff - 1;   // the split that owns the tail
     Kv8Ref vref = {0.f, 0.f};
-    if (mine && sp.tail && wave < 4 && (ri.len - 1) / BLK * BLK + wave * 16 < ri.len) kv8_tail16<HD, QHL>(p, ri, row, kvh, wave * 16, x, c[0], vref);
+    if (mine && sp.tail && tw >= 0 && (ri.len - 1) / BLK * BLK + tw * 16 < ri.len) kv8_tail16<HD, QHL>(p, ri, row, kvh, tw * 16, raw, x, c[0], vref);
     while (b < s1) {
         // the next requests are not conditional (a wave's last ones read its last block again, from the cache): the waits of a
         // straight line count them exactly, those behind a branch would wait for everything
@@ -987,7 +1039,7 @@ __global__ __launch_bounds__(256, KV8_WPE) void kv8_attn_many_kernel(const Kv8At
     int buf = 0;
     float x[QB][NK][8];
 #pragma unroll
-    for (int g = 0; g < QB; ++g) kv8_load_q<HD>(p, row, kvh, c0 + g * 16 + nl, kg, x[g]);
+    for (int g = 0; g < QB; ++g) kv8_load_q<HD>(p.q, kv8_query_at(p, row, kvh, c0 + g * 16 + nl), p.q_bf16, kg, x[g]);
     if (sp.bf < sp.bt) request(sp.bf);
     Kv8Col<HD, QHL> c[QB];
 #pragma unroll
@@ -1292,7 +1344,11 @@ extern "C" int acmi_kv8_attn(const acmi_kv8_cache* cache, const acmi_kv8_attn_de
         ACMI_REQUIRE((long long)cache->H * qtiles <= 65535, "acmi_kv8_attn: %d heads x %d column tiles", cache->H, qtiles);
         const dim3 grid(cache->H * qtiles, cache->rows, a.splits);
         a.tiles = qtiles;
-#define KV8_SPLIT(HDv, Q, P) hipLaunchKernelGGL((kv8_attn_split_kernel<HDv, Q, P>), grid, dim3(kv8_nw<HDv>() * 64), 0, st, a)
+        ACMI_REQUIRE(d.q_row == (int)d.q_row && (d.S == 1 || d.q_tok == (int)d.q_tok) && d.q_head == (int)d.q_head && a.G <= 65535,
+                     "acmi_kv8_attn: query strides beyond 2^31 elements, or %d query heads per cache head", a.G);
+        const unsigned g0 = (unsigned)cache->H | (unsigned)a.G << 16;
+        const unsigned g1 = (unsigned)qtiles | (unsigned)a.q_bf16 << 16 | (unsigned)(cache->tail_dtype == ACMI_BF16) << 17 | (unsigned)d.len_stride << 18;
+#define KV8_SPLIT(HDv, Q, P) hipLaunchKernelGGL((kv8_attn_split_kernel<HDv, Q, P>), grid, dim3(kv8_nw<HDv>() * 64), 0, st, a.q, a.len, cache->k_tail, cache->v_tail, g0, g1, (int)d.q_row, d.S > 1 ? (int)d.q_tok : 0, (int)d.q_head, d.S, a)
 #define KV8_CASE(HDv)                                            \
     case HDv:                                                    \
         if (out_f32) KV8_SPLIT(HDv, true, true);                 \
