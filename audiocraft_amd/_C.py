@@ -669,9 +669,8 @@ def attn_prefill(q, k_cache, vt, out, npos, npos_pad, pos, past_context=0, out_r
 _raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 
-def launch(device: torch.device, what: str, fn, *args):
-    """fn(*args, stream) on `device` and its current stream, whatever the current device is."""
-    i = device.index
+def launch(i: int, what: str, fn, *args):
+    """fn(*args, stream) on device `i` and its current stream, whatever the current device is."""
     if _current_device() == i:
         rc = fn(*args, _raw_stream(i))
     else:
@@ -686,11 +685,11 @@ def kv8_store(cache: KV8CacheDesc, k, v, start, n):
     ks, vs = k.stride(), v.stride()
     d = KV8StoreDesc(k.data_ptr(), v.data_ptr(), dtype_code(k.dtype), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], k.shape[1],
                      None if start is None else start.data_ptr(), None if n is None else n.data_ptr())
-    launch(k.device, 'acmi_kv8_store', _kv8_store, C.byref(cache), C.byref(d))
+    launch(k.get_device(), 'acmi_kv8_store', _kv8_store, C.byref(cache), C.byref(d))
 
 
 def kv8_load(cache: KV8CacheDesc, lens, T, k_out, v_out):
-    launch(k_out.device, 'acmi_kv8_load', _kv8_load, C.byref(cache), lens.data_ptr(), T, k_out.data_ptr(), v_out.data_ptr(),
+    launch(k_out.get_device(), 'acmi_kv8_load', _kv8_load, C.byref(cache), lens.data_ptr(), T, k_out.data_ptr(), v_out.data_ptr(),
            dtype_code(k_out.dtype))
 
 
@@ -698,22 +697,23 @@ def kv8_attn_work_floats(cache: KV8CacheDesc, S: int, Hq: int) -> int:
     return int(_kv8_attn_work(C.byref(cache), S, Hq))
 
 
-def kv8_attn(cache: KV8CacheDesc, q, q_strides, S, out, lens, len_bias=0, causal=True, past_context=0, q_lens=None, starts=None,
-             k_new=None, v_new=None):
-    """q [rows, (S,) Hq, hd] with strides (row, query, head) -> out [rows, (S,) Hq, hd] dense; k_new / v_new [rows, H, hd]."""
+def kv8_attn(cache: KV8CacheDesc, work_floats: int, q, q_strides, S, out, lens, len_bias=0, causal=True, past_context=0, q_lens=None,
+             starts=None, k_new=None, v_new=None):
+    """q [rows, (S,) Hq, hd] with strides (row, query, head) -> out [rows, (S,) Hq, hd] dense; k_new / v_new [rows, H, hd];
+    work_floats: kv8_attn_work_floats(cache, S, Hq)."""
     Hq = q.shape[-2]
     if k_new is None:
         new = (None, None, 0, 0, 0, 0, 0)
     else:
         kn, vn = k_new.stride(), v_new.stride()
         new = (k_new.data_ptr(), v_new.data_ptr(), dtype_code(k_new.dtype), kn[0], kn[1], vn[0], vn[1])
-    nw = _kv8_attn_work(C.byref(cache), S, Hq)
-    work = torch.empty(nw, device=q.device, dtype=torch.float32) if nw else None
+    work = torch.empty(work_floats, device=q.device, dtype=torch.float32) if work_floats else None
+    code = dtype_code(out.dtype)
     d = KV8AttnDesc(q.data_ptr(), dtype_code(q.dtype), *q_strides, S, Hq, lens.data_ptr(), 1, len_bias,
-                    None if q_lens is None else q_lens.data_ptr(), None if starts is None else starts.data_ptr(), int(causal),
-                    past_context, *new, 0, out.data_ptr(), OUT_BF16 if out.dtype == torch.bfloat16 else OUT_F32,
-                    dtype_code(out.dtype), 0, 0, None if work is None else work.data_ptr())
-    launch(q.device, 'acmi_kv8_attn', _kv8_attn, C.byref(cache), C.byref(d))
+                    None if q_lens is None else q_lens.data_ptr(), None if starts is None else starts.data_ptr(), causal,
+                    past_context, *new, 0, out.data_ptr(), OUT_BF16 if code == BF16 else OUT_F32,
+                    code, 0, 0, None if work is None else work.data_ptr())
+    launch(q.get_device(), 'acmi_kv8_attn', _kv8_attn, C.byref(cache), C.byref(d))
     return out
 
 
@@ -722,7 +722,7 @@ def quantize_rows_i8(x: torch.Tensor):
     R, K = x.shape
     codes = torch.empty(-(-R // 16) * -(-K // 64) * 1024, device=x.device, dtype=torch.int8)
     scale = torch.empty(R, device=x.device, dtype=torch.float32)
-    launch(x.device, 'acmi_quantize_rows_i8', _quantize_rows_i8, x.data_ptr(), dtype_code(x.dtype), x.stride(0) if R > 1 else K, R, K,
+    launch(x.get_device(), 'acmi_quantize_rows_i8', _quantize_rows_i8, x.data_ptr(), dtype_code(x.dtype), x.stride(0) if R > 1 else K, R, K,
            codes.data_ptr(), scale.data_ptr())
     return codes, scale
 
@@ -743,7 +743,7 @@ def linear_i8(x, w, w_scale, out, bias=None, residual=None, act=0, a_scale=None,
         src, act8 = (None, 0, 0, None), (x.data_ptr(), a_scale.data_ptr())
     d = LinearI8Desc(*act8, w.data_ptr(), w_scale.data_ptr(), None if bias is None else bias.data_ptr(),
                      None if residual is None else residual.data_ptr(), out.data_ptr(), dtype_code(out.dtype), N, act, M, N, K, *src)
-    launch(out.device, 'acmi_linear_i8', _linear_i8, C.byref(d))
+    launch(out.get_device(), 'acmi_linear_i8', _linear_i8, C.byref(d))
     return out
 
 

@@ -289,7 +289,10 @@ __global__ __launch_bounds__(BigTile<BIG>::NW * 64, BIG ? 1 : 2) void lin_big_ke
         // accumulators, spills; from LDS a wave takes whole rows of the tile, its column scales and biases loaded once.
         constexpr int HI = WI / 2, PITCH = TC::T + 4, HR = 2 * HI * 16, CW = TC::T / 4;   // (two waves along m)
         float* sm = reinterpret_cast<float*>(smem);
+        float* srow = sm + HR * PITCH;   // the tile's row scales: a request per row in the loop below would be waited for each time
         const int c4 = threadIdx.x % CW, col = (tn << TS) + c4 * 4;
+        float rs = 0.f;
+        if (threadIdx.x < TC::T) rs = p.a_scale[min((tm << TS) + (int)threadIdx.x, p.rows - 1)];
         float sw[4], bi[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -299,6 +302,7 @@ __global__ __launch_bounds__(BigTile<BIG>::NW * 64, BIG ? 1 : 2) void lin_big_ke
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             __syncthreads();
+            if (h == 0 && threadIdx.x < TC::T) srow[threadIdx.x] = rs;
 #pragma unroll
             for (int i = 0; i < HI; ++i)
 #pragma unroll
@@ -308,12 +312,12 @@ __global__ __launch_bounds__(BigTile<BIG>::NW * 64, BIG ? 1 : 2) void lin_big_ke
                         f32x4{(float)v[0], (float)v[1], (float)v[2], (float)v[3]};
                 }
             __syncthreads();
-#pragma unroll 2
+#pragma unroll 4
             for (int rr = threadIdx.x / CW; rr < HR; rr += TC::NW * 64 / CW) {
-                const int row = (tm << TS) + (rr / (HI * 16)) * (WI * 16) + h * HI * 16 + rr % (HI * 16);
+                const int rt = (rr / (HI * 16)) * (WI * 16) + h * HI * 16 + rr % (HI * 16), row = (tm << TS) + rt;
                 if (row >= p.rows || col >= p.N) continue;
                 const f32x4 x = *reinterpret_cast<const f32x4*>(sm + rr * PITCH + c4 * 4);
-                const float sa = p.a_scale[row];
+                const float sa = srow[rt];
                 float v[4];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) v[r] = __builtin_fmaf(x[r], sa * sw[r], bi[r]);
@@ -444,7 +448,7 @@ __global__ __launch_bounds__(BigTile<BIG>::NW * 64, BIG ? 1 : 2) void lin_big_ke
 
 template <typename WT, int E, int BIG>
 static int launch_big_k(const BigArgs& a, int tiles, hipStream_t st) {
-    constexpr size_t ring = 4 * BigTile<BIG>::SLOT * 1024, joint = (size_t)BigTile<BIG>::WI * 16 * (BigTile<BIG>::T + 4) * 4;
+    constexpr size_t ring = 4 * BigTile<BIG>::SLOT * 1024, joint = ((size_t)BigTile<BIG>::WI * 16 * (BigTile<BIG>::T + 4) + BigTile<BIG>::T) * 4;
     constexpr size_t lds = E == ACMI_BIG_I8 && joint > ring ? joint : ring;   // the int8 epilogue's half tile of sums
     static const bool attr_ok = hipFuncSetAttribute(reinterpret_cast<const void*>(&lin_big_kernel<WT, E, BIG>),
                                                     hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) == hipSuccess;   // once, thread safe

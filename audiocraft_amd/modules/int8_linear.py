@@ -34,6 +34,7 @@ class Int8Linear:
         self.activation, self._act = activation, self.ACTIVATIONS[activation]
         w = weight.detach()
         self.codes, self.scale = _C.quantize_rows_i8(w if w.stride(1) == 1 else w.contiguous())
+        self._index = self.codes.get_device()
         self.bias = None
         if bias is not None:
             if bias.shape != (self.out_features,) or bias.device != weight.device:
@@ -46,13 +47,14 @@ class Int8Linear:
 
     def __call__(self, x: torch.Tensor, residual: tp.Optional[torch.Tensor] = None) -> torch.Tensor:
         """x [..., K] f32 or bf16 -> [..., N] in x's dtype; residual [..., N] f32 is added last."""
-        if x.shape[-1:] != (self.in_features,) or x.dtype not in _DTYPES or x.device != self.codes.device:
+        dt = x.dtype
+        if x.dim() == 0 or x.shape[-1] != self.in_features or (dt is not torch.float32 and dt is not torch.bfloat16) or x.get_device() != self._index:
             raise ValueError(f"Int8Linear: x {tuple(x.shape)} {x.dtype} on {x.device}: [..., {self.in_features}] float32 or bfloat16 on {self.codes.device}")
         rows = x if x.dim() == 2 else x.reshape(-1, self.in_features)
         M = rows.shape[0]
         if rows.stride(1) != 1 or (M > 1 and rows.stride(0) < self.in_features):
             rows = rows.contiguous()
-        out = torch.empty(M, self.out_features, device=x.device, dtype=x.dtype)
+        out = torch.empty(M, self.out_features, device=x.device, dtype=dt)
         if residual is not None:
             if residual.shape != x.shape[:-1] + (self.out_features,) or residual.dtype != torch.float32 or residual.device != x.device:
                 raise ValueError(f"Int8Linear: residual {tuple(residual.shape)} {residual.dtype}, expected float32 {tuple(x.shape[:-1]) + (self.out_features,)}")

@@ -53,6 +53,7 @@ class KV8Cache:
         self.k_tail = torch.zeros(rows, heads, blk, head_dim, device=device, dtype=dtype)
         self.v_tail = torch.zeros(rows, heads, blk, head_dim, device=device, dtype=dtype)
         self.device = self.k_codes.device
+        self._index, self._row_shape, self._work_floats = self.k_codes.get_device(), torch.Size((rows,)), {}
         self.desc = _C.KV8CacheDesc(self.k_codes.data_ptr(), self.v_codes.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(),
                                     self.k_tail.data_ptr(), self.v_tail.data_ptr(), _C.dtype_code(dtype), rows, heads, head_dim, nb)
 
@@ -63,20 +64,27 @@ class KV8Cache:
     def _data(self, who: str, name: str, t: torch.Tensor, shape) -> torch.Tensor:
         if not isinstance(t, torch.Tensor) or t.shape != shape:
             raise ValueError(f"KV8Cache.{who}: {name} {tuple(getattr(t, 'shape', ()))}, expected {tuple(shape)}")
-        if t.dtype not in _DTYPES or t.device != self.device:
-            raise ValueError(f"KV8Cache.{who}: {name} is {t.dtype} on {t.device}, expected float32 or bfloat16 on {self.device}")
+        dt = t.dtype
+        if (dt is not torch.float32 and dt is not torch.bfloat16) or t.get_device() != self._index:
+            raise ValueError(f"KV8Cache.{who}: {name} is {dt} on {t.device}, expected float32 or bfloat16 on {self.device}")
         # the kernels read 16 bytes at a time: a view whose rows do not start on 16 bytes is copied
-        es, strides = t.element_size(), t.stride()
-        if strides[-1] != 1 or (t.data_ptr() | es * strides[0] | es * strides[1] | es * strides[-2]) & 15:
+        st = t.stride()
+        if st[-1] != 1 or (t.data_ptr() | (st[0] | st[1] | st[-2]) * (4 if dt is torch.float32 else 2)) & 15:
             t = t.clone(memory_format=torch.contiguous_format)
         return t
 
     def _words(self, who: str, name: str, t: tp.Optional[torch.Tensor], need: bool) -> tp.Optional[torch.Tensor]:
         if t is None and not need:
             return None
-        if not isinstance(t, torch.Tensor) or t.shape != (self.rows,) or t.dtype != torch.int32 or t.device != self.device:
+        if not isinstance(t, torch.Tensor) or t.shape != self._row_shape or t.dtype is not torch.int32 or t.get_device() != self._index:
             raise ValueError(f"KV8Cache.{who}: {name} must be int32 [{self.rows}] on {self.device}")
         return t if t.is_contiguous() else t.contiguous()
+
+    def _work(self, S: int, Hq: int) -> int:
+        n = self._work_floats.get((S, Hq))
+        if n is None:
+            n = self._work_floats[S, Hq] = _C.kv8_attn_work_floats(self.desc, S, Hq)
+        return n
 
     # ------------------------------------------------------------------------------------- operators
     def store(self, k: torch.Tensor, v: torch.Tensor, start: tp.Optional[torch.Tensor] = None, n: tp.Optional[torch.Tensor] = None) -> None:
@@ -118,7 +126,7 @@ class KV8Cache:
         lens, starts = self._words('decode', 'lens', lens, True), self._words('decode', 'starts', starts, False)
         out = torch.empty(self.rows, Hq, self.head_dim, device=self.device, dtype=q.dtype)
         qs = q.stride()
-        _C.kv8_attn(self.desc, q, (qs[0], 0, qs[1]), 1, out, lens, 1, True, self._past('decode', past_context), None, starts, k, v)
+        _C.kv8_attn(self.desc, self._work(1, Hq), q, (qs[0], 0, qs[1]), 1, out, lens, 1, True, self._past('decode', past_context), None, starts, k, v)
         return out
 
     def attend(self, q: torch.Tensor, lens: torch.Tensor, causal: bool = True, past_context: int = 0,
@@ -138,7 +146,7 @@ class KV8Cache:
         q_lens = self._words('attend', 'q_lens', q_lens, False)
         out = torch.empty(self.rows, S, Hq, self.head_dim, device=self.device, dtype=q.dtype)
         if S:
-            _C.kv8_attn(self.desc, q, q.stride()[:3], S, out, lens, 0, bool(causal), past, q_lens, starts)
+            _C.kv8_attn(self.desc, self._work(S, Hq), q, q.stride()[:3], S, out, lens, 0, bool(causal), past, q_lens, starts)
         return out
 
     def _q_heads(self, who: str, q: torch.Tensor, dims: int) -> int:
