@@ -281,8 +281,8 @@ __global__ __launch_bounds__(256) void kv8_load_kernel(const Kv8LoadArgs p) {
 // the codes are stored in).  Codes become f16 exactly: byte u = code + 128 under 0x64 is the f16 number 1024 + u, minus 1152.
 // Queries are f16 relative to a power of two near the row's largest feature; an f32 query is a pair of f16 (22 bits).
 // Per score the vector ALU does a maximum, one multiply-add (scale, running maximum), one exp2 and half a conversion: the value
-// block's scale, relative to the largest one met (vref), sits in the exponent too, and the row sums come out of the matrix
-// cores (a product with ones), from the very f16 numbers that multiply the values.
+// block's scale sits in the exponent too, relative to the largest p * scale met, and the row sums come out of the matrix cores (a
+// product with ones), from the very f16 numbers that multiply the values.
 struct Kv8AttnArgs {
     acmi_kv8_cache c;
     const void* q; int q_bf16; long long q_row, q_tok, q_head;
@@ -356,15 +356,14 @@ template <int HD, bool QHL> struct Kv8Col {
     float sfac;          // score factor: softmax scale * log2(e) * the query's power of two
     int lo, lim;         // positions [lo, lim) are seen
     float m, l;          // running maximum (log2 units, lagging); sum of 2^8 p
-    f32x4 o[Kv8Geo<HD>::ND];   // sum of 2^8 p v, in units of the wave's vref
+    float w;             // log2 of o's unit: like m, but for p times the block's value scale, and counted from m
+    f32x4 o[Kv8Geo<HD>::ND];   // sum of 2^8 p v / 2^w
 };
-
-struct Kv8Ref { float v, inv; };   // largest value scale met, its reciprocal
 
 // A block of 64 tokens into QB column tiles.  K(tt, k) / V(i, u): the fragments (LO: KL / VL their f16 remainders, for a tail in
 // f32); ks, vs: the block's scales; t0 its first position; after_k(): called once the K fragments have been used.
 template <int HD, bool QHL, bool PHL, bool LO, int QB, typename FK, typename FV, typename FKL, typename FVL, typename FA, typename FS>
-__device__ __forceinline__ void kv8_block(Kv8Col<HD, QHL> (&c)[QB], Kv8Ref& vref, const FK& K, const FV& V, const FKL& KL, const FVL& VL,
+__device__ __forceinline__ void kv8_block(Kv8Col<HD, QHL> (&c)[QB], const FK& K, const FV& V, const FKL& KL, const FVL& VL,
                                           float ks, float vs, int t0, const FA& after_k, const FS& fix_scores) {
     constexpr int NK = Kv8Geo<HD>::NK, ND = Kv8Geo<HD>::ND;
     const int kg = (threadIdx.x & 63) >> 4;
@@ -399,20 +398,11 @@ __device__ __forceinline__ void kv8_block(Kv8Col<HD, QHL> (&c)[QB], Kv8Ref& vref
         }
     after_k();
     fix_scores(s);
-    // the block's value scale relative to the largest one met; a scale of 0 belongs to codes that are all 0
     const bool vnan = !(vs == vs);
-    float rescale = 1.f;
+    const float lv = vs > 0.f ? __builtin_amdgcn_logf(vs) : -300.f;   // log2; codes that are all 0 (or poisoned: below) count for nothing
     bool moved = false;
-    if (vs > vref.v) {
-        rescale = vref.v > 0.f ? vref.v / vs : 0.f;
-        vref.v = vs;
-        vref.inv = 1.f / vs;
-        moved = true;
-    }
-    const float lr = (vs > 0.f && vs < vref.v) ? __builtin_amdgcn_logf(vs * vref.inv) : 0.f;   // log2
-    const float ie = __builtin_amdgcn_exp2f(-lr);
     f16x8 ph[QB][2], pl[QB][PHL ? 2 : 1];
-    float alpha[QB];
+    float shrink[QB];
 #pragma unroll
     for (int g = 0; g < QB; ++g) {
         const int hi = c[g].lim - t0 - kg * 4, lo = c[g].lo - t0 - kg * 4;   // token tt * 16 + r of this lane is seen when lo <= it < hi
@@ -436,14 +426,25 @@ __device__ __forceinline__ void kv8_block(Kv8Col<HD, QHL> (&c)[QB], Kv8Ref& vref
         // a column that sees nothing here keeps clear of the block's scales (which a NaN may have poisoned); a key scale of 0
         // belongs to scores that are all 0
         float f = ks * c[g].sfac;
-        f = (none || f == 0.f) ? 1.f : f;
+        if (f == 0.f) f = ks == 0.f ? 1.f : 1.17549435e-38f;   // (a product too small for f32: scores that are 0 beside a masked -infinity)
+        f = none ? 1.f : f;
         const float top = cmax * f;
         const float m_new = top > c[g].m + KV8_LAG ? top : c[g].m;
         const float m_use = m_new == -INFINITY ? 0.f : m_new;
-        alpha[g] = __builtin_amdgcn_exp2f(c[g].m - m_use);
+        const float alpha = __builtin_amdgcn_exp2f(c[g].m - m_use);
+        // the numbers that multiply the values: p 2^d, d = the block's value scale against what o is counted in, so that neither
+        // large values with small p nor small ones with large p leave f16's range
+        const float w_old = top > c[g].m + KV8_LAG ? c[g].w - (m_new - c[g].m) : c[g].w, here = top - m_use + lv;
+        const float w_new = here > w_old + KV8_LAG ? here : w_old;
+        const float w_use = w_new == -INFINITY ? lv : w_new;
+        shrink[g] = __builtin_amdgcn_exp2f(w_old - w_use);
+        moved |= w_new > w_old;
         c[g].m = m_new;
-        moved |= alpha[g] != 1.f;
-        float base = lr + KV8_PSHIFT - m_use, f2 = f;
+        c[g].w = w_new;
+        const float d = fmaxf(lv - w_use, -100.f);   // (so far below: nothing in o, but still itself in the sum l)
+        const float ie = d > 100.f ? 0.f : __builtin_amdgcn_exp2f(-d);
+        const bool plain = fabsf(d) <= 4.f;   // else f16 would not hold p 2^d as exactly as p: the sum is taken in f32 then
+        float base = d + KV8_PSHIFT - m_use, f2 = f;
         if (__any(fabsf(m_use) > 1024.f)) {
             // large scores: the multiply-add below subtracts the ROUNDED maximum from the exact product (and the shift drowns in it);
             // scaled and shifted apart, the largest score gives exactly 0
@@ -452,7 +453,7 @@ __device__ __forceinline__ void kv8_block(Kv8Col<HD, QHL> (&c)[QB], Kv8Ref& vref
 #pragma unroll
                 for (int r = 0; r < 4; ++r) s[g][tt][r] = s[g][tt][r] * f - m_use;
             f2 = 1.f;
-            base = lr + KV8_PSHIFT;
+            base = d + KV8_PSHIFT;
         }
 #pragma unroll
         for (int tt = 0; tt < 4; ++tt)
@@ -471,11 +472,21 @@ __device__ __forceinline__ void kv8_block(Kv8Col<HD, QHL> (&c)[QB], Kv8Ref& vref
                 }
             }
         // the row sums: every row of (ones) P is the sum over the block's tokens
-        const _Float16 o1 = (_Float16)1.f;
-        const f16x8 ones = {o1, o1, o1, o1, o1, o1, o1, o1};
-        f32x4 sum = kv8_mma(ones, ph[g][1], kv8_mma(ones, ph[g][0], zero));
-        if constexpr (PHL) sum = kv8_mma(ones, pl[g][1], kv8_mma(ones, pl[g][0], sum));
-        c[g].l = fmaf(c[g].l, alpha[g], sum[0] * ie);
+        float sum;
+        if (__all(plain)) {
+            const _Float16 o1 = (_Float16)1.f;
+            const f16x8 ones = {o1, o1, o1, o1, o1, o1, o1, o1};
+            f32x4 t = kv8_mma(ones, ph[g][1], kv8_mma(ones, ph[g][0], zero));
+            if constexpr (PHL) t = kv8_mma(ones, pl[g][1], kv8_mma(ones, pl[g][0], t));
+            sum = t[0];
+        } else {
+            sum = 0.f;
+#pragma unroll
+            for (int tt = 0; tt < 4; ++tt) sum += (s[g][tt][0] + s[g][tt][1]) + (s[g][tt][2] + s[g][tt][3]);
+            sum += __shfl_xor(sum, 16, 64);
+            sum += __shfl_xor(sum, 32, 64);
+        }
+        c[g].l = fmaf(c[g].l, alpha, sum * ie);
         if (vnan && !none) c[g].l = __uint_as_float(0x7fc00000u);
     }
     if (__any(moved)) {
@@ -484,7 +495,7 @@ __device__ __forceinline__ void kv8_block(Kv8Col<HD, QHL> (&c)[QB], Kv8Ref& vref
 #pragma unroll
             for (int i = 0; i < ND; ++i)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) c[g].o[i][r] *= alpha[g] * rescale;
+                for (int r = 0; r < 4; ++r) c[g].o[i][r] *= shrink[g];
     }
 #pragma unroll
     for (int i = 0; i < ND; ++i)
@@ -567,7 +578,7 @@ __device__ __forceinline__ void kv8_column(const Kv8AttnArgs& p, const Kv8RowInf
     c.lo = live ? ri.start : 0;
     if (live && p.causal && p.past > 0) c.lo = max(c.lo, pos - p.past);
     if (c.lo >= c.lim) { c.lo = 0; c.lim = 0; }
-    c.m = -INFINITY; c.l = 0.f;
+    c.m = c.w = -INFINITY; c.l = 0.f;
 #pragma unroll
     for (int i = 0; i < Kv8Geo<HD>::ND; ++i) c.o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
     float amax = 0.f, bad = 0.f;   // bad: NaN as soon as a feature is not finite (which a maximum would not tell)
@@ -685,7 +696,7 @@ __device__ __forceinline__ void kv8_tail_request(const void* kt, const void* vt,
 // The tail's 16 tokens slot0 .. in f32, through the f32 matrix instruction, before any block of codes.
 template <int HD, bool QHL>
 __device__ __forceinline__ void kv8_tail16(const Kv8AttnArgs& p, const Kv8RowInfo& ri, int row, int kvh, int slot0, const Kv8TailRaw<HD>& raw,
-                                           const float (&x)[Kv8Geo<HD>::NK][8], Kv8Col<HD, QHL>& c, Kv8Ref& vref) {
+                                           const float (&x)[Kv8Geo<HD>::NK][8], Kv8Col<HD, QHL>& c) {
     constexpr int NK = Kv8Geo<HD>::NK, ND = Kv8Geo<HD>::ND;
     const int lane = threadIdx.x & 63, nl = lane & 15, kg = lane >> 4;
     const int last = (ri.len - 1) / BLK, t0 = last * BLK + slot0, tb = p.c.tail_dtype == ACMI_BF16;
@@ -787,12 +798,12 @@ __device__ __forceinline__ void kv8_tail16(const Kv8AttnArgs& p, const Kv8RowInf
         }
     }
     // in units of a scale like the blocks': largest value / 127
-    vref.v = fmaxf(wave_max(vmax) * (1.f / 127.f), 7.52316384526264e-37f);
-    vref.inv = 1.f / vref.v;
+    const float unit = fmaxf(wave_max(vmax) * (1.f / 127.f), 7.52316384526264e-37f), iu = 1.f / unit;
+    c.w = c.m == -INFINITY ? -INFINITY : __builtin_amdgcn_logf(unit);
 #pragma unroll
     for (int i = 0; i < ND; ++i)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) c.o[i][r] *= vref.inv;
+        for (int r = 0; r < 4; ++r) c.o[i][r] *= iu;
 }
 
 // The leading arguments are what the first requests need -- query, length word, tail -- and arrive in scalar registers at wave
@@ -856,20 +867,20 @@ __global__ __launch_bounds__(kv8_nw<HD>() * 64, kv8_wpe<HD>()) void kv8_attn_spl
     Kv8Col<HD, QHL> c[1];
     kv8_column<HD, QHL>(p, ri, qt * 16 + nl, x, c[0]);
     const bool mine = split == sp.eff - 1;   // the split that owns the tail
-    Kv8Ref vref = {0.f, 0.f};
-    if (mine && sp.tail && tw >= 0 && (ri.len - 1) / BLK * BLK + tw * 16 < ri.len) kv8_tail16<HD, QHL>(p, ri, row, kvh, tw * 16, raw, x, c[0], vref);
+    if (mine && sp.tail && tw >= 0 && (ri.len - 1) / BLK * BLK + tw * 16 < ri.len) kv8_tail16<HD, QHL>(p, ri, row, kvh, tw * 16, raw, x, c[0]);
     while (b < s1) {
         // the next requests are not conditional (a wave's last ones read its last block again, from the cache): the waits of a
         // straight line count them exactly, those behind a branch would wait for everything
         const int nb = b + NW, rq = min(nb, s1 - 1);
         const float kcur = ksn, vcur = vsn;
-        kv8_block<HD, QHL, PHL, false, 1>(c, vref, [&](int tt, int k) { return kv8_cvt(kr[tt][2 * k], kr[tt][2 * k + 1]); },
+        kv8_block<HD, QHL, PHL, false, 1>(c, [&](int tt, int k) { return kv8_cvt(kr[tt][2 * k], kr[tt][2 * k + 1]); },
                                           [&](int i, int u) { return kv8_cvt(vr[i][2 * u], vr[i][2 * u + 1]); }, 0, 0, kcur, vcur, b * BLK,
                                           [&] { get_k(rq); }, [](auto&) {});
         get_v(rq);
         b = nb;
     }
-    const float unit = vref.v * (1.f / 256.f);
+    // relative to the wave's maximum (a column that has seen nothing has o = 0)
+    const float unit = __builtin_amdgcn_exp2f(c[0].w) * (1.f / 256.f);
 #pragma unroll
     for (int i = 0; i < ND; ++i) {
         f32x4 o = c[0].o[i];
@@ -1007,7 +1018,6 @@ __global__ __launch_bounds__(256, KV8_WPE) void kv8_attn_many_kernel(const Kv8At
     const Kv8Span sp = kv8_span(p, ri, w0, min(w0 + 64 * QB, cols));
     Kv8Span me = kv8_span(p, ri, min(c0, cols - 1), min(c0 + 16 * QB, cols));
     if (c0 >= cols) { me.live = me.tail = false; me.bf = me.bt = 0; }
-    Kv8Ref vref = {0.f, 0.f};
     const size_t rh = (size_t)row * p.c.H + kvh, hb = rh * p.c.nblk;
     const uint8_t* kc = reinterpret_cast<const uint8_t*>(p.c.k_codes) + hb * (size_t)(BLK * HD);
     const uint8_t* vc = reinterpret_cast<const uint8_t*>(p.c.v_codes) + hb * (size_t)(BLK * HD);
@@ -1053,7 +1063,7 @@ __global__ __launch_bounds__(256, KV8_WPE) void kv8_attn_many_kernel(const Kv8At
             if (more) request(b + 1);
             __builtin_amdgcn_sched_barrier(0);
             if (b >= me.bf && b < me.bt)
-                kv8_block<HD, QHL, PHL, false, QB>(c, vref, [&](int tt, int k) { return sm.k[buf][tt * NK + k][lane]; },
+                kv8_block<HD, QHL, PHL, false, QB>(c, [&](int tt, int k) { return sm.k[buf][tt * NK + k][lane]; },
                                                    [&](int i, int u) { return sm.v[buf][i * 2 + u][lane]; }, 0, 0,
                                                    ks, vs, b * BLK, none, keep);
             if (more) stage(buf ^ 1);
@@ -1175,8 +1185,8 @@ __global__ __launch_bounds__(256, KV8_WPE) void kv8_attn_many_kernel(const Kv8At
             auto V = [&](int i, int u) { return sm.v[0][i * 2 + u][lane]; };
             auto KL = [&](int tt, int k) { return sm.k[1][tt * NK + k][lane]; };
             auto VL = [&](int i, int u) { return sm.v[1][i * 2 + u][lane]; };
-            if (tb) kv8_block<HD, QHL, PHL, false, QB>(c, vref, K, V, 0, 0, ks, vs, t0, none, fix);
-            else kv8_block<HD, QHL, PHL, true, QB>(c, vref, K, V, KL, VL, ks, vs, t0, none, fix);
+            if (tb) kv8_block<HD, QHL, PHL, false, QB>(c, K, V, 0, 0, ks, vs, t0, none, fix);
+            else kv8_block<HD, QHL, PHL, true, QB>(c, K, V, KL, VL, ks, vs, t0, none, fix);
 #pragma unroll 1
             for (int t = 0; t < (vbad != 0 ? nt : 0); ++t) {   // values that are not finite one by one, each column for itself
                 if (!(vbad >> t & 1)) continue;
@@ -1200,12 +1210,12 @@ __global__ __launch_bounds__(256, KV8_WPE) void kv8_attn_many_kernel(const Kv8At
         const int cidx = c0 + g * 16 + nl, s = kv8_query(p, cidx), h = cidx - s * p.G;
         if (cidx >= cols) continue;
         const bool zero = s >= ri.qlen || c[g].l == 0.f;
-        const float inv = vref.v / c[g].l;
+        const float inv = 1.f / c[g].l, unit = __builtin_amdgcn_exp2f(c[g].w);
 #pragma unroll
         for (int i = 0; i < ND; ++i) {
             f32x4 o;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) o[r] = zero ? 0.f : c[g].o[i][r] * inv;
+            for (int r = 0; r < 4; ++r) o[r] = zero ? 0.f : c[g].o[i][r] * inv * unit;
             kv8_put4(p, row, s, kvh * p.G + h, HD, i * 16 + kg * 4, o);
         }
     }

@@ -340,6 +340,54 @@ def test_large_scores_and_flat_ones(KV8Cache):
     check(got[0, 1], ref[1], torch.float32, v.abs().max().item())
 
 
+@pytest.mark.parametrize('S', [1, 100])
+@pytest.mark.parametrize('order', ['falling', 'rising', 'mixed'])
+def test_blocks_of_very_different_size(KV8Cache, S, order):
+    """Values from 1e-25 to 1e10 from block to block, keys from 1e-30 to 1: the queries look at the small ones.
+
+    The size of a result is sum p |v|, far below the largest value held: 2^-15 of that, and what f16 drops of p (n * 2^-33 of the
+    largest value a query gives weight to: the large blocks have p < 2^-40 by their keys)."""
+    n, hd = 64 * 8 + 10, 64
+    k, v = make(1, n, 1, hd, torch.float32, 15)
+    size = [1e10, 1e-25, 1.0, 1e-12, 1e-3, 1e5, 1e-20, 1e-7, 1e-15]
+    if order != 'mixed':
+        size = sorted(size, reverse=order == 'falling')
+    q = torch.randn(1, S, 1, hd, generator=torch.Generator().manual_seed(7))
+    q[..., 0] = 1.0
+    for b, s in enumerate(size):
+        v[:, b * BLK:(b + 1) * BLK] *= s
+        k[:, b * BLK:(b + 1) * BLK] *= (0.05 if s < 1e-6 else 0.5)
+        if s > 1e-6:
+            k[:, b * BLK:(b + 1) * BLK, :, 0] = -400.0       # score -50: p < 1e-20 beside the small blocks
+    if order == 'mixed':
+        k[:, 3 * BLK:4 * BLK] *= 1e-30
+    c = KV8Cache(1, 1, hd, n, dtype=torch.float32)
+    c.store(k.cuda(), v.cuda())
+    got = c.attend(q.cuda(), words(n), causal=False).cpu().double()
+    kh, vh = held(k[0]), held(v[0])
+    for i in range(S):
+        p = torch.softmax(kh[:, 0] @ q[0, i, 0].double() / math.sqrt(hd), 0)
+        err = (got[0, i, 0] - p @ vh[:, 0]).abs()
+        bound = 2.0 ** -15 * (p @ vh[:, 0].abs()) + n * 2.0 ** -33 * vh[:, 0].abs().amax(0) * 1e-17
+        assert (err <= bound).all(), (i, (err / bound).max().item())
+
+
+@pytest.mark.parametrize('S', [1, 60])
+@pytest.mark.parametrize('scale', [1e-30, 1e30])
+def test_tiny_and_huge_products(KV8Cache, S, scale):
+    """Keys and queries of 1e-30 each: every score is 0 in f32, the result the mean; values of 1e30: f32's range holds."""
+    n = 300
+    k, v = make(1, n, 1, 64, torch.float32, 16)
+    k, v = (k * 1e-30, v) if scale < 1 else (k, v * 1e30)
+    q = torch.randn(1, S, 1, 64, generator=torch.Generator().manual_seed(8)) * (1e-30 if scale < 1 else 1)
+    c = KV8Cache(1, 1, 64, n, dtype=torch.float32)
+    c.store(k.cuda(), v.cuda())
+    for starts in (None, words(70)):
+        got = c.attend(q.cuda(), words(n), causal=False, starts=starts)
+        ref = attention(q[0].double(), held(k[0]), held(v[0]), False, S, 0, 0 if starts is None else 70)
+        check(got[0], ref, torch.float32, v.abs().max().item())
+
+
 @pytest.mark.parametrize('S', [1, 40])
 def test_query_strides(KV8Cache, S):
     c, k, v = filled(KV8Cache, [100, 90], 2, 64, torch.bfloat16, 12)
