@@ -33,7 +33,8 @@ class Int8Linear:
         self.out_features, self.in_features = weight.shape
         self.activation, self._act = activation, self.ACTIVATIONS[activation]
         w = weight.detach()
-        self.codes, self.scale = _C.quantize_rows_i8(w if w.stride(1) == 1 else w.contiguous())
+        with _C.device_lock:
+            self.codes, self.scale = _C.quantize_rows_i8(w if w.stride(1) == 1 else w.contiguous())
         self._index = self.codes.get_device()
         self.bias = None
         if bias is not None:
@@ -54,11 +55,12 @@ class Int8Linear:
         M = rows.shape[0]
         if rows.stride(1) != 1 or (M > 1 and rows.stride(0) < self.in_features):
             rows = rows.contiguous()
-        out = torch.empty(M, self.out_features, device=x.device, dtype=dt)
         if residual is not None:
             if residual.shape != x.shape[:-1] + (self.out_features,) or residual.dtype != torch.float32 or residual.device != x.device:
                 raise ValueError(f"Int8Linear: residual {tuple(residual.shape)} {residual.dtype}, expected float32 {tuple(x.shape[:-1]) + (self.out_features,)}")
             residual = residual.contiguous()
-        if M:
-            _C.linear_i8(rows, self.codes, self.scale, out, self.bias, residual, self._act)
+        with _C.device_lock:
+            out = torch.empty(M, self.out_features, device=x.device, dtype=dt)
+            if M:
+                _C.linear_i8(rows, self.codes, self.scale, out, self.bias, residual, self._act)
         return out if x.dim() == 2 else out.view(x.shape[:-1] + (self.out_features,))

@@ -27,7 +27,8 @@ class KV8Cache:
     order; rows that a call has no tokens for are left as they are.
 
     A call reads and writes the cache on the current stream, as any tensor operation does: calls on one cache from several
-    streams need the caller's events between them; calls on different caches are independent (scratch belongs to a call).
+    streams need the caller's events between them; calls on different caches are independent (scratch belongs to a call).  Every call
+    takes the process-wide `_C.device_lock`, like the models' device entries.
     """
 
     def __init__(self, rows: int, heads: int, head_dim: int, capacity: int, dtype: torch.dtype = torch.bfloat16,
@@ -97,7 +98,8 @@ class KV8Cache:
             raise ValueError(f"KV8Cache.store: k is {k.dtype}, v is {v.dtype}")
         start, n = self._words('store', 'start', start, False), self._words('store', 'n', n, False)
         if L:
-            _C.kv8_store(self.desc, k, v, start, n)
+            with _C.device_lock:
+                _C.kv8_store(self.desc, k, v, start, n)
 
     def load(self, lens: torch.Tensor, T: tp.Optional[int] = None, dtype: torch.dtype = torch.float32) -> tp.Tuple[torch.Tensor, torch.Tensor]:
         """The keys and values the cache holds, [rows, heads, T, head_dim] each (T None: the whole capacity), zeros past lens[r]."""
@@ -105,10 +107,11 @@ class KV8Cache:
         T = self.capacity if T is None else int(T)
         if not 0 <= T <= self.capacity or dtype not in _DTYPES:
             raise ValueError(f"KV8Cache.load: T {T} (0 .. {self.capacity}), dtype {dtype}")
-        k = torch.empty(self.rows, self.heads, T, self.head_dim, device=self.device, dtype=dtype)
-        v = torch.empty_like(k)
-        if T:
-            _C.kv8_load(self.desc, lens, T, k, v)
+        with _C.device_lock:
+            k = torch.empty(self.rows, self.heads, T, self.head_dim, device=self.device, dtype=dtype)
+            v = torch.empty_like(k)
+            if T:
+                _C.kv8_load(self.desc, lens, T, k, v)
         return k, v
 
     def decode(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lens: torch.Tensor, past_context: int = 0,
@@ -124,10 +127,10 @@ class KV8Cache:
         if k.dtype != v.dtype:
             raise ValueError(f"KV8Cache.decode: k is {k.dtype}, v is {v.dtype}")
         lens, starts = self._words('decode', 'lens', lens, True), self._words('decode', 'starts', starts, False)
-        out = torch.empty(self.rows, Hq, self.head_dim, device=self.device, dtype=q.dtype)
-        qs = q.stride()
-        _C.kv8_attn(self.desc, self._work(1, Hq), q, (qs[0], 0, qs[1]), 1, out, lens, 1, True, self._past('decode', past_context), None, starts, k, v)
-        return out
+        past, qs = self._past('decode', past_context), q.stride()
+        with _C.device_lock:
+            out = torch.empty(self.rows, Hq, self.head_dim, device=self.device, dtype=q.dtype)
+            return _C.kv8_attn(self.desc, self._work(1, Hq), q, (qs[0], 0, qs[1]), 1, out, lens, 1, True, past, None, starts, k, v)
 
     def attend(self, q: torch.Tensor, lens: torch.Tensor, causal: bool = True, past_context: int = 0,
                q_lens: tp.Optional[torch.Tensor] = None, starts: tp.Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -144,9 +147,10 @@ class KV8Cache:
             raise ValueError("KV8Cache.attend: past_context needs causal=True")
         lens, starts = self._words('attend', 'lens', lens, True), self._words('attend', 'starts', starts, False)
         q_lens = self._words('attend', 'q_lens', q_lens, False)
-        out = torch.empty(self.rows, S, Hq, self.head_dim, device=self.device, dtype=q.dtype)
-        if S:
-            _C.kv8_attn(self.desc, self._work(S, Hq), q, q.stride()[:3], S, out, lens, 0, bool(causal), past, q_lens, starts)
+        with _C.device_lock:
+            out = torch.empty(self.rows, S, Hq, self.head_dim, device=self.device, dtype=q.dtype)
+            if S:
+                _C.kv8_attn(self.desc, self._work(S, Hq), q, q.stride()[:3], S, out, lens, 0, bool(causal), past, q_lens, starts)
         return out
 
     def _q_heads(self, who: str, q: torch.Tensor, dims: int) -> int:
