@@ -605,9 +605,9 @@ __device__ __forceinline__ void kv8_column(const Kv8AttnArgs& p, const Kv8RowInf
 // the blocks of codes a column tile visits, and how many workgroups share them
 struct Kv8Span { int bf, bt, eff; bool live, tail; };
 constexpr int KV8_MAX_SPLITS = 64;
-#ifndef KV8_TARGET
-#define KV8_TARGET 512
-#endif
+// Workgroups that a split call aims at: two per CU, what its registers let run at once.  4 rows x 8 cache heads of 128 features, up
+// to 32768 tokens: 512 35.5 us (256 34.6, within the noise, but half as many on a call whose rows differ in length), 1024 41.6.
+constexpr int KV8_TARGET = 512;
 __device__ __forceinline__ Kv8Span kv8_span(const Kv8AttnArgs& p, const Kv8RowInfo& ri, int c0, int c1) {   // columns [c0, c1)
     Kv8Span s;
     const int s0 = c0 / p.G, s1 = min((c1 - 1) / p.G, ri.qlen - 1);
@@ -647,20 +647,11 @@ __device__ __forceinline__ void kv8_put4(const Kv8AttnArgs& p, int row, int s, i
 // ---- few queries: one workgroup per (split, column tile of a cache head, row); its 8 waves take the blocks in turn, four of them
 // 16 tokens of the tail each, and are joined through LDS.  A wave keeps one block in flight: the next block's K is requested as
 // soon as this block's K has been multiplied, its V likewise.
-#ifndef KV8_NW64
-#define KV8_NW64 8
-#endif
-#ifndef KV8_NW128
-#define KV8_NW128 4
-#endif
-#ifndef KV8_B64
-#define KV8_B64 4
-#endif
-#ifndef KV8_B128
-#define KV8_B128 2
-#endif
-template <int HD> constexpr int kv8_nw() { return HD == 128 ? KV8_NW128 : KV8_NW64; }
-template <int HD> constexpr int kv8_wpe() { return HD == 128 ? KV8_B128 : KV8_B64; }
+// Waves per workgroup and (launch bound) per SIMD: every wave has a block in flight, so two workgroups of 8 (hd 128: of 4) cover the
+// memory's latency.  16 rows of 500 to 1251 tokens x 24 heads of 64: 8 waves, 4 per SIMD 15.6 us (at 2 per SIMD 17.2); one row's
+// first token 6.7 (4 waves 7.1).  32768 tokens, hd 128: 4 waves, 2 per SIMD 35.5 us; 8 waves 40.2; 1 per SIMD 42.2.
+template <int HD> constexpr int kv8_nw() { return HD == 128 ? 4 : 8; }
+template <int HD> constexpr int kv8_wpe() { return HD == 128 ? 2 : 4; }
 
 __device__ __forceinline__ float raw8(bf16_t v) { return bf16_to_f32(v); }
 __device__ __forceinline__ float raw8(float v) { return v; }
@@ -1000,11 +991,11 @@ template <int HD> struct Kv8ManyLds {
     unsigned long long kbad, vbad;   // tokens of the tail that hold a NaN or an infinity
 };
 
-#ifndef KV8_WPE
-#define KV8_WPE 3
-#endif
+// Waves per SIMD: bf16 results 3 (600 tokens x 16 rows x 24 heads of 64: 55.6 us, at 2 66.3); f32 results, whose probabilities
+// take two f16 registers, 2 (100 queries of 16 heads over a window of 250, 6 rows: 19.5 us, at 3 with spills 21.4).
+template <bool PHL> constexpr int kv8_many_wpe() { return PHL ? 2 : 3; }
 template <int HD, bool QHL, bool PHL, int QB>
-__global__ __launch_bounds__(256, KV8_WPE) void kv8_attn_many_kernel(const Kv8AttnArgs p) {
+__global__ __launch_bounds__(256, kv8_many_wpe<PHL>()) void kv8_attn_many_kernel(const Kv8AttnArgs p) {
     constexpr int NK = Kv8Geo<HD>::NK, ND = Kv8Geo<HD>::ND, KW = Kv8Geo<HD>::KW, VT = ND >= 4 ? ND / 4 : 1;
     __shared__ Kv8ManyLds<HD> sm;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1231,6 +1222,8 @@ static int kv8_check(const acmi_kv8_cache* c, const char* who) {
                  "%s: bad cache shape rows=%d H=%d nblk=%d", who, c->rows, c->H, c->nblk);
     ACMI_REQUIRE(c->tail_dtype == ACMI_F32 || c->tail_dtype == ACMI_BF16, "%s: tail_dtype %d", who, c->tail_dtype);
     ACMI_REQUIRE(c->k_codes && c->v_codes && c->k_scale && c->v_scale && c->k_tail && c->v_tail, "%s: null cache buffer", who);
+    ACMI_REQUIRE(((reinterpret_cast<size_t>(c->k_codes) | reinterpret_cast<size_t>(c->v_codes) | reinterpret_cast<size_t>(c->k_tail) |
+                   reinterpret_cast<size_t>(c->v_tail)) & 15) == 0, "%s: codes and tails must be 16-byte aligned", who);
     return ACMI_OK;
 }
 static bool kv8_dtype_ok(int d) { return d == ACMI_F32 || d == ACMI_BF16; }
@@ -1274,7 +1267,8 @@ extern "C" int acmi_kv8_load(const acmi_kv8_cache* cache, const int* len, int T,
     ACMI_REQUIRE(len != nullptr && T >= 0 && T <= cache->nblk * BLK && kv8_dtype_ok(out_dtype), "acmi_kv8_load: T=%d outside [0, %d] or dtype %d",
                  T, cache->nblk * BLK, out_dtype);
     if (T == 0) return ACMI_OK;
-    ACMI_REQUIRE(k_out && v_out, "acmi_kv8_load: null output");
+    ACMI_REQUIRE(k_out && v_out && ((reinterpret_cast<size_t>(k_out) | reinterpret_cast<size_t>(v_out)) & 15) == 0,
+                 "acmi_kv8_load: outputs must be 16-byte aligned");
     Kv8LoadArgs a = {};
     a.c = *cache; a.len = len; a.T = T; a.k = k_out; a.v = v_out; a.bf16 = out_dtype == ACMI_BF16;
     const dim3 grid((T + BLK - 1) / BLK, cache->H, cache->rows);
@@ -1284,9 +1278,9 @@ extern "C" int acmi_kv8_load(const acmi_kv8_cache* cache, const int* len, int T,
     return acmi_check_launch("kv8_load_kernel");
 }
 
-// column tiles up to which the split form runs
+// column tiles up to which the split form runs; one query per head always does (it alone stores a new token)
 constexpr int KV8_SPLIT_TILES = 4;
-static bool kv8_few(int S, int G) { return (S * G + 15) / 16 <= KV8_SPLIT_TILES; }
+static bool kv8_few(int S, int G) { return S == 1 || ((long long)S * G + 15) / 16 <= KV8_SPLIT_TILES; }
 // Blocks per workgroup: the longest possible row in so many chunks that the call has about KV8_TARGET workgroups; one chunk (and
 // no second launch) when the tiles alone fill the chip.  The rows' lengths are not known here: shorter rows take fewer chunks of
 // the same size, so that all workgroups take equally long.

@@ -34,7 +34,7 @@ class Int8Linear:
         self.activation, self._act = activation, self.ACTIVATIONS[activation]
         w = weight.detach()
         with _C.device_lock:
-            self.codes, self.scale = _C.quantize_rows_i8(w if w.stride(1) == 1 else w.contiguous())
+            self.codes, self.scale = _C.quantize_rows_i8(w if w.stride(1) == 1 and w.stride(0) >= w.shape[1] else w.contiguous())
         self._index = self.codes.get_device()
         self.bias = None
         if bias is not None:

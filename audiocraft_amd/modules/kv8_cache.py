@@ -61,6 +61,9 @@ class KV8Cache:
     def nbytes(self) -> int:
         return sum(t.numel() * t.element_size() for t in (self.k_codes, self.v_codes, self.k_scale, self.v_scale, self.k_tail, self.v_tail))
 
+    def __reduce_ex__(self, protocol):   # (copy, deepcopy and pickle: `desc` would still name this cache's buffers)
+        raise TypeError("KV8Cache: not copied as an object; store() what load() returned into a new one")
+
     # ------------------------------------------------------------------------------------- checks of arguments
     def _data(self, who: str, name: str, t: torch.Tensor, shape) -> torch.Tensor:
         if not isinstance(t, torch.Tensor) or t.shape != shape:
@@ -91,7 +94,7 @@ class KV8Cache:
     def store(self, k: torch.Tensor, v: torch.Tensor, start: tp.Optional[torch.Tensor] = None, n: tp.Optional[torch.Tensor] = None) -> None:
         """Keys and values [rows, L, heads, head_dim] of the tokens start[r] .. start[r] + n[r] - 1 of every row (n None: all L;
         start[r]: how many the row holds already, None: none).  Tokens past n[r] are padding and never read."""
-        L = k.shape[1] if k.dim() == 4 else -1
+        L = k.shape[1] if isinstance(k, torch.Tensor) and k.dim() == 4 else -1
         k = self._data('store', 'k', k, (self.rows, L, self.heads, self.head_dim))
         v = self._data('store', 'v', v, k.shape)
         if k.dtype != v.dtype:

@@ -163,6 +163,13 @@ def test_empty_and_from_linear(Int8Linear):
     check(layer, x, lin.weight.detach().cpu(), lin.bias.detach().cpu(), 'none')
 
 
+def test_repeated_weight_rows(Int8Linear):
+    """A weight whose rows are one row in memory."""
+    w = torch.randn(1, 64).expand(20, 64)
+    layer = Int8Linear(w.cuda()[:1].expand(20, 64))
+    check(layer, torch.randn(5, 64), w, None, 'none')
+
+
 def test_refusals(Int8Linear):
     w = torch.randn(8, 16, device='cuda')
     for bad in (w.cpu(), w[0], w.half(), w[:0], w[:, :0]):

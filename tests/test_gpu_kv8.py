@@ -232,6 +232,33 @@ def test_decode_token_by_token_equals_store(KV8Cache):
         assert torch.equal(getattr(a, name), getattr(b, name))
 
 
+@pytest.mark.parametrize('dt', ['f32', 'bf16'])
+@pytest.mark.parametrize('G,lens', [(65, [127, 3]), (80, [63, 0]), (130, [700, 65])])
+def test_decode_with_many_heads_on_one(KV8Cache, dt, G, lens):
+    """More query heads per cache head than one workgroup's column tile times four: the token is stored all the same."""
+    dt, hd = DT[dt], 64
+    c, k, v = filled(KV8Cache, lens, 1, hd, dt, G, capacity=max(lens) + 1)
+    g = torch.Generator().manual_seed(G)
+    q = torch.randn(2, G, hd, generator=g).to(dt)
+    k1, v1 = torch.randn(2, 1, hd, generator=g).to(dt), torch.randn(2, 1, hd, generator=g).to(dt)
+    got = c.decode(q.cuda(), k1.cuda(), v1.cuda(), words(*lens))
+    after = c.load(words(*[n + 1 for n in lens]), max(lens) + 1)
+    for r, n in enumerate(lens):
+        kr, vr = (torch.cat([x[r, :n], x1[r:r + 1]]).float() for x, x1 in ((k, k1), (v, v1)))
+        check(got[r:r + 1], attention(q[r:r + 1].double(), held(kr), held(vr), True, 1, 0, 0), dt, vr.abs().max().item())
+        for t, x in zip(after, (kr, vr)):
+            ref = held(x).permute(1, 0, 2)
+            assert ((t[r, :, :n + 1].cpu().double() - ref).abs() <= 3 * 2.0 ** -24 * ref.abs()).all()
+
+
+def test_a_cache_is_not_copied_as_an_object(KV8Cache):
+    import copy
+    c = KV8Cache(1, 1, 16, 64)
+    for f in (copy.copy, copy.deepcopy):
+        with pytest.raises(TypeError, match="load"):
+            f(c)
+
+
 def test_decode_on_a_full_row_drops_the_token(KV8Cache):
     c, k, v = filled(KV8Cache, [128, 100], 2, 64, torch.float32, 2, capacity=128)
     before = [t[0].clone() for t in (c.k_codes, c.v_codes, c.k_tail, c.v_tail, c.k_scale)]

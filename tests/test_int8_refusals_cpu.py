@@ -49,6 +49,17 @@ def test_bad_stores(C, kw, word):
     refused(C, C._kv8_store(ctypes.byref(cache(C)), ctypes.byref(d), None), word)
 
 
+@pytest.mark.parametrize('name', ['k_codes', 'v_codes', 'k_tail', 'v_tail'])
+def test_misaligned_buffers(C, name):
+    d = C.KV8StoreDesc(k=256, v=256, dtype=0, L=1, start=256)
+    refused(C, C._kv8_store(ctypes.byref(cache(C, **{name: 264})), ctypes.byref(d), None), 'aligned')
+    refused(C, C._kv8_load(ctypes.byref(cache(C)), 256, 1, 256 + 4 * (name[0] == 'k'), 256 + 4 * (name[0] == 'v'), 0, None), 'aligned')
+
+
+def test_scratch_of_absurd_sizes(C):
+    assert C._kv8_attn_work(ctypes.byref(cache(C, H=1)), 1 << 30, 1 << 16) == 0
+
+
 @pytest.mark.parametrize('T,dt,k', [(257, 0, 256), (-1, 0, 256), (5, 3, 256), (5, 0, None)])
 def test_bad_loads(C, T, dt, k):
     assert C._kv8_load(ctypes.byref(cache(C)), 256, T, k, 256, dt, None) == -1
