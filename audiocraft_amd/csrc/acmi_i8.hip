@@ -56,7 +56,8 @@ struct QuantRowsArgs { RowSrc s; int nkc, kchunk; uint8_t* codes; float* scale; 
 
 // One workgroup per 16 rows, a wave per row: the row is read once (NV x 256 columns of it stay in registers, longer ones are read
 // again from L2), its codes are laid down in LDS, and the 16 rows leave as whole fragments, 1 KB at a time.  (One workgroup per row
-// wrote 16-byte pieces 256 bytes apart: 38 us for 9600 x 1536 f32, now ~15; profiles: bound by the read.)
+// wrote 16-byte pieces 256 bytes apart: 38 us for 9600 x 1536 f32, now 13.2: 74 MB at 5.6 TB/s, part of it out of the last-level
+// cache.)  9600 x 6144 f32, of whose rows two thirds are read twice: 79 us.
 template <int NV>
 __global__ __launch_bounds__(1024) void quant_rows_kernel(const QuantRowsArgs p) {
     extern __shared__ __attribute__((aligned(16))) unsigned char sm[];   // [16][kchunk + 16]
@@ -149,8 +150,10 @@ static RowSrc row_src(const void* x, int dtype, long long ldx, int R, int K) {
 static int launch_quant_rows(const RowSrc& s, uint8_t* codes, float* scale, hipStream_t st) {
     QuantRowsArgs a = {s, (s.K + 63) / 64, 0, codes, scale};
     a.kchunk = min(a.nkc * 64, 8192);
-    // up to two workgroups per CU by rows; above, whole fragments (us: 384 x 1536 f32 3.9 against 4.3, 1000 x 1000 5.4 against 4.6)
-    if (s.R <= 512) {
+    // A workgroup per row until they are many; then 16 rows to one, whose wave keeps 2048 columns of its row -- longer rows are read
+    // again, so those change over later.  us, per row / 16 rows (kernels): 384 x 1536 f32 3.9 / 4.3, 1000 x 1000 5.4 / 4.6; (calls)
+    // 1024 x 6144 9.1 / 12.7, 2048 x 6144 16.9 / 21.2, 4096 x 6144 31.9 / 27.9, 2048 x 2048 9.3 / 6.9, 4096 x 1536 14.2 / 7.2
+    if (s.R <= (s.K > 2048 ? 2048 : 512)) {
         hipLaunchKernelGGL(quant_row_wide_kernel, dim3(s.R), dim3(512), (size_t)a.kchunk, st, a);
         return acmi_check_launch("quant_row_wide_kernel");
     }
@@ -167,6 +170,7 @@ extern "C" int acmi_quantize_rows_i8(const void* x, int dtype, long long ldx, in
     ACMI_REQUIRE(dtype == ACMI_F32 || dtype == ACMI_BF16, "acmi_quantize_rows_i8: dtype %d", dtype);
     ACMI_REQUIRE(R >= 0 && K > 0 && K <= 131072, "acmi_quantize_rows_i8: R=%d K=%d (K in [1, 131072])", R, K);
     if (R == 0) return ACMI_OK;
+    ACMI_REQUIRE(R <= 1 << 30, "acmi_quantize_rows_i8: R=%d (at most 2^30)", R);
     ACMI_REQUIRE(x && codes && scale && ldx >= K, "acmi_quantize_rows_i8: null buffer or ldx=%lld < K=%d", ldx, K);
     ACMI_REQUIRE((reinterpret_cast<size_t>(codes) & 15) == 0, "acmi_quantize_rows_i8: codes must be 16-byte aligned");
     return launch_quant_rows(row_src(x, dtype, ldx, R, K), reinterpret_cast<uint8_t*>(codes), scale, (hipStream_t)stream);
@@ -313,6 +317,7 @@ extern "C" int acmi_linear_i8(const acmi_linear_i8_desc* desc, void* stream) {
     ACMI_REQUIRE(d.out_dtype == ACMI_F32 || d.out_dtype == ACMI_BF16, "acmi_linear_i8: out_dtype %d", d.out_dtype);
     ACMI_REQUIRE(d.act == 0 || d.act == 1, "acmi_linear_i8: act %d", d.act);
     if (d.M == 0) return ACMI_OK;
+    ACMI_REQUIRE(d.M <= 1 << 30 && d.N <= 1 << 30 && (long long)d.M * d.N <= 1LL << 38, "acmi_linear_i8: M=%d N=%d (each at most 2^30, M N at most 2^38)", d.M, d.N);
     ACMI_REQUIRE(d.w && d.w_scale && d.out && d.ldo >= d.N, "acmi_linear_i8: null operand or ldo=%lld < N=%d", d.ldo, d.N);
     ACMI_REQUIRE((d.x != nullptr) != (d.a != nullptr && d.a_scale != nullptr), "acmi_linear_i8: either x or the quantised a, a_scale");
     ACMI_REQUIRE(((reinterpret_cast<size_t>(d.a) | reinterpret_cast<size_t>(d.w) | reinterpret_cast<size_t>(d.work)) & 15) == 0,
@@ -339,9 +344,9 @@ extern "C" int acmi_linear_i8(const acmi_linear_i8_desc* desc, void* stream) {
         if (int rc = launch_quant_rows(a.s, codes, scale, st)) return rc;
         a.a = reinterpret_cast<const u32x4*>(codes); a.a_scale = scale;
     }
-    // the tiled form once its 128 x 128 tiles give 3 of 8 CUs one; below, 64-row groups of the streaming form.  Measured with the
-    // quantiser, us tiled / streamed: 256 x 4608 x 1536 (72 tiles) 17.8 / 15.9, 1000 x 1000 x 1000 (64) 17.2 / 14.9;
-    // 1024 x 1536 x 6144 (96) 44.6 / 59.7, 512 x 4096 x 1024 (128) 16.5 / 19.9, 600 x 6144 x 1536 (240) 19.9 / 41.3
+    // the tiled form once its 128 x 128 tiles give 3 of 8 CUs one; below, 64-row groups of the streaming form.  Measured without
+    // the quantiser, us tiled / streamed: 256 x 4608 x 1536 (72 tiles) 12.3 / 12.0, 1000 x 1000 x 1000 (64) 10.5 / 9.0;
+    // 1024 x 1536 x 6144 (96) 27.2 / 43.8, 512 x 4096 x 1024 (128) 10.5 / 15.9, 600 x 6144 x 1536 (240) 13.2 / 35.3
     if (((d.M + 127) / 128) * ((d.N + 127) / 128) >= 96) {
         BigArgs b = {};
         b.a = a.a; b.w = d.w; b.bias = d.bias; b.M = mt * 16; b.N = d.N; b.K = d.K; b.act = d.act;

@@ -87,14 +87,15 @@ def test_attention_scratch_is_required(C):
 
 
 @pytest.mark.parametrize('kw,word', [(dict(K=0), 'K=0'), (dict(K=131073), 'K=131073'), (dict(dtype=2), 'dtype'), (dict(ldx=7), 'ldx'),
-                                     (dict(codes=264), 'aligned'), (dict(x=None), 'null'), (dict(R=-1), 'R=-1')])
+                                     (dict(codes=264), 'aligned'), (dict(x=None), 'null'), (dict(R=-1), 'R=-1'), (dict(R=2 ** 31 - 1), '2^30')])
 def test_bad_quantisations(C, kw, word):
     a = {**dict(x=256, dtype=0, ldx=8, R=2, K=8, codes=256, scale=256), **kw}
     refused(C, C._quantize_rows_i8(a['x'], a['dtype'], a['ldx'], a['R'], a['K'], a['codes'], a['scale'], None), word)
 
 
 @pytest.mark.parametrize('kw,word', [(dict(K=131073), 'K=131073'), (dict(N=0), 'N=0'), (dict(M=-1), 'M=-1'), (dict(out_dtype=3), 'out_dtype'),
-                                     (dict(act=2), 'act'), (dict(ldo=3), 'ldo'), (dict(a=260), 'aligned'), (dict(w_scale=None), 'null')])
+                                     (dict(act=2), 'act'), (dict(ldo=3), 'ldo'), (dict(a=260), 'aligned'), (dict(w_scale=None), 'null'),
+                                     (dict(M=1 << 30, N=1 << 20), '2^38'), (dict(M=2 ** 31 - 1), '2^30')])
 def test_bad_projections(C, kw, word):
     d = C.LinearI8Desc(**{**dict(a=256, a_scale=256, w=256, w_scale=256, out=256, out_dtype=0, ldo=4, act=0, M=2, N=4, K=64), **kw})
     refused(C, C._linear_i8(ctypes.byref(d), None), word)
