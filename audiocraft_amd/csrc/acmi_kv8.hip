@@ -5,6 +5,7 @@
 #include <math.h>
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float kv8_f32x2 __attribute__((ext_vector_type(2)));
 
@@ -50,6 +51,16 @@ __device__ __forceinline__ void kv8_ld16(const void* p, size_t i, int bf16, floa
             for (int e = 0; e < 4; ++e) x[h * 4 + e] = w[e];
         }
     }
+}
+// 4 consecutive features (aligned as one) -> f32
+__device__ __forceinline__ void kv8_ld4(const bf16_t* p, float (&x)[4]) {
+    const uint2 w = *reinterpret_cast<const uint2*>(p);
+    x[0] = __uint_as_float(w.x << 16); x[1] = __uint_as_float(w.x & 0xffff0000u); x[2] = __uint_as_float(w.y << 16); x[3] = __uint_as_float(w.y & 0xffff0000u);
+}
+__device__ __forceinline__ void kv8_ld4(const float* p, float (&x)[4]) {
+    const f32x4 w = *reinterpret_cast<const f32x4*>(p);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = w[e];
 }
 // 8 consecutive features (16-byte aligned) -> f32
 template <typename T> __device__ __forceinline__ void kv8_ld8(const T* p, float (&x)[8]) { ld8(p, x); }
@@ -646,7 +657,8 @@ __device__ __forceinline__ void kv8_put4(const Kv8AttnArgs& p, int row, int s, i
 
 // ---- few queries: one workgroup per (split, column tile of a cache head, row); its 8 waves take the blocks in turn, four of them
 // 16 tokens of the tail each, and are joined through LDS.  A wave keeps one block in flight: the next block's K is requested as
-// soon as this block's K has been multiplied, its V likewise.
+// soon as this block's K has been multiplied, its V likewise.  Bound by the codes' bytes: 4 rows of 9001 to 32768 tokens x 8 heads of
+// 128, 171 MB in 35.5 us = 4.8 TB/s, the rate of a large copy; 16 rows of 500 to 1251 x 24 heads of 64 43 MB in 15.6 us.
 // Waves per workgroup and (launch bound) per SIMD: every wave has a block in flight, so two workgroups of 8 (hd 128: of 4) cover the
 // memory's latency.  16 rows of 500 to 1251 tokens x 24 heads of 64: 8 waves, 4 per SIMD 15.6 us (at 2 per SIMD 17.2); one row's
 // first token 6.7 (4 waves 7.1).  32768 tokens, hd 128: 4 waves, 2 per SIMD 35.5 us; 8 waves 40.2; 1 per SIMD 42.2.
@@ -982,7 +994,9 @@ __global__ __launch_bounds__(256) void kv8_attn_join_kernel(const Kv8AttnArgs p)
 
 // ---- many queries: a workgroup's 4 waves own QB column tiles each and walk the blocks together.  Every wave converts a quarter of
 // the next block's codes to f16 fragments in LDS while this block is multiplied (two buffers, one barrier per block).  The tail
-// is staged the same way, relative to a power of two, as f16 (bf16 tails: exact) or a pair of f16 (f32 tails).
+// is staged the same way, relative to a power of two, as f16 (bf16 tails: exact down to 2^-30 of the largest) or a pair of f16.
+// Bound by vector issue beside the matrix cores: causal over 4096 tokens, 4 x 16 heads of 64, 571 TFLOP/s (f32 403).  Short calls
+// are latencies one after another: 16 x 32 heads x 251 queries over 0 .. 77 states 21 us, of which the tail's staging is 7.
 // All workgroups of a (row, cache head) run on one XCD (workgroup i on XCD i % 8), whose L2 then holds its codes; the last (causal:
 // longest) tiles of all pairs go first, the short ones fill the end.
 template <int HD> struct Kv8ManyLds {
@@ -991,11 +1005,11 @@ template <int HD> struct Kv8ManyLds {
     unsigned long long kbad, vbad;   // tokens of the tail that hold a NaN or an infinity
 };
 
-// Waves per SIMD: bf16 results 3 (600 tokens x 16 rows x 24 heads of 64: 55.6 us, at 2 66.3); f32 results, whose probabilities
-// take two f16 registers, 2 (100 queries of 16 heads over a window of 250, 6 rows: 19.5 us, at 3 with spills 21.4).
-template <bool PHL> constexpr int kv8_many_wpe() { return PHL ? 2 : 3; }
+// Waves per SIMD: what the registers allow without spilling more than a few (hd 64, two tiles: 3 55.6 us, 2 66.3, for 600 tokens x
+// 16 rows x 24 heads).
+template <int HD, int QB> constexpr int kv8_many_wpe() { return HD == 128 ? 2 : QB == 2 ? 3 : 4; }
 template <int HD, bool QHL, bool PHL, int QB>
-__global__ __launch_bounds__(256, kv8_many_wpe<PHL>()) void kv8_attn_many_kernel(const Kv8AttnArgs p) {
+__global__ __launch_bounds__(256, (kv8_many_wpe<HD, QB>())) void kv8_attn_many_kernel(const Kv8AttnArgs p) {
     constexpr int NK = Kv8Geo<HD>::NK, ND = Kv8Geo<HD>::ND, KW = Kv8Geo<HD>::KW, VT = ND >= 4 ? ND / 4 : 1;
     __shared__ Kv8ManyLds<HD> sm;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1065,19 +1079,21 @@ __global__ __launch_bounds__(256, kv8_many_wpe<PHL>()) void kv8_attn_many_kernel
     if (sp.tail) {   // (workgroup uniform)
         const int tb = p.c.tail_dtype == ACMI_BF16, t0 = (ri.len - 1) / BLK * BLK, nt = ri.len - t0;
         const size_t base = rh * (BLK * HD);
-        float kx[NK][8], vx[VT][16], ka = 0.f, va = 0.f;
+        constexpr int UN = HD > 64 ? HD / 64 : 1;   // 4 tokens x 4 features of V per thread, so many times
+        float kx[NK][8], vx[UN][4][4], ka = 0.f, va = 0.f;
         bool kb = false;
-        unsigned vb = 0;
+        unsigned long long vb = 0;
         if (threadIdx.x == 0) { sm.kbad = 0; sm.vbad = 0; }
         const int tk = wave * 16 + nl;   // this lane's token of K
         auto from = [&](auto* kt, auto* vt) {   // every load of the tail in flight at once (places past the length are masked below)
 #pragma unroll
             for (int k = 0; k < NK; ++k) kv8_ld8(kt + (size_t)tk * HD + (HD == 16 ? (kg & 1) * 8 : kv8_qdim<HD>(kg, k)), kx[k]);
 #pragma unroll
-            for (int q = 0; q < VT; ++q)
+            for (int u = 0; u < UN; ++u) {
+                const int un = min(u * 256 + (int)threadIdx.x, HD * 4 - 1), t4 = un / (HD / 4) * 4, f4 = un % (HD / 4) * 4;
 #pragma unroll
-                for (int j = 0; j < 16; ++j)
-                    vx[q][j] = raw8(vt[(size_t)((j >> 2) * 16 + kg * 4 + (j & 3)) * HD + min(wave + q * 4, ND - 1) * 16 + nl]);
+                for (int r = 0; r < 4; ++r) kv8_ld4(vt + (t4 + r) * HD + f4, vx[u][r]);
+            }
         };
         if (tb) from(reinterpret_cast<const bf16_t*>(p.c.k_tail) + base, reinterpret_cast<const bf16_t*>(p.c.v_tail) + base);
         else from(reinterpret_cast<const float*>(p.c.k_tail) + base, reinterpret_cast<const float*>(p.c.v_tail) + base);
@@ -1092,56 +1108,60 @@ __global__ __launch_bounds__(256, kv8_many_wpe<PHL>()) void kv8_attn_many_kernel
                 ka = fmaxf(ka, fabsf(v));
             }
 #pragma unroll
-        for (int q = 0; q < VT; ++q)
+        for (int u = 0; u < UN; ++u) {
+            const int t4 = min(u * 256 + (int)threadIdx.x, HD * 4 - 1) / (HD / 4) * 4;
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                float v = (j >> 2) * 16 + kg * 4 + (j & 3) < nt ? vx[q][j] : 0.f;
-                const float a = fabsf(v);
-                if (!(a <= 3.4028234663852886e38f)) { vb |= 1u << j; v = 0.f; }
-                vx[q][j] = v;
-                va = fmaxf(va, fabsf(v));
-            }
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float v = t4 + r < nt ? vx[u][r][e] : 0.f;
+                    const float a = fabsf(v);
+                    if (!(a <= 3.4028234663852886e38f)) { vb |= 1ull << (t4 + r); v = 0.f; }
+                    vx[u][r][e] = v;
+                    va = fmaxf(va, fabsf(v));
+                }
+        }
         ka = wave_max(ka);
         va = wave_max(va);
         if (lane == 0) { sm.red[0][wave] = ka; sm.red[1][wave] = va; }
         __syncthreads();
         if (kb) atomicOr(&sm.kbad, 1ull << tk);
-        if (vb != 0) {
-            unsigned long long m = 0;
-            for (int j = 0; j < 16; ++j)
-                if (vb >> j & 1) m |= 1ull << ((j >> 2) * 16 + kg * 4 + (j & 3));
-            atomicOr(&sm.vbad, m);
-        }
+        if (vb != 0) atomicOr(&sm.vbad, vb);
         ka = fmaxf(fmaxf(sm.red[0][0], sm.red[0][1]), fmaxf(sm.red[0][2], sm.red[0][3]));
         va = fmaxf(fmaxf(sm.red[1][0], sm.red[1][1]), fmaxf(sm.red[1][2], sm.red[1][3]));
         const float ku = ldexpf(1.f, min(14 - (ka > 0.f ? ilogbf(ka) : 0), 126)), vu = ldexpf(1.f, min(14 - (va > 0.f ? ilogbf(va) : 0), 126));
 #pragma unroll
         for (int k = 0; k < NK; ++k) {
-            f16x8 h, l;
+            f16x8 h;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float y = kx[k][j] * ku;
-                h[j] = (_Float16)y;
-                l[j] = (_Float16)(y - (float)h[j]);
-            }
+            for (int j = 0; j < 8; ++j) { kx[k][j] *= ku; h[j] = (_Float16)kx[k][j]; }
             sm.k[0][wave * NK + k][lane] = h;
-            if (!tb) sm.k[1][wave * NK + k][lane] = l;
+            if (!tb) {
+                f16x8 l;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) l[j] = (_Float16)(kx[k][j] - (float)h[j]);
+                sm.k[1][wave * NK + k][lane] = l;
+            }
         }
 #pragma unroll
-        for (int q = 0; q < VT; ++q)
-            if (wave + q * 4 < ND)
+        for (int u = 0; u < UN; ++u) {
+            const int un = u * 256 + (int)threadIdx.x, t4 = un / (HD / 4), f = un % (HD / 4) * 4;
+            if (un < HD * 4)
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    f16x8 h, l;
+                for (int e = 0; e < 4; ++e) {   // feature f + e of tokens 4 t4 ..: half a lane's operand
+                    const int at = (f >> 4) * 2 + (t4 >> 3), ln = (t4 & 3) * 16 + (f & 15) + e, half = (t4 >> 2) & 1;
+                    f16x4 h;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const float y = vx[q][u * 8 + j] * vu;
-                        h[j] = (_Float16)y;
-                        l[j] = (_Float16)(y - (float)h[j]);
+                    for (int r = 0; r < 4; ++r) { vx[u][r][e] *= vu; h[r] = (_Float16)vx[u][r][e]; }
+                    reinterpret_cast<f16x4*>(&sm.v[0][at][ln])[half] = h;
+                    if (!tb) {
+                        f16x4 l;
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) l[r] = (_Float16)(vx[u][r][e] - (float)h[r]);
+                        reinterpret_cast<f16x4*>(&sm.v[1][at][ln])[half] = l;
                     }
-                    sm.v[0][(wave + q * 4) * 2 + u][lane] = h;
-                    if (!tb) sm.v[1][(wave + q * 4) * 2 + u][lane] = l;
                 }
+        }
         __syncthreads();
         if (me.tail) {
             // tokens past the row's length are masked for every stored column by its limit; a column without a query may count them
@@ -1370,17 +1390,22 @@ extern "C" int acmi_kv8_attn(const acmi_kv8_cache* cache, const acmi_kv8_attn_de
 #undef KV8_CASE
         return acmi_check_launch("kv8_attn_join_kernel");
     }
-    const int QB = cache->hd <= 64 ? 2 : 1;   // (hd 128: two column tiles do not fit the registers)
+    const long long pairs = ((long long)cache->rows * cache->H + 7) / 8 * 8;
+    // two column tiles per wave where bf16 results at 64 features leave the registers for it and the workgroups still fill the chip,
+    // three per CU.  Measured, us one / two: 4 x 16 heads x 4096 tokens (2048 workgroups of two) 273 / 241, 16 x 24 x 600 (1920)
+    // 58.8 / 56.6, 8 x 8 x 4 x 512 of 2048 (1024) 120 / 114; 16 x 16 x 100 of 1500 (256) 36.9 / 44.4, 4 x 8 x 128 of 300 (32)
+    // 10.8 / 14.8; f32 4 x 16 x 4096 341 / 344; hd 32 8 x 16 x 2048 101 / 100
+    const int QB = cache->hd == 64 && !out_f32 && !qhl && pairs * ((qtiles + 7) / 8) >= 768 ? 2 : 1;
     a.tiles = (qtiles + 4 * QB - 1) / (4 * QB);
-    const long long groups = ((long long)cache->rows * cache->H + 7) / 8 * 8;
-    ACMI_REQUIRE(groups * a.tiles <= 0x7fffffffLL, "acmi_kv8_attn: %lld workgroups", groups * a.tiles);
-    const dim3 mgrid((unsigned)(groups * a.tiles));
-#define KV8_MANY(HDv, Q, P) hipLaunchKernelGGL((kv8_attn_many_kernel<HDv, Q, P, (HDv <= 64 ? 2 : 1)>), mgrid, dim3(256), 0, st, a)
+    ACMI_REQUIRE(pairs * a.tiles <= 0x7fffffffLL, "acmi_kv8_attn: %lld workgroups", pairs * a.tiles);
+    const dim3 mgrid((unsigned)(pairs * a.tiles));
+#define KV8_MANY(HDv, Q, P, QBv) hipLaunchKernelGGL((kv8_attn_many_kernel<HDv, Q, P, QBv>), mgrid, dim3(256), 0, st, a)
 #define KV8_CASE(HDv)                                            \
     case HDv:                                                    \
-        if (out_f32) KV8_MANY(HDv, true, true);                  \
-        else if (qhl) KV8_MANY(HDv, true, false);                \
-        else KV8_MANY(HDv, false, false);                        \
+        if (out_f32) KV8_MANY(HDv, true, true, 1);               \
+        else if (qhl) KV8_MANY(HDv, true, false, 1);             \
+        else if (QB == 1) KV8_MANY(HDv, false, false, 1);        \
+        else KV8_MANY(64, false, false, 2);                      \
         break;
     KV8_HD_SWITCH(cache->hd, KV8_CASE)
 #undef KV8_CASE
