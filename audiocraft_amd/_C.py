@@ -260,6 +260,9 @@ def dtype_code(dt: torch.dtype) -> int:
     raise ValueError(f"unsupported dtype {dt}")
 
 
+_CODES = {torch.float32: F32, torch.bfloat16: BF16}   # (for callers that have checked the type)
+
+
 # ---------------------------------------------------------------------------------- thin wrappers
 
 def rvq_codebook_norms(codebooks: torch.Tensor) -> torch.Tensor:
@@ -701,18 +704,16 @@ def kv8_attn(cache: KV8CacheDesc, work_floats: int, q, q_strides, S, out, lens, 
              starts=None, k_new=None, v_new=None):
     """q [rows, (S,) Hq, hd] with strides (row, query, head) -> out [rows, (S,) Hq, hd] dense; k_new / v_new [rows, H, hd];
     work_floats: kv8_attn_work_floats(cache, S, Hq)."""
-    Hq = q.shape[-2]
     if k_new is None:
         new = (None, None, 0, 0, 0, 0, 0)
     else:
         kn, vn = k_new.stride(), v_new.stride()
-        new = (k_new.data_ptr(), v_new.data_ptr(), dtype_code(k_new.dtype), kn[0], kn[1], vn[0], vn[1])
+        new = (k_new.data_ptr(), v_new.data_ptr(), _CODES[k_new.dtype], kn[0], kn[1], vn[0], vn[1])
     work = torch.empty(work_floats, device=q.device, dtype=torch.float32) if work_floats else None
-    code = dtype_code(out.dtype)
-    d = KV8AttnDesc(q.data_ptr(), dtype_code(q.dtype), *q_strides, S, Hq, lens.data_ptr(), 1, len_bias,
+    code = _CODES[out.dtype]   # (OUT_F32 / OUT_BF16 are the types' codes)
+    d = KV8AttnDesc(q.data_ptr(), _CODES[q.dtype], *q_strides, S, q.shape[-2], lens.data_ptr(), 1, len_bias,
                     None if q_lens is None else q_lens.data_ptr(), None if starts is None else starts.data_ptr(), causal,
-                    past_context, *new, 0, out.data_ptr(), OUT_BF16 if code == BF16 else OUT_F32,
-                    code, 0, 0, None if work is None else work.data_ptr())
+                    past_context, *new, 0, out.data_ptr(), code, code, 0, 0, None if work is None else work.data_ptr())
     launch(q.get_device(), 'acmi_kv8_attn', _kv8_attn, C.byref(cache), C.byref(d))
     return out
 
@@ -737,12 +738,12 @@ def linear_i8(x, w, w_scale, out, bias=None, residual=None, act=0, a_scale=None,
         nw = _linear_i8_work(M, K)
         if nw:
             work = torch.empty(nw, device=x.device, dtype=torch.uint8)
-        src = (x.data_ptr(), dtype_code(x.dtype), x.stride(0) if M > 1 else K, None if work is None else work.data_ptr())
+        src = (x.data_ptr(), _CODES[x.dtype], x.stride(0) if M > 1 else K, None if work is None else work.data_ptr())
         act8 = (None, None)
     else:
         src, act8 = (None, 0, 0, None), (x.data_ptr(), a_scale.data_ptr())
     d = LinearI8Desc(*act8, w.data_ptr(), w_scale.data_ptr(), None if bias is None else bias.data_ptr(),
-                     None if residual is None else residual.data_ptr(), out.data_ptr(), dtype_code(out.dtype), N, act, M, N, K, *src)
+                     None if residual is None else residual.data_ptr(), out.data_ptr(), _CODES[out.dtype], N, act, M, N, K, *src)
     launch(out.get_device(), 'acmi_linear_i8', _linear_i8, C.byref(d))
     return out
 

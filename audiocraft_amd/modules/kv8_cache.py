@@ -68,6 +68,9 @@ class KV8Cache:
     def _data(self, who: str, name: str, t: torch.Tensor, shape) -> torch.Tensor:
         if not isinstance(t, torch.Tensor) or t.shape != shape:
             raise ValueError(f"KV8Cache.{who}: {name} {tuple(getattr(t, 'shape', ()))}, expected {tuple(shape)}")
+        return self._rows(who, name, t)
+
+    def _rows(self, who: str, name: str, t: torch.Tensor) -> torch.Tensor:
         dt = t.dtype
         if (dt is not torch.float32 and dt is not torch.bfloat16) or t.get_device() != self._index:
             raise ValueError(f"KV8Cache.{who}: {name} is {dt} on {t.device}, expected float32 or bfloat16 on {self.device}")
@@ -123,8 +126,7 @@ class KV8Cache:
         [rows, G * heads, head_dim] attended over lens[r] + 1 tokens, in one launch (`lens` is not advanced).  past_context > 0:
         only the last past_context tokens before it are seen; starts [rows]: first token seen.  A row that is full (lens[r] at the
         capacity) drops the token and attends to what it holds.  -> like q, in q's dtype."""
-        Hq = self._q_heads('decode', q, 3)
-        q = self._data('decode', 'q', q, (self.rows, Hq, self.head_dim))
+        q, Hq = self._queries('decode', q, 3)
         k = self._data('decode', 'k', k, (self.rows, self.heads, self.head_dim))
         v = self._data('decode', 'v', v, k.shape)
         if k.dtype != v.dtype:
@@ -142,9 +144,8 @@ class KV8Cache:
         past_context > 0 each sees only that many tokens before itself.  Not causal: every query sees the whole row (the states of
         an encoder).  starts [rows]: first token seen.  A query that sees nothing, and queries past q_lens[r], give zeros.
         -> like q, in q's dtype."""
-        Hq = self._q_heads('attend', q, 4)
+        q, Hq = self._queries('attend', q, 4)
         S = q.shape[1]
-        q = self._data('attend', 'q', q, (self.rows, S, Hq, self.head_dim))
         past = self._past('attend', past_context)
         if past and not causal:
             raise ValueError("KV8Cache.attend: past_context needs causal=True")
@@ -156,10 +157,11 @@ class KV8Cache:
                 _C.kv8_attn(self.desc, self._work(S, Hq), q, q.stride()[:3], S, out, lens, 0, bool(causal), past, q_lens, starts)
         return out
 
-    def _q_heads(self, who: str, q: torch.Tensor, dims: int) -> int:
-        if not isinstance(q, torch.Tensor) or q.dim() != dims or q.shape[-2] == 0 or q.shape[-2] % self.heads:
-            raise ValueError(f"KV8Cache.{who}: q {tuple(getattr(q, 'shape', ()))}: {dims} dimensions, heads a multiple of {self.heads}")
-        return q.shape[-2]
+    def _queries(self, who: str, q: torch.Tensor, dims: int) -> tp.Tuple[torch.Tensor, int]:
+        sh = q.shape if isinstance(q, torch.Tensor) else ()
+        if len(sh) != dims or sh[0] != self.rows or sh[-1] != self.head_dim or sh[-2] == 0 or sh[-2] % self.heads:
+            raise ValueError(f"KV8Cache.{who}: q {tuple(sh)}: {dims} dimensions, {self.rows} rows, heads a multiple of {self.heads}, head_dim {self.head_dim}")
+        return self._rows(who, 'q', q), sh[-2]
 
     def _past(self, who: str, past_context: tp.Optional[int]) -> int:
         past = int(past_context or 0)
