@@ -237,7 +237,7 @@ typedef struct {
     /* 0.3.0: self-attention cache in 8 bits: host pointer to an acmi_kv8_cache of Beff rows, num_heads heads and tail_dtype ==
      * kvdtype, or NULL (on every layer or none).  k_cache / v_cache are then unused; the step's QKV launch appends to the tail
      * and its attention (acmi_kv8_attn) quantises a block that the position completes.  One position per call, or the one-forward
-     * prefill (which stores the whole prompt, acmi_kv8_store, after attending to it in kvdtype); no rotary positions, no
+     * prefill from position 0 (which stores the whole prompt, acmi_kv8_store, after attending to it in kvdtype); no rotary positions, no
      * qk_layer_norm (both rewrite the appended key), head size 16 .. 128. */
     const void* kv8;
 } acmi_lm_layer;

@@ -294,6 +294,38 @@ def test_attend(KV8Cache, dt, causal, past, H, G, hd, S):
         assert (got[r, dead] == 0).all()
 
 
+@pytest.mark.parametrize('H,G,hd,S', [(1, 1, 64, 64), (1, 1, 64, 65), (1, 1, 128, 64), (1, 1, 128, 65), (1, 33, 16, 2), (1, 13, 32, 5), (2, 1, 64, 129)])
+@pytest.mark.parametrize('dt', ['f32', 'bf16'])
+def test_attend_where_the_forms_change(KV8Cache, dt, H, G, hd, S):
+    """One column more than the split form takes, one more than a workgroup's tiles."""
+    dt, lens = DT[dt], [190, S, 0]
+    c, k, v = filled(KV8Cache, lens, H, hd, dt, S + G)
+    q = torch.randn(3, S, H * G, hd, generator=torch.Generator().manual_seed(S)).to(dt)
+    got = c.attend(q.cuda(), words(*lens))
+    for r, n in enumerate(lens):
+        kr, vr = k[r, :n].float(), v[r, :n].float()
+        check(got[r], attention(q[r].double(), held(kr), held(vr), True, S, 0, 0), dt, max(vr.abs().max().item() if n else 0, 1e-30))
+
+
+@pytest.mark.parametrize('causal,past', [(True, 0), (True, 90), (False, 0)])
+def test_attend_on_a_full_grid(KV8Cache, causal, past):
+    """Enough heads that a wave takes two column tiles."""
+    H, hd, S, lens = 384, 64, 70, [333, 64]
+    c, k, v = filled(KV8Cache, lens, H, hd, torch.bfloat16, 41)
+    q = torch.randn(2, S, H, hd, generator=torch.Generator().manual_seed(42)).bfloat16()
+    starts, q_lens = [0, 9], [S, 50]
+    got = c.attend(q.cuda(), words(*lens), causal, past, words(*q_lens), words(*starts))
+    for r, n in enumerate(lens):
+        kr, vr = k[r, :n].float(), v[r, :n].float()
+        s = torch.einsum('shd,thd->hst', q[r].double(), held(kr)) / math.sqrt(hd)
+        i, t = (n - q_lens[r] + torch.arange(S))[:, None], torch.arange(n)[None]
+        seen = (t >= starts[r]) & (torch.arange(S)[:, None] < q_lens[r])
+        if causal:
+            seen = seen & (t <= i) & ((t >= i - past) if past else (t >= 0))
+        p = torch.softmax(s.masked_fill(~seen, -math.inf), -1).nan_to_num(0.0)
+        check(got[r], torch.einsum('hst,thd->shd', p, held(vr)), torch.bfloat16, vr.abs().max().item())
+
+
 def test_attend_long_context_is_split_and_joined(KV8Cache):
     """One row, 9000 tokens: the split form; the same call again gives the same bits."""
     c, k, v = filled(KV8Cache, [9000, 70], 2, 64, torch.float32, 4)

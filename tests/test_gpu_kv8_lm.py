@@ -21,7 +21,7 @@ def models(wdt=torch.float32, dims=(256, 4, 3), **kw):
     dim, heads, layers = dims
     cfg = dict(dim=dim, num_heads=heads, num_layers=layers, n_q=4, card=512, hidden_scale=4, cfg_coef=3.0,
                conditioners={'description': {'kind': 't5', 'embedder': 'synthetic', 'dim': 64, 'length': 6}},
-               fuser={'cross': ['description']}, **kw)
+               **{'fuser': {'cross': ['description']}, **kw})
     out = []
     for kv in (None, torch.int8):
         torch.manual_seed(0)
@@ -86,6 +86,22 @@ def test_generate_with_a_prompt(wdt, prefill, monkeypatch):
     t2, l2 = b.generate(prompt, [], use_graph=False, **kw)
     assert torch.equal(t1, t2) and torch.equal(l1, l2)
     assert rel(l1[:, :, 0], l0[:, :, 0]) < 3e-2        # the first decision: same past
+
+
+@pytest.mark.parametrize('fuser', ['cross', 'prepend'])
+def test_two_step_guidance(fuser):
+    """Conditional and unconditional rows of their own condition length; prepended, the shorter stream is padded on the left and its
+    first positions are never seen.  Within 64 positions as with the plain cache, beyond captured and eager steps agree."""
+    a, b = models(fuser={fuser: ['description']})
+    B = 2
+
+    def source(n, seed):
+        return {'description': (torch.randn(B, n, 256, generator=torch.Generator().manual_seed(seed)).cuda(), torch.ones(B, n, dtype=torch.int64).cuda())}
+    kw = dict(num_samples=B, use_sampling=False, condition_tensors=(source(6, 1), source(2, 2)), return_logits=True)
+    (t0, l0), (t1, l1) = (m.generate(None, [], max_gen_len=40, **kw) for m in (a, b))
+    assert torch.equal(t0, t1) and rel(l1, l0) < 1e-4
+    (t2, l2), (t3, l3) = (b.generate(None, [], max_gen_len=150, use_graph=g, **kw) for g in (True, False))
+    assert torch.equal(t2, t3) and torch.equal(l2, l3) and torch.isfinite(l2).all()
 
 
 def test_streaming_state_goes_out_and_in():
