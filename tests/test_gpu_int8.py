@@ -81,6 +81,16 @@ def test_long_rows(Int8Linear, M, N, K):
     check(Int8Linear(w.cuda(), bias.cuda()), x, w, bias, 'none')
 
 
+def test_results_past_32_bit_offsets(Int8Linear):
+    if torch.cuda.mem_get_info()[0] < 30 << 30:
+        pytest.skip("needs 30 GB")
+    x, w, bias = make(66000, 33000, 64, torch.bfloat16, 7)
+    got = Int8Linear(w.cuda(), bias.cuda())(x.cuda())
+    for r in (0, 32600, 65200, 65999):
+        y, err = reference(x[r:r + 1], w, bias, 'none', None)
+        assert ((got[r].cpu().double() - y[0]).abs() <= err[0]).all(), r
+
+
 @pytest.mark.parametrize('M', [2, 20, 100])
 @pytest.mark.parametrize('N', [96, 95])
 def test_residual_no_bias_and_leading_dimensions(Int8Linear, M, N):

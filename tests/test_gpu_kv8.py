@@ -537,6 +537,27 @@ def test_tiled_output_and_one_length_word(KV8Cache):
         assert torch.equal(getattr(c, name), getattr(whole, name))
 
 
+def test_positions_past_32_bit_offsets(KV8Cache):
+    """Row 1 begins past 2^31 bytes, its newest tokens lie 2^31 bytes further on."""
+    if torch.cuda.mem_get_info()[0] < 30 << 30:
+        pytest.skip("needs 30 GB")
+    hd, start, n, past = 128, 16999040, 200, 100
+    c = KV8Cache(2, 1, hd, 17000000)
+    k, v = make(1, n, 1, hd, torch.float32, 50)
+    both = [torch.cat([x, x]).cuda() for x in (k, v)]
+    c.store(*both, words(0, start), words(0, n))
+    q = torch.randn(2, 70, 1, hd, generator=torch.Generator().manual_seed(51))
+    kr, vr = k[0].bfloat16().float(), v[0].bfloat16().float()
+    for S in (3, 70):
+        got = c.attend(q[:, :S].cuda(), words(0, start + n), past_context=past)
+        assert (got[0] == 0).all()
+        check(got[1], attention(q[1, :S].double(), held(kr), held(vr), True, S, past, 0), torch.float32, vr.abs().max().item())
+    k1 = torch.randn(2, 1, hd, generator=torch.Generator().manual_seed(52))
+    got = c.decode(q[:, 0].cuda(), k1.cuda(), k1.cuda(), words(0, start + n), past)
+    kr, vr = (torch.cat([x, k1[1:].bfloat16().float()]) for x in (kr, vr))
+    check(got[1:2], attention(q[1, :1].double(), held(kr), held(vr), True, 1, past, 0), torch.float32, max(vr.abs().max().item(), 1))
+
+
 def test_another_stream(KV8Cache):
     c, k, v = filled(KV8Cache, [700], 2, 64, torch.float32, 14)
     q = torch.randn(1, 1, 2, 64, device='cuda')
