@@ -655,14 +655,12 @@ __device__ __forceinline__ void kv8_put4(const Kv8AttnArgs& p, int row, int s, i
     }
 }
 
-// ---- few queries: one workgroup per (split, column tile of a cache head, row); its 8 waves take the blocks in turn, four of them
-// 16 tokens of the tail each, and are joined through LDS.  A wave keeps one block in flight: the next block's K is requested as
+// ---- few queries: one workgroup per (split, column tile of a cache head, row); its NW waves take the blocks in turn, the last four of
+// them 16 tokens of the tail each, and are joined through LDS.  A wave keeps one block in flight: the next block's K is requested as
 // soon as this block's K has been multiplied, its V likewise.  Bound by the codes' bytes: 4 rows of 9001 to 32768 tokens x 8 heads of
-// 128, 171 MB in 35.5 us = 4.8 TB/s, the rate of a large copy; 16 rows of 500 to 1251 x 24 heads of 64 43 MB in 15.6 us.
-// Waves per workgroup and (launch bound) per SIMD: every wave has a block in flight, so two workgroups of 8 (hd 128: of 4) cover the
-// memory's latency.  16 rows of 500 to 1251 tokens x 24 heads of 64: 8 waves, 4 per SIMD 15.6 us (at 2 per SIMD 17.2); one row's
-// first token 6.7 (4 waves 7.1).  32768 tokens, hd 128: 4 waves, 2 per SIMD 35.5 us; 8 waves 40.2; 1 per SIMD 42.2.
-template <int HD> constexpr int kv8_nw() { return HD == 128 ? 4 : 8; }
+// 128, 171 MB in 35.2 us = 4.9 TB/s, the rate of a large copy; 64 rows of 1400 x 24 heads of 64 4.4 TB/s; 16 rows of 750 2.5 TB/s.
+// Launch bound per SIMD: a wave's block in flight takes 128 registers at 64 features, 240 at 128.  16 rows of 500 to 1251 tokens x
+// 24 heads of 64, 8 waves: 4 per SIMD 15.6 us, 2 17.2; 32768 tokens, hd 128: 2 per SIMD 35.5 us, 1 42.2, 8 waves per workgroup 40.2.
 template <int HD> constexpr int kv8_wpe() { return HD == 128 ? 2 : 4; }
 
 __device__ __forceinline__ float raw8(bf16_t v) { return bf16_to_f32(v); }
@@ -812,11 +810,11 @@ __device__ __forceinline__ void kv8_tail16(const Kv8AttnArgs& p, const Kv8RowInf
 // The leading arguments are what the first requests need -- query, length word, tail -- and arrive in scalar registers at wave
 // start (kernarg preload); the rest of the descriptor is fetched behind those requests.
 //   g0 = H | G << 16   g1 = column tiles | q bf16 << 16 | tail bf16 << 17 | length per row << 18   query strides in elements
-template <int HD, bool QHL, bool PHL>
-__global__ __launch_bounds__(kv8_nw<HD>() * 64, kv8_wpe<HD>()) void kv8_attn_split_kernel(const void* hq, const int* hlen, const void* hkt, const void* hvt,
-                                                                                          unsigned g0, unsigned g1, int q_row, int q_tok, int q_head, int S,
-                                                                                          const Kv8AttnArgs p) {
-    constexpr int NK = Kv8Geo<HD>::NK, ND = Kv8Geo<HD>::ND, KW = Kv8Geo<HD>::KW, PITCH = HD + 4, NW = kv8_nw<HD>();
+template <int HD, bool QHL, bool PHL, int NW>
+__global__ __launch_bounds__(NW * 64, kv8_wpe<HD>()) void kv8_attn_split_kernel(const void* hq, const int* hlen, const void* hkt, const void* hvt,
+                                                                                unsigned g0, unsigned g1, int q_row, int q_tok, int q_head, int S,
+                                                                                const Kv8AttnArgs p) {
+    constexpr int NK = Kv8Geo<HD>::NK, ND = Kv8Geo<HD>::ND, KW = Kv8Geo<HD>::KW, PITCH = HD + 4;
     __shared__ __attribute__((aligned(16))) float sm_o[NW][16][PITCH];
     __shared__ float sm_m[NW][16], sm_l[NW][16];
     __shared__ Kv8QuantLds<HD> sm_q;
@@ -829,17 +827,21 @@ __global__ __launch_bounds__(kv8_nw<HD>() * 64, kv8_wpe<HD>()) void kv8_attn_spl
     const int len0 = hlen[(g1 >> 18 & 1) ? row : 0];
     float x[NK][8];
     Kv8TailRaw<HD> raw;
+    const bool early = g1 >> 19 & 1;
     const int tw = wave - (NW - 4);   // the last four waves take 16 places of the tail each (they have the fewer blocks)
     {
         // column -> query and head (a column past the last one reads some query of the call)
         const int cidx = qt * 16 + nl, sq = (int)(((float)cidx + 0.5f) * __builtin_amdgcn_rcpf((float)G)), g = cidx - sq * G;
         const size_t qb = (size_t)((long long)row * q_row + (long long)min(sq, S - 1) * q_tok + (long long)(kvh * G + g) * q_head);
-        if (tw >= 0) kv8_tail_request<HD>(hkt, hvt, (((size_t)row * H + kvh) * BLK + tw * 16) * HD, g1 >> 17 & 1, nl, kg, raw);
+        if (early && tw >= 0) kv8_tail_request<HD>(hkt, hvt, (((size_t)row * H + kvh) * BLK + tw * 16) * HD, g1 >> 17 & 1, nl, kg, raw);
         kv8_load_q<HD>(hq, qb, g1 >> 16 & 1, kg, x);
     }
     const Kv8RowInfo ri = kv8_row_of(p, row, len0);
     const Kv8Span sp = kv8_span(p, ri, qt * 16, min(qt * 16 + 16, p.S * p.G));
     if (split >= sp.eff) return;
+    const bool mine = split == sp.eff - 1;   // the split that owns the tail
+    const bool tail = mine && sp.tail && tw >= 0 && (ri.len - 1) / BLK * BLK + tw * 16 < ri.len;
+    if (!early && tail) kv8_tail_request<HD>(hkt, hvt, (((size_t)row * H + kvh) * BLK + tw * 16) * HD, g1 >> 17 & 1, nl, kg, raw);
     const int s0 = sp.bf + split * p.chunk, s1 = sp.eff == 1 ? sp.bt : min(sp.bt, s0 + p.chunk);
     const size_t rh = (size_t)row * p.c.H + kvh, hb = rh * p.c.nblk;
     const uint8_t* kc = reinterpret_cast<const uint8_t*>(p.c.k_codes) + hb * (size_t)(BLK * HD);
@@ -869,8 +871,7 @@ __global__ __launch_bounds__(kv8_nw<HD>() * 64, kv8_wpe<HD>()) void kv8_attn_spl
     if (b < s1) { get_k(b); get_v(b); }
     Kv8Col<HD, QHL> c[1];
     kv8_column<HD, QHL>(p, ri, qt * 16 + nl, x, c[0]);
-    const bool mine = split == sp.eff - 1;   // the split that owns the tail
-    if (mine && sp.tail && tw >= 0 && (ri.len - 1) / BLK * BLK + tw * 16 < ri.len) kv8_tail16<HD, QHL>(p, ri, row, kvh, tw * 16, raw, x, c[0]);
+    if (tail) kv8_tail16<HD, QHL>(p, ri, row, kvh, tw * 16, raw, x, c[0]);
     while (b < s1) {
         // the next requests are not conditional (a wave's last ones read its last block again, from the cache): the waits of a
         // straight line count them exactly, those behind a branch would wait for everything
@@ -1307,7 +1308,7 @@ static bool kv8_few(int S, int G) { return S == 1 || ((long long)S * G + 15) / 1
 static void kv8_split_plan(const acmi_kv8_cache* c, int S, int G, int* splits, int* chunk) {
     const long long tiles = (long long)c->H * ((S * G + 15) / 16) * c->rows;
     long long n = 1;
-    const int least = 4 * (c->hd == 128 ? kv8_nw<128>() : kv8_nw<64>());   // four blocks per wave: below, the second launch costs more
+    const int least = c->hd == 128 ? 16 : 32;   // four blocks per wave: below, the second launch costs more
     if (tiles * 4 <= KV8_TARGET) n = max(1LL, min(min(KV8_TARGET / tiles, (long long)(c->nblk / least)), (long long)KV8_MAX_SPLITS));
     *chunk = (int)((c->nblk + n - 1) / n);
     *splits = (c->nblk + *chunk - 1) / *chunk;
@@ -1371,17 +1372,31 @@ extern "C" int acmi_kv8_attn(const acmi_kv8_cache* cache, const acmi_kv8_attn_de
         ACMI_REQUIRE(d.q_row == (int)d.q_row && (d.S == 1 || d.q_tok == (int)d.q_tok) && d.q_head == (int)d.q_head && a.G <= 65535,
                      "acmi_kv8_attn: query strides beyond 2^31 elements, or %d query heads per cache head", a.G);
         const unsigned g0 = (unsigned)cache->H | (unsigned)a.G << 16;
-        const unsigned g1 = (unsigned)qtiles | (unsigned)a.q_bf16 << 16 | (unsigned)(cache->tail_dtype == ACMI_BF16) << 17 | (unsigned)d.len_stride << 18;
-#define KV8_SPLIT(HDv, Q, P) hipLaunchKernelGGL((kv8_attn_split_kernel<HDv, Q, P>), grid, dim3(kv8_nw<HDv>() * 64), 0, st, a.q, a.len, cache->k_tail, cache->v_tail, g0, g1, (int)d.q_row, d.S > 1 ? (int)d.q_tok : 0, (int)d.q_head, d.S, a)
+        // A grid of at most one workgroup per CU is one chain of latencies: 8 waves share the blocks, and the tail is requested before
+        // the row's length is known.  Larger grids are bytes: 4 waves, twice the workgroups in flight, and only the part of the tail
+        // that is needed, by the split that needs it.  us in a graph, caches cold, 8 waves / 4: 16 rows x 24 heads of 64, 750 tokens
+        // 16.5 / 15.4 (bf16 15.7 / 14.2), 64 rows 41.8 / 38.5, 16 rows x 200 tokens 8.9 / 10.2; tail early / late: 64 rows x 200 tokens
+        // f32 28.2 / 23.2, 2 rows x 16 heads x 700 tokens 8.6 / 9.1, 128 rows x 8 x 4 heads of 128 x 1000 tokens 72.6 / 62.2
+        const long long wgs = (long long)grid.x * grid.y * grid.z;
+        const bool early = a.splits == 1 && wgs <= 256, wide = cache->hd <= 64 && wgs <= 256;
+        const unsigned g1 = (unsigned)qtiles | (unsigned)a.q_bf16 << 16 | (unsigned)(cache->tail_dtype == ACMI_BF16) << 17 | (unsigned)d.len_stride << 18 |
+                            (unsigned)early << 19;
+#define KV8_SPLIT_NW(HDv, Q, P, NWv)                                                                                                              \
+    hipLaunchKernelGGL((kv8_attn_split_kernel<HDv, Q, P, NWv>), grid, dim3(NWv * 64), 0, st, a.q, a.len, cache->k_tail, cache->v_tail, g0, g1,        \
+                       (int)d.q_row, d.S > 1 ? (int)d.q_tok : 0, (int)d.q_head, d.S, a)
+#define KV8_SPLIT(HDv, Q, P)                                               \
+    if (wide) KV8_SPLIT_NW(HDv, Q, P, (HDv <= 64 ? 8 : 4));               \
+    else KV8_SPLIT_NW(HDv, Q, P, 4)
 #define KV8_CASE(HDv)                                            \
     case HDv:                                                    \
-        if (out_f32) KV8_SPLIT(HDv, true, true);                 \
-        else if (qhl) KV8_SPLIT(HDv, true, false);               \
-        else KV8_SPLIT(HDv, false, false);                       \
+        if (out_f32) { KV8_SPLIT(HDv, true, true); }             \
+        else if (qhl) { KV8_SPLIT(HDv, true, false); }           \
+        else { KV8_SPLIT(HDv, false, false); }                   \
         break;
         KV8_HD_SWITCH(cache->hd, KV8_CASE)
 #undef KV8_CASE
 #undef KV8_SPLIT
+#undef KV8_SPLIT_NW
         if (int rc = acmi_check_launch("kv8_attn_split_kernel")) return rc;
         if (a.splits == 1) return ACMI_OK;
         const dim3 jgrid(min(d.S * a.G, 16), cache->H * qtiles, cache->rows);
