@@ -1299,9 +1299,16 @@ extern "C" int acmi_kv8_load(const acmi_kv8_cache* cache, const int* len, int T,
     return acmi_check_launch("kv8_load_kernel");
 }
 
-// column tiles up to which the split form runs; one query per head always does (it alone stores a new token)
-constexpr int KV8_SPLIT_TILES = 4;
-static bool kv8_few(int S, int G) { return S == 1 || ((long long)S * G + 15) / 16 <= KV8_SPLIT_TILES; }
+// The split form: one query per head (it alone stores a new token), one column tile, or few workgroups, three per CU -- a workgroup of
+// it has a column tile and its waves share the blocks, where the prompt form's waves walk all blocks with a tile each.  Measured, us
+// split / prompt form, in a graph: 4 x 8 heads x 128 queries of 300 (256 workgroups) 8.9 / 12.8, 1 x 16 x 600 of 600 (608) 13.1 /
+// 18.4, 1 x 8 x 128 of 8000 (64) 23.8 / 137, 16 x 24 x 29 of 600 (768) 20.8 / 24.6; 8 x 8 x 200 of 600 (832) 19.5 / 18.9,
+// 16 x 12 x 77 of 251 (960) 19.6 / 15.7, 64 x 8 x 4 x 16 of 1000 (2048) 65.6 / 38.8
+constexpr int KV8_SPLIT_WGS = 768;
+static bool kv8_few(const acmi_kv8_cache* c, int S, int G) {
+    const long long tiles = ((long long)S * G + 15) / 16;
+    return S == 1 || tiles == 1 || tiles * c->H * c->rows <= KV8_SPLIT_WGS;
+}
 // Blocks per workgroup: the longest possible row in so many chunks that the call has about KV8_TARGET workgroups; one chunk (and
 // no second launch) when the tiles alone fill the chip.  The rows' lengths are not known here: shorter rows take fewer chunks of
 // the same size, so that all workgroups take equally long.
@@ -1317,7 +1324,7 @@ static void kv8_split_plan(const acmi_kv8_cache* c, int S, int G, int* splits, i
 extern "C" size_t acmi_kv8_attn_work_floats(const acmi_kv8_cache* cache, int S, int Hq) {
     if (kv8_check(cache, "acmi_kv8_attn_work_floats") || S <= 0 || Hq <= 0 || Hq % cache->H) return 0;
     const int G = Hq / cache->H;
-    if (!kv8_few(S, G)) return 0;
+    if (!kv8_few(cache, S, G)) return 0;
     int sp, chunk;
     kv8_split_plan(cache, S, G, &sp, &chunk);
     return sp == 1 ? 0 : (size_t)cache->rows * cache->H * ((S * G + 15) / 16) * sp * 16 * (cache->hd + 4);
@@ -1361,7 +1368,8 @@ extern "C" int acmi_kv8_attn(const acmi_kv8_cache* cache, const acmi_kv8_attn_de
     const bool qhl = d.q_dtype == ACMI_F32 || out_f32;   // (a bf16 query is one f16 exactly)
     hipStream_t st = (hipStream_t)stream;
     const int qtiles = (d.S * a.G + 15) / 16;
-    if (kv8_few(d.S, a.G)) {
+    const bool narrow = d.q_row == (int)d.q_row && (d.S == 1 || d.q_tok == (int)d.q_tok) && d.q_head == (int)d.q_head;   // query strides below 2^31
+    if (kv8_few(cache, d.S, a.G) && (narrow || d.S == 1)) {
         kv8_split_plan(cache, d.S, a.G, &a.splits, &a.chunk);
         a.work = d.work;
         ACMI_REQUIRE(a.splits == 1 || (d.work != nullptr && (reinterpret_cast<size_t>(d.work) & 15) == 0),
@@ -1369,8 +1377,7 @@ extern "C" int acmi_kv8_attn(const acmi_kv8_cache* cache, const acmi_kv8_attn_de
         ACMI_REQUIRE((long long)cache->H * qtiles <= 65535, "acmi_kv8_attn: %d heads x %d column tiles", cache->H, qtiles);
         const dim3 grid(cache->H * qtiles, cache->rows, a.splits);
         a.tiles = qtiles;
-        ACMI_REQUIRE(d.q_row == (int)d.q_row && (d.S == 1 || d.q_tok == (int)d.q_tok) && d.q_head == (int)d.q_head && a.G <= 65535,
-                     "acmi_kv8_attn: query strides beyond 2^31 elements, or %d query heads per cache head", a.G);
+        ACMI_REQUIRE(narrow && a.G <= 65535, "acmi_kv8_attn: query strides beyond 2^31 elements, or %d query heads per cache head", a.G);
         const unsigned g0 = (unsigned)cache->H | (unsigned)a.G << 16;
         // A grid of at most one workgroup per CU is one chain of latencies: 8 waves share the blocks, and the tail is requested before
         // the row's length is known.  Larger grids are bytes: 4 waves, twice the workgroups in flight, and only the part of the tail
@@ -1408,8 +1415,8 @@ extern "C" int acmi_kv8_attn(const acmi_kv8_cache* cache, const acmi_kv8_attn_de
     const long long pairs = ((long long)cache->rows * cache->H + 7) / 8 * 8;
     // two column tiles per wave where bf16 results at 64 features leave the registers for it and the workgroups still fill the chip,
     // three per CU.  Measured, us one / two: 4 x 16 heads x 4096 tokens (2048 workgroups of two) 273 / 241, 16 x 24 x 600 (1920)
-    // 58.8 / 56.6, 8 x 8 x 4 x 512 of 2048 (1024) 120 / 114; 16 x 16 x 100 of 1500 (256) 36.9 / 44.4, 4 x 8 x 128 of 300 (32)
-    // 10.8 / 14.8; f32 4 x 16 x 4096 341 / 344; hd 32 8 x 16 x 2048 101 / 100
+    // 58.8 / 56.6, 8 x 8 x 4 x 512 of 2048 (1024) 120 / 114; 16 x 16 x 100 of 1500 (256) 36.9 / 44.4; f32 4 x 16 x 4096 341 / 344;
+    // hd 32 8 x 16 x 2048 101 / 100
     const int QB = cache->hd == 64 && !out_f32 && !qhl && pairs * ((qtiles + 7) / 8) >= 768 ? 2 : 1;
     a.tiles = (qtiles + 4 * QB - 1) / (4 * QB);
     ACMI_REQUIRE(pairs * a.tiles <= 0x7fffffffLL, "acmi_kv8_attn: %lld workgroups", pairs * a.tiles);

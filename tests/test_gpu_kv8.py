@@ -29,6 +29,37 @@ def KV8Cache():
     return KV8Cache
 
 
+@pytest.fixture(params=['own rows', 'among many rows'])
+def AnyCache(request, KV8Cache):
+    """The cache, or the same rows in front of 800 empty ones: the grid is then large, and prompts take the form for that."""
+    if request.param == 'own rows':
+        return KV8Cache
+
+    class Among(KV8Cache):
+        extra = 800
+
+        def __init__(self, rows, *a, **kw):
+            super().__init__(rows + self.extra, *a, **kw)
+
+        def more(self, t):
+            if t is None or t.shape[0] == self.rows:
+                return t
+            out = t.new_zeros(self.rows, *t.shape[1:])
+            out[:t.shape[0]] = t
+            return out
+
+        def store(self, k, v, start=None, n=None):
+            n = torch.full((k.shape[0],), k.shape[1], dtype=torch.int32, device='cuda') if n is None else n
+            super().store(self.more(k), self.more(v), self.more(start), self.more(n))
+
+        def attend(self, q, lens, causal=True, past_context=0, q_lens=None, starts=None):
+            return super().attend(self.more(q), self.more(lens), causal, past_context, self.more(q_lens), self.more(starts))[:q.shape[0]]
+
+        def decode(self, q, k, v, lens, past_context=0, starts=None):
+            return super().decode(self.more(q), self.more(k), self.more(v), self.more(lens), past_context, self.more(starts))[:q.shape[0]]
+    return Among
+
+
 # ------------------------------------------------------------------------------------------ the definition
 
 def quantised(block):
@@ -274,14 +305,14 @@ def test_decode_on_a_full_row_drops_the_token(KV8Cache):
 @pytest.mark.parametrize('dt', ['f32', 'bf16'])
 @pytest.mark.parametrize('causal,past', [(True, 0), (True, 1), (True, 100), (False, 0)])
 @pytest.mark.parametrize('H,G,hd,S', [(2, 1, 64, 1), (1, 4, 64, 5), (2, 2, 128, 70), (1, 3, 32, 150), (3, 1, 16, 33), (1, 1, 64, 200)])
-def test_attend(KV8Cache, dt, causal, past, H, G, hd, S):
+def test_attend(AnyCache, dt, causal, past, H, G, hd, S):
     dt = DT[dt]
     lens = [max(S, 1), 257, 64, 130, 0, 40]
     q_lens = [min(S, n) if causal else S for n in lens]
     q_lens[1] = min(S, 3)                              # a padded batch
     starts = [0, 70, 0, 0, 0, 1000]                    # left padding; the last row sees nothing at all
     R = len(lens)
-    c, k, v = filled(KV8Cache, lens, H, hd, dt, S + hd)
+    c, k, v = filled(AnyCache, lens, H, hd, dt, S + hd)
     g = torch.Generator().manual_seed(S)
     q = torch.randn(R, S, H * G, hd, generator=g).to(dt)
     got = c.attend(q.cuda(), words(*lens), causal=causal, past_context=past, q_lens=words(*q_lens), starts=words(*starts))
@@ -296,10 +327,10 @@ def test_attend(KV8Cache, dt, causal, past, H, G, hd, S):
 
 @pytest.mark.parametrize('H,G,hd,S', [(1, 1, 64, 64), (1, 1, 64, 65), (1, 1, 128, 64), (1, 1, 128, 65), (1, 33, 16, 2), (1, 13, 32, 5), (2, 1, 64, 129)])
 @pytest.mark.parametrize('dt', ['f32', 'bf16'])
-def test_attend_where_the_forms_change(KV8Cache, dt, H, G, hd, S):
-    """One column more than the split form takes, one more than a workgroup's tiles."""
+def test_attend_where_the_forms_change(AnyCache, dt, H, G, hd, S):
+    """Whole column tiles and one column more, of a workgroup and of a wave."""
     dt, lens = DT[dt], [190, S, 0]
-    c, k, v = filled(KV8Cache, lens, H, hd, dt, S + G)
+    c, k, v = filled(AnyCache, lens, H, hd, dt, S + G)
     q = torch.randn(3, S, H * G, hd, generator=torch.Generator().manual_seed(S)).to(dt)
     got = c.attend(q.cuda(), words(*lens))
     for r, n in enumerate(lens):
@@ -307,14 +338,15 @@ def test_attend_where_the_forms_change(KV8Cache, dt, H, G, hd, S):
         check(got[r], attention(q[r].double(), held(kr), held(vr), True, S, 0, 0), dt, max(vr.abs().max().item() if n else 0, 1e-30))
 
 
+@pytest.mark.parametrize('H', [384, 200])
 @pytest.mark.parametrize('causal,past', [(True, 0), (True, 90), (False, 0)])
-def test_attend_on_a_full_grid(KV8Cache, causal, past):
-    """Enough heads that a wave takes two column tiles."""
-    H, hd, S, lens = 384, 64, 70, [333, 64]
+def test_attend_on_a_full_grid(KV8Cache, causal, past, H):
+    """Enough heads that a wave takes two column tiles, and enough for the prompt form; the queries heads first in memory."""
+    hd, S, lens = 64, 70, [333, 64]
     c, k, v = filled(KV8Cache, lens, H, hd, torch.bfloat16, 41)
     q = torch.randn(2, S, H, hd, generator=torch.Generator().manual_seed(42)).bfloat16()
     starts, q_lens = [0, 9], [S, 50]
-    got = c.attend(q.cuda(), words(*lens), causal, past, words(*q_lens), words(*starts))
+    got = c.attend(q.transpose(1, 2).contiguous().cuda().transpose(1, 2), words(*lens), causal, past, words(*q_lens), words(*starts))
     for r, n in enumerate(lens):
         kr, vr = k[r, :n].float(), v[r, :n].float()
         s = torch.einsum('shd,thd->hst', q[r].double(), held(kr)) / math.sqrt(hd)
@@ -326,9 +358,9 @@ def test_attend_on_a_full_grid(KV8Cache, causal, past):
         check(got[r], torch.einsum('hst,thd->shd', p, held(vr)), torch.bfloat16, vr.abs().max().item())
 
 
-def test_attend_long_context_is_split_and_joined(KV8Cache):
+def test_attend_long_context_is_split_and_joined(AnyCache):
     """One row, 9000 tokens: the split form; the same call again gives the same bits."""
-    c, k, v = filled(KV8Cache, [9000, 70], 2, 64, torch.float32, 4)
+    c, k, v = filled(AnyCache, [9000, 70], 2, 64, torch.float32, 4)
     q = torch.randn(2, 2, 4, 64, generator=torch.Generator().manual_seed(0))
     got = c.attend(q.cuda(), words(9000, 70))
     for r, n in enumerate((9000, 70)):
@@ -337,9 +369,9 @@ def test_attend_long_context_is_split_and_joined(KV8Cache):
         assert torch.equal(got, c.attend(q.cuda(), words(9000, 70)))
 
 
-def test_q_longer_than_the_row(KV8Cache):
+def test_q_longer_than_the_row(AnyCache):
     """Causal queries that would sit before the row's first token see nothing."""
-    c, k, v = filled(KV8Cache, [3, 80], 1, 32, torch.float32, 8)
+    c, k, v = filled(AnyCache, [3, 80], 1, 32, torch.float32, 8)
     q = torch.randn(2, 90, 1, 32, generator=torch.Generator().manual_seed(2))
     got = c.attend(q.cuda(), words(3, 80))
     for r, n in enumerate((3, 80)):
@@ -349,11 +381,11 @@ def test_q_longer_than_the_row(KV8Cache):
 
 
 @pytest.mark.parametrize('S', [1, 100])
-def test_what_is_not_seen_does_not_matter(KV8Cache, S):
+def test_what_is_not_seen_does_not_matter(AnyCache, S):
     """NaN and infinity in tail places past the row's length, in tokens before `starts`, and (causal) in later tokens."""
     n = 150
     k, v = make(1, n, 2, 64, torch.float32, 6)
-    c, d = (KV8Cache(1, 2, 64, 256, dtype=torch.float32) for _ in range(2))
+    c, d = (AnyCache(1, 2, 64, 256, dtype=torch.float32) for _ in range(2))
     c.store(k.cuda(), v.cuda(), words(0))
     kb, vb = k.clone(), v.clone()
     kb[:, :64], vb[:, :64] = math.nan, math.inf         # a whole block before `starts`
@@ -369,8 +401,8 @@ def test_what_is_not_seen_does_not_matter(KV8Cache, S):
     assert torch.isfinite(got).all()
 
 
-def test_queries_with_special_values(KV8Cache):
-    c, k, v = filled(KV8Cache, [200], 1, 64, torch.float32, 9)
+def test_queries_with_special_values(AnyCache):
+    c, k, v = filled(AnyCache, [200], 1, 64, torch.float32, 9)
     q = torch.randn(1, 20, 1, 64, generator=torch.Generator().manual_seed(3))
     q[0, 3, 0, 5] = math.nan
     q[0, 4, 0, 5] = math.inf
@@ -385,11 +417,11 @@ def test_queries_with_special_values(KV8Cache):
     check(got[0, live], ref, torch.float32, v.abs().max().item())
 
 
-def test_large_scores_and_flat_ones(KV8Cache):
+def test_large_scores_and_flat_ones(AnyCache):
     """Scores of +-900 (one token takes all, far tokens underflow) and exactly equal scores over a long row."""
     n = 3000
     k, v = make(1, n, 1, 64, torch.float32, 10)
-    c = KV8Cache(1, 1, 64, n, dtype=torch.float32)
+    c = AnyCache(1, 1, 64, n, dtype=torch.float32)
     c.store(k.cuda(), v.cuda(), words(0))
     q = torch.stack([100.0 * torch.randn(64, generator=torch.Generator().manual_seed(1)), torch.zeros(64)]).view(1, 2, 1, 64)
     got = c.attend(q.cuda(), words(n), causal=False)
@@ -401,7 +433,7 @@ def test_large_scores_and_flat_ones(KV8Cache):
 
 @pytest.mark.parametrize('S', [1, 100])
 @pytest.mark.parametrize('order', ['falling', 'rising', 'mixed'])
-def test_blocks_of_very_different_size(KV8Cache, S, order):
+def test_blocks_of_very_different_size(AnyCache, S, order):
     """Values from 1e-25 to 1e10 from block to block, keys from 1e-30 to 1: the queries look at the small ones.
 
     The size of a result is sum p |v|, far below the largest value held: 2^-15 of that, and what f16 drops of p (n * 2^-33 of the
@@ -420,7 +452,7 @@ def test_blocks_of_very_different_size(KV8Cache, S, order):
             k[:, b * BLK:(b + 1) * BLK, :, 0] = -400.0       # score -50: p < 1e-20 beside the small blocks
     if order == 'mixed':
         k[:, 3 * BLK:4 * BLK] *= 1e-30
-    c = KV8Cache(1, 1, hd, n, dtype=torch.float32)
+    c = AnyCache(1, 1, hd, n, dtype=torch.float32)
     c.store(k.cuda(), v.cuda())
     got = c.attend(q.cuda(), words(n), causal=False).cpu().double()
     kh, vh = held(k[0]), held(v[0])
@@ -433,13 +465,13 @@ def test_blocks_of_very_different_size(KV8Cache, S, order):
 
 @pytest.mark.parametrize('S', [1, 60])
 @pytest.mark.parametrize('scale', [1e-30, 1e30])
-def test_tiny_and_huge_products(KV8Cache, S, scale):
+def test_tiny_and_huge_products(AnyCache, S, scale):
     """Keys and queries of 1e-30 each: every score is 0 in f32, the result the mean; values of 1e30: f32's range holds."""
     n = 300
     k, v = make(1, n, 1, 64, torch.float32, 16)
     k, v = (k * 1e-30, v) if scale < 1 else (k, v * 1e30)
     q = torch.randn(1, S, 1, 64, generator=torch.Generator().manual_seed(8)) * (1e-30 if scale < 1 else 1)
-    c = KV8Cache(1, 1, 64, n, dtype=torch.float32)
+    c = AnyCache(1, 1, 64, n, dtype=torch.float32)
     c.store(k.cuda(), v.cuda())
     for starts in (None, words(70)):
         got = c.attend(q.cuda(), words(n), causal=False, starts=starts)
@@ -448,8 +480,8 @@ def test_tiny_and_huge_products(KV8Cache, S, scale):
 
 
 @pytest.mark.parametrize('S', [1, 40])
-def test_query_strides(KV8Cache, S):
-    c, k, v = filled(KV8Cache, [100, 90], 2, 64, torch.bfloat16, 12)
+def test_query_strides(AnyCache, S):
+    c, k, v = filled(AnyCache, [100, 90], 2, 64, torch.bfloat16, 12)
     q = torch.randn(2, S, 4, 64, generator=torch.Generator().manual_seed(4)).to(torch.bfloat16).cuda()
     want = c.attend(q, words(100, 90))
     packed = torch.zeros(2, S, 4 * 64 * 3 + 1, device='cuda', dtype=torch.bfloat16)
