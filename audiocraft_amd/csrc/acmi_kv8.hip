@@ -1311,12 +1311,14 @@ static bool kv8_few(const acmi_kv8_cache* c, int S, int G) {
 }
 // Blocks per workgroup: the longest possible row in so many chunks that the call has about KV8_TARGET workgroups; one chunk (and
 // no second launch) when the tiles alone fill the chip.  The rows' lengths are not known here: shorter rows take fewer chunks of
-// the same size, so that all workgroups take equally long.
+// the same size, so that all workgroups take equally long.  A chunk is at least a block per wave, and a row of less than four per wave
+// is not split: the second launch costs 4 us.  us in a graph, unsplit or chunks of four per wave / as here: 2 rows x 16 heads of 64 x
+// 2800 tokens 14.9 / 11.6, 7 x 2 x 3700 17.6 / 11.2, 4 x 8 x 4 heads of 128 x 2000 20.4 / 14.3; 2 x 16 x 1400 unsplit 10.9, split 12.7
 static void kv8_split_plan(const acmi_kv8_cache* c, int S, int G, int* splits, int* chunk) {
     const long long tiles = (long long)c->H * ((S * G + 15) / 16) * c->rows;
     long long n = 1;
-    const int least = c->hd == 128 ? 16 : 32;   // four blocks per wave: below, the second launch costs more
-    if (tiles * 4 <= KV8_TARGET) n = max(1LL, min(min(KV8_TARGET / tiles, (long long)(c->nblk / least)), (long long)KV8_MAX_SPLITS));
+    const int least = c->hd == 128 ? 4 : 8;
+    if (tiles * 4 <= KV8_TARGET && c->nblk >= 4 * least) n = max(1LL, min(min(KV8_TARGET / tiles, (long long)(c->nblk / least)), (long long)KV8_MAX_SPLITS));
     *chunk = (int)((c->nblk + n - 1) / n);
     *splits = (c->nblk + *chunk - 1) / *chunk;
 }
