@@ -603,6 +603,52 @@ def test_another_stream(KV8Cache):
     assert torch.equal(got, want)
 
 
+def test_a_split_call_captured_and_replayed(KV8Cache):
+    """A call that needs scratch, captured; replayed at other lengths while eager calls allocate and use theirs."""
+    c, k, v = filled(KV8Cache, [9000, 5000], 2, 64, torch.float32, 60)
+    other, _, _ = filled(KV8Cache, [7000, 64], 2, 64, torch.float32, 61)
+    q = torch.randn(2, 3, 4, 64, device='cuda', generator=torch.Generator(device='cuda').manual_seed(7))
+    lens = words(9000, 5000)
+    c.attend(q, lens)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = c.attend(q, lens)
+    for a, b in ((9000, 5000), (8999, 1), (64, 4097), (0, 3000)):
+        lens.copy_(words(a, b))
+        want = c.attend(q, lens).clone()
+        g.replay()
+        other.attend(q, words(7000, 64))
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), (a, b)
+
+
+def test_two_threads_on_two_streams(KV8Cache):
+    import threading
+    made = [filled(KV8Cache, [5000, 700], 2, 64, torch.bfloat16, 70 + i) for i in range(2)]
+    qs = [torch.randn(20, 2, 4, 64, device='cuda').bfloat16() for _ in range(2)]
+    lens = words(5000, 700)
+    want = [[c.attend(q[:, None], lens).clone() for q in qq] for (c, _, _), qq in zip(made, qs)]
+    torch.cuda.synchronize()
+    got, errors = [[], []], []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                got[i] = [made[i][0].attend(q[:, None], lens) for q in qs[i]]
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:   # noqa: BLE001
+            errors.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    for g, w in zip(got, want):
+        assert len(g) == 20 and all(torch.equal(a, b) for a, b in zip(g, w))
+
+
 def test_empty_calls(KV8Cache):
     c = KV8Cache(2, 2, 64, 100)
     z = words(0, 0)
