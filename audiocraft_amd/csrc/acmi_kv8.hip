@@ -605,11 +605,14 @@ __device__ __forceinline__ void kv8_column(const Kv8AttnArgs& p, const Kv8RowInf
 #pragma unroll
     for (int k = 0; k < Kv8Geo<HD>::NK; ++k)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float y = amax == INFINITY ? 0.f : x[k][j] * down;
-            const _Float16 h = (_Float16)y;
-            c.qh[k][j] = h;
-            if constexpr (QHL) c.ql[k][j] = (_Float16)(y - (float)h);
+        for (int j = 0; j < 8; j += 2) {
+            const float y0 = amax == INFINITY ? 0.f : x[k][j] * down, y1 = amax == INFINITY ? 0.f : x[k][j + 1] * down;
+            const f16x2 h = kv8_pk(y0, y1);
+            c.qh[k][j] = h[0]; c.qh[k][j + 1] = h[1];
+            if constexpr (QHL) {
+                const f16x2 l = kv8_pk(y0 - (float)h[0], y1 - (float)h[1]);
+                c.ql[k][j] = l[0]; c.ql[k][j + 1] = l[1];
+            }
         }
 }
 
@@ -997,7 +1000,7 @@ __global__ __launch_bounds__(256) void kv8_attn_join_kernel(const Kv8AttnArgs p)
 // the next block's codes to f16 fragments in LDS while this block is multiplied (two buffers, one barrier per block).  The tail
 // is staged the same way, relative to a power of two, as f16 (bf16 tails: exact down to 2^-30 of the largest) or a pair of f16.
 // Bound by vector issue beside the matrix cores: causal over 4096 tokens, 4 x 16 heads of 64, 571 TFLOP/s (f32 403).  Short calls
-// are latencies one after another: 16 x 32 heads x 251 queries over 0 .. 77 states 21 us, of which the tail's staging is 7.
+// are latencies one after another: 16 x 32 heads x 251 queries over 0 .. 77 states 20 us, of which the tail's staging is 6.
 // All workgroups of a (row, cache head) run on one XCD (workgroup i on XCD i % 8), whose L2 then holds its codes; the last (causal:
 // longest) tiles of all pairs go first, the short ones fill the end.
 template <int HD> struct Kv8ManyLds {
@@ -1098,15 +1101,14 @@ __global__ __launch_bounds__(256, (kv8_many_wpe<HD, QB>())) void kv8_attn_many_k
         };
         if (tb) from(reinterpret_cast<const bf16_t*>(p.c.k_tail) + base, reinterpret_cast<const bf16_t*>(p.c.v_tail) + base);
         else from(reinterpret_cast<const float*>(p.c.k_tail) + base, reinterpret_cast<const float*>(p.c.v_tail) + base);
+        float odd = 0.f;   // NaN as soon as a value is not finite
 #pragma unroll
         for (int k = 0; k < NK; ++k)
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                float v = tk < nt ? kx[k][j] : 0.f;
-                const float a = fabsf(v);
-                if (!(a <= 3.4028234663852886e38f)) { kb = true; v = 0.f; }
-                kx[k][j] = v;
-                ka = fmaxf(ka, fabsf(v));
+                kx[k][j] = tk < nt ? kx[k][j] : 0.f;
+                ka = fmaxf(ka, fabsf(kx[k][j]));
+                odd = fmaf(kx[k][j], 0.f, odd);
             }
 #pragma unroll
         for (int u = 0; u < UN; ++u) {
@@ -1115,12 +1117,31 @@ __global__ __launch_bounds__(256, (kv8_many_wpe<HD, QB>())) void kv8_attn_many_k
             for (int r = 0; r < 4; ++r)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    float v = t4 + r < nt ? vx[u][r][e] : 0.f;
-                    const float a = fabsf(v);
-                    if (!(a <= 3.4028234663852886e38f)) { vb |= 1ull << (t4 + r); v = 0.f; }
-                    vx[u][r][e] = v;
-                    va = fmaxf(va, fabsf(v));
+                    vx[u][r][e] = t4 + r < nt ? vx[u][r][e] : 0.f;
+                    va = fmaxf(va, fabsf(vx[u][r][e]));
+                    odd = fmaf(vx[u][r][e], 0.f, odd);
                 }
+        }
+        if (__any(odd != 0.f)) {   // those values are left out here, their tokens noted
+            ka = va = 0.f;
+#pragma unroll
+            for (int k = 0; k < NK; ++k)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    if (!(fabsf(kx[k][j]) <= 3.4028234663852886e38f)) { kb = true; kx[k][j] = 0.f; }
+                    ka = fmaxf(ka, fabsf(kx[k][j]));
+                }
+#pragma unroll
+            for (int u = 0; u < UN; ++u) {
+                const int t4 = min(u * 256 + (int)threadIdx.x, HD * 4 - 1) / (HD / 4) * 4;
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        if (!(fabsf(vx[u][r][e]) <= 3.4028234663852886e38f)) { vb |= 1ull << (t4 + r); vx[u][r][e] = 0.f; }
+                        va = fmaxf(va, fabsf(vx[u][r][e]));
+                    }
+            }
         }
         ka = wave_max(ka);
         va = wave_max(va);
@@ -1135,7 +1156,11 @@ __global__ __launch_bounds__(256, (kv8_many_wpe<HD, QB>())) void kv8_attn_many_k
         for (int k = 0; k < NK; ++k) {
             f16x8 h;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) { kx[k][j] *= ku; h[j] = (_Float16)kx[k][j]; }
+            for (int j = 0; j < 8; j += 2) {
+                kx[k][j] *= ku; kx[k][j + 1] *= ku;
+                const f16x2 y = kv8_pk(kx[k][j], kx[k][j + 1]);
+                h[j] = y[0]; h[j + 1] = y[1];
+            }
             sm.k[0][wave * NK + k][lane] = h;
             if (!tb) {
                 f16x8 l;
@@ -1153,7 +1178,11 @@ __global__ __launch_bounds__(256, (kv8_many_wpe<HD, QB>())) void kv8_attn_many_k
                     const int at = (f >> 4) * 2 + (t4 >> 3), ln = (t4 & 3) * 16 + (f & 15) + e, half = (t4 >> 2) & 1;
                     f16x4 h;
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) { vx[u][r][e] *= vu; h[r] = (_Float16)vx[u][r][e]; }
+                    for (int r = 0; r < 4; r += 2) {
+                        vx[u][r][e] *= vu; vx[u][r + 1][e] *= vu;
+                        const f16x2 y = kv8_pk(vx[u][r][e], vx[u][r + 1][e]);
+                        h[r] = y[0]; h[r + 1] = y[1];
+                    }
                     reinterpret_cast<f16x4*>(&sm.v[0][at][ln])[half] = h;
                     if (!tb) {
                         f16x4 l;
