@@ -10,17 +10,21 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 // =====================================================================================================
 // rows -> int8 fragments + a scale each
 // =====================================================================================================
-struct RowSrc { const void* x; long long ldx; int bf16, vec, R, K; };   // vec: rows start on 4-element boundaries
+struct RowSrc { const void* x; long long ldx; int bf16, R, K; };
+// 4 elements of a row that starts anywhere: global loads need no more than the element's alignment (loaded one by one where a row
+// does not start on 4 elements: 9187 x 4065 bf16 67 us, now 32; 9600 x 1535 21 and 14, as aligned ones)
+typedef uint32_t row_u32x2 __attribute__((ext_vector_type(2), aligned(2)));
+typedef float row_f32x4 __attribute__((ext_vector_type(4), aligned(4)));
 
 // columns [col, col + 4) of a row; 0 past K
 __device__ __forceinline__ f32x4 row_ld4(const RowSrc& s, size_t base, int col) {
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    if (s.vec && col + 4 <= s.K) {
+    if (col + 4 <= s.K) {
         if (s.bf16) {
-            const uint2 w = *reinterpret_cast<const uint2*>(reinterpret_cast<const bf16_t*>(s.x) + base + col);
-            v = f32x4{__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u)};
+            const row_u32x2 w = *reinterpret_cast<const row_u32x2*>(reinterpret_cast<const bf16_t*>(s.x) + base + col);
+            v = f32x4{__uint_as_float(w[0] << 16), __uint_as_float(w[0] & 0xffff0000u), __uint_as_float(w[1] << 16), __uint_as_float(w[1] & 0xffff0000u)};
         } else {
-            v = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(s.x) + base + col);
+            v = *reinterpret_cast<const row_f32x4*>(reinterpret_cast<const float*>(s.x) + base + col);
         }
         return v;
     }
@@ -144,8 +148,7 @@ __global__ __launch_bounds__(512) void quant_row_wide_kernel(const QuantRowsArgs
 }
 
 static RowSrc row_src(const void* x, int dtype, long long ldx, int R, int K) {
-    const int bf16 = dtype == ACMI_BF16;
-    return RowSrc{x, ldx, bf16, (reinterpret_cast<size_t>(x) & (bf16 ? 7 : 15)) == 0 && ldx % 4 == 0, R, K};
+    return RowSrc{x, ldx, dtype == ACMI_BF16, R, K};
 }
 static int launch_quant_rows(const RowSrc& s, uint8_t* codes, float* scale, hipStream_t st) {
     QuantRowsArgs a = {s, (s.K + 63) / 64, 0, codes, scale};
@@ -344,10 +347,14 @@ extern "C" int acmi_linear_i8(const acmi_linear_i8_desc* desc, void* stream) {
         if (int rc = launch_quant_rows(a.s, codes, scale, st)) return rc;
         a.a = reinterpret_cast<const u32x4*>(codes); a.a_scale = scale;
     }
-    // the tiled form once its 128 x 128 tiles give 3 of 8 CUs one; below, 64-row groups of the streaming form.  Measured without
-    // the quantiser, us tiled / streamed: 256 x 4608 x 1536 (72 tiles) 12.3 / 12.0, 1000 x 1000 x 1000 (64) 10.5 / 9.0;
-    // 1024 x 1536 x 6144 (96) 27.2 / 43.8, 512 x 4096 x 1024 (128) 10.5 / 15.9, 600 x 6144 x 1536 (240) 13.2 / 35.3
-    if (((d.M + 127) / 128) * ((d.N + 127) / 128) >= 96) {
+    // the tiled form once its 128 x 128 tiles give 3 of 8 CUs one; below, 64-row groups of the streaming form -- unless the
+    // activation is larger than the L2s, from which the streaming form reads it once per 16 columns.  Measured without the
+    // quantiser, us tiled / streamed: 256 x 4608 x 1536 (72 tiles) 12.3 / 12.0, 1000 x 1000 x 1000 (64) 10.5 / 9.0;
+    // 1024 x 1536 x 6144 (96) 27.2 / 43.8, 512 x 4096 x 1024 (128) 10.5 / 15.9, 600 x 6144 x 1536 (240) 13.2 / 35.3; large
+    // activations: 9187 x 117 x 4065 (72) 23.6 / 44.0, 9600 x 100 x 1536 (75) 11.9 / 21.8, 4800 x 100 x 3000 (38) 16.7 / 20.1, but
+    // 2000 x 100 x 8000 (16) 31.6 / 21.5, 9600 x 30 x 4096 (75, of two column groups) 23.1 / 15.5
+    const long long tiles = (long long)((d.M + 127) / 128) * ((d.N + 127) / 128);
+    if (tiles >= 96 || (tiles >= 32 && d.N > 64 && (long long)d.M * d.K >= 1 << 23)) {
         BigArgs b = {};
         b.a = a.a; b.w = d.w; b.bias = d.bias; b.M = mt * 16; b.N = d.N; b.K = d.K; b.act = d.act;
         b.a_scale = a.a_scale; b.w_scale = d.w_scale; b.residual = d.residual; b.rows = d.M;

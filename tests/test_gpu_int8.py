@@ -74,7 +74,7 @@ def test_linear(Int8Linear, dt, act, M, N, K):
     check(Int8Linear(w.cuda(), bias.cuda(), act), x, w, bias, act)
 
 
-@pytest.mark.parametrize('M,N,K', [(600, 20, 2500), (2049, 18, 2112), (520, 33, 8200), (2060, 17, 9000)])
+@pytest.mark.parametrize('M,N,K', [(600, 20, 2500), (2049, 18, 2112), (520, 33, 8200), (2060, 17, 9000), (4100, 70, 2050)])
 def test_long_rows(Int8Linear, M, N, K):
     """Rows longer than a wave or a workgroup keeps in registers, either way of quantising them."""
     x, w, bias = make(M, N, K, torch.float32, 6)
