@@ -61,7 +61,7 @@ struct QuantRowsArgs { RowSrc s; int nkc, kchunk; uint8_t* codes; float* scale; 
 // One workgroup per 16 rows, a wave per row: the row is read once (NV x 256 columns of it stay in registers, longer ones are read
 // again from L2), its codes are laid down in LDS, and the 16 rows leave as whole fragments, 1 KB at a time.  (One workgroup per row
 // wrote 16-byte pieces 256 bytes apart: 38 us for 9600 x 1536 f32, now 13.2: 74 MB at 5.6 TB/s, part of it out of the last-level
-// cache.)  9600 x 6144 f32, of whose rows two thirds are read twice: 79 us.
+// cache.)  9600 x 6144 f32, of whose rows a third is read twice: 65 us.
 template <int NV>
 __global__ __launch_bounds__(1024) void quant_rows_kernel(const QuantRowsArgs p) {
     extern __shared__ __attribute__((aligned(16))) unsigned char sm[];   // [16][kchunk + 16]
@@ -162,9 +162,13 @@ static int launch_quant_rows(const RowSrc& s, uint8_t* codes, float* scale, hipS
     }
     const size_t lds = (size_t)16 * (a.kchunk + 16);
     static const bool ok = hipFuncSetAttribute(reinterpret_cast<const void*>(&quant_rows_kernel<8>), hipFuncAttributeMaxDynamicSharedMemorySize, 16 * (8192 + 16)) == hipSuccess &&
-                           hipFuncSetAttribute(reinterpret_cast<const void*>(&quant_rows_kernel<2>), hipFuncAttributeMaxDynamicSharedMemorySize, 16 * (8192 + 16)) == hipSuccess;
+                           hipFuncSetAttribute(reinterpret_cast<const void*>(&quant_rows_kernel<2>), hipFuncAttributeMaxDynamicSharedMemorySize, 16 * (8192 + 16)) == hipSuccess &&
+                           hipFuncSetAttribute(reinterpret_cast<const void*>(&quant_rows_kernel<16>), hipFuncAttributeMaxDynamicSharedMemorySize, 16 * (8192 + 16)) == hipSuccess;
     ACMI_REQUIRE(ok, "acmi_quantize_rows_i8: cannot set the dynamic LDS limit");
     if (s.K <= 512) hipLaunchKernelGGL(quant_rows_kernel<2>, dim3((s.R + 15) / 16), dim3(1024), lds, st, a);
+    // (16 x 256 columns in registers halve the workgroups per CU; us 8 x 256 / 16 x 256: 9600 x 6144 f32 77 / 65, bf16 62 / 53, 4096 x 8000
+    // bf16 31 / 28; 8192 x 4096 bf16 21.5 / 26, 9600 x 2100 16.3 / 25.9)
+    else if (s.K > 4096) hipLaunchKernelGGL(quant_rows_kernel<16>, dim3((s.R + 15) / 16), dim3(1024), lds, st, a);
     else hipLaunchKernelGGL(quant_rows_kernel<8>, dim3((s.R + 15) / 16), dim3(1024), lds, st, a);
     return acmi_check_launch("quant_rows_kernel");
 }
