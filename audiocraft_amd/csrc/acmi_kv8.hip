@@ -360,6 +360,10 @@ __device__ __forceinline__ u32x4 kv8_fetch_v(const uint8_t* vb, int i, int nl, i
 // more than 2^7, so p <= 2^15 stays in f16's range and the sums are rescaled in the first block and almost never after.  f16
 // resolves them down to 2^-32 of the maximum.
 constexpr float KV8_PSHIFT = 8.f, KV8_LAG = 7.f;
+// The unit of o goes down as well, where a block's value scale lies more than 2^10 below it: relative to it the block's probabilities
+// would sink among the f16 subnormals (at 2^-10 the largest is 2^-2, a step 2^-24).  A unit is set by a scale, which tokens that are
+// not seen or have no weight may have made large, so it says little about what o holds; o is f32 and may grow to 2^110.
+constexpr float KV8_SINK = -10.f;
 
 // one column tile's state: lane (kg, n) belongs to column n
 template <int HD, bool QHL> struct Kv8Col {
@@ -445,16 +449,27 @@ __device__ __forceinline__ void kv8_block(Kv8Col<HD, QHL> (&c)[QB], const FK& K,
         const float alpha = __builtin_amdgcn_exp2f(c[g].m - m_use);
         // the numbers that multiply the values: p 2^d, d = the block's value scale against what o is counted in, so that neither
         // large values with small p nor small ones with large p leave f16's range
-        const float w_old = top > c[g].m + KV8_LAG ? c[g].w - (m_new - c[g].m) : c[g].w, here = top - m_use + lv;
-        const float w_new = here > w_old + KV8_LAG ? here : w_old;
+        const float w_old = top > c[g].m + KV8_LAG ? c[g].w - (m_new - c[g].m) : c[g].w;
+        const float here = top - m_use + lv;
+        float w_new = here > w_old + KV8_LAG ? here : w_old;
+        const bool sink = lv < w_old + KV8_SINK;
+        if (__any(sink)) {
+            float omax = 0.f;
+#pragma unroll
+            for (int i = 0; i < ND; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) omax = fmaxf(omax, fabsf(c[g].o[i][r]) < INFINITY ? fabsf(c[g].o[i][r]) : 0.f);
+            omax = kv8_xmax(omax);
+            const float room = omax > 0.f ? fminf(110.f - (float)ilogbf(omax), 120.f) : 120.f;
+            if (sink) w_new = fmaxf(here, w_old - room);
+        }
         const float w_use = w_new == -INFINITY ? lv : w_new;
-        shrink[g] = __builtin_amdgcn_exp2f(w_old - w_use);
-        moved |= w_new > w_old;
+        shrink[g] = w_old - w_use;
+        moved |= w_new != w_old;
         c[g].m = m_new;
         c[g].w = w_new;
-        const float d = fmaxf(lv - w_use, -100.f);   // (so far below: nothing in o, but still itself in the sum l)
-        const float ie = d > 100.f ? 0.f : __builtin_amdgcn_exp2f(-d);
-        const bool plain = fabsf(d) <= 4.f;   // else f16 would not hold p 2^d as exactly as p: the sum is taken in f32 then
+        const float d = fmaxf(lv - w_use, -100.f);
+        const float ie = __builtin_amdgcn_exp2f(-d);
         float base = d + KV8_PSHIFT - m_use, f2 = f;
         if (__any(fabsf(m_use) > 1024.f)) {
             // large scores: the multiply-add below subtracts the ROUNDED maximum from the exact product (and the shift drowns in it);
@@ -484,7 +499,7 @@ __device__ __forceinline__ void kv8_block(Kv8Col<HD, QHL> (&c)[QB], const FK& K,
             }
         // the row sums: every row of (ones) P is the sum over the block's tokens
         float sum;
-        if (__all(plain)) {
+        if (!__any(d < KV8_SINK)) {   // (further down than o goes: nothing beside what it holds, but still itself in the sum l)
             const _Float16 o1 = (_Float16)1.f;
             const f16x8 ones = {o1, o1, o1, o1, o1, o1, o1, o1};
             f32x4 t = kv8_mma(ones, ph[g][1], kv8_mma(ones, ph[g][0], zero));
@@ -502,11 +517,15 @@ __device__ __forceinline__ void kv8_block(Kv8Col<HD, QHL> (&c)[QB], const FK& K,
     }
     if (__any(moved)) {
 #pragma unroll
-        for (int g = 0; g < QB; ++g)
+        for (int g = 0; g < QB; ++g) {
+            // in two steps where one factor would leave f32 (o itself, near 2^15, does not: it may have to come back)
+            const bool far = shrink[g] < -100.f;
+            const float f0 = __builtin_amdgcn_exp2f(far ? 0.5f * shrink[g] : shrink[g]), f1 = far ? f0 : 1.f;
 #pragma unroll
             for (int i = 0; i < ND; ++i)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) c[g].o[i][r] *= shrink[g];
+                for (int r = 0; r < 4; ++r) c[g].o[i][r] = c[g].o[i][r] * f0 * f1;
+        }
     }
 #pragma unroll
     for (int i = 0; i < ND; ++i)

@@ -1,0 +1,105 @@
+"""-m gpu: the 8-bit cache's attention where the numbers it holds differ in size: what a query does not see, or gives no weight
+to, leaves its result alone however large it is.
+
+Every result is held to its own size, sum p |v| over what the query sees (the definition in 64 bits, test_gpu_kv8.held): scores
+carry 2^-17 and probabilities 2^-22 (f32 results) or 2^-12 (bf16) of relative error, sums are f32: 2^-15 sum p |v| in f32,
+2^-11 sum p |v| + 2^-8 |result| in bf16 (the last its one rounding).  Not seen means no term at all; a token seen with a
+probability of e^-100 adds its p |v| < 1e-4 of the rest.
+"""
+import math
+
+import pytest
+import torch
+
+from test_gpu_kv8 import AnyCache, BLK, DT, KV8Cache, held, make, words   # noqa: F401  (fixtures)
+
+pytestmark = pytest.mark.gpu
+
+
+def expect(q, k, v, lo, hi):
+    """q [S, H, hd], k / v [n, H, hd] f64; query i sees [lo[i], hi[i]) -> result, sum p |v|."""
+    t = torch.arange(k.shape[0])
+    seen = (t[None] >= torch.tensor(lo)[:, None]) & (t[None] < torch.tensor(hi)[:, None])
+    s = torch.einsum('shd,thd->hst', q.double(), k) / math.sqrt(q.shape[-1])
+    p = torch.softmax(s.masked_fill(~seen, -math.inf), -1).nan_to_num(0.0)
+    return torch.einsum('hst,thd->shd', p, v), torch.einsum('hst,thd->shd', p, v.abs())
+
+
+def close(got, ref, size, dt):
+    bound = 2.0 ** -15 * size if dt == torch.float32 else 2.0 ** -11 * size + 2.0 ** -8 * ref.abs()
+    err = (got.cpu().double() - ref).abs()
+    assert torch.isfinite(got).all()
+    assert (err <= bound).all(), (err / bound.clamp_min(1e-300)).max().item()
+
+
+@pytest.mark.parametrize('R', [1e8, 1e12, 3e38])
+@pytest.mark.parametrize('what', ['v', 'k'])
+@pytest.mark.parametrize('place', ['block before starts', 'block before the window'])
+@pytest.mark.parametrize('dt,S,hd', [('f32', 2, 64), ('f32', 100, 64), ('bf16', 100, 64), ('f32', 70, 128), ('bf16', 20, 16)])
+def test_large_and_not_seen(AnyCache, dt, S, hd, place, what, R):
+    dt, n, H = DT[dt], 150, 2
+    start, past, S = 0, 0, (min(S, 12) if place == 'tail before starts' else S)
+    k, v = make(1, n, H, hd, dt, 6)
+    x = v if what == 'v' else k
+    first = n - S                                    # position of query 0
+    if place == 'newest':
+        large = range(n - 1, n)                      # every query but the last is before it
+    elif place == 'tail before starts':
+        start, large = 133, range(129, 133)
+    elif place == 'block before starts':
+        start, large = 30, range(5, 30)
+    else:
+        past = 30
+        large = range(first - past - 10 if first - past - 10 > 0 else 0, max(first - past, 1))
+    sign = torch.where(torch.rand(x[:, large].shape, generator=torch.Generator().manual_seed(1)) < 0.5, -1.0, 1.0)
+    x[:, large] = (R * sign).to(dt)
+    q = torch.randn(1, S, H, hd, generator=torch.Generator().manual_seed(2)).to(dt)
+    c = AnyCache(1, H, hd, 256, dtype=dt)
+    c.store(k.cuda(), v.cuda(), words(0))
+    got = c.attend(q.cuda(), words(n), past_context=past, starts=words(start))
+    kh, vh = held(k[0].float()), held(v[0].float())
+    pos = [first + i for i in range(S)]
+    lo = [max(start, p - past if past else 0) for p in pos]
+    live = [i for i, p in enumerate(pos) if not any(lo[i] <= t <= p for t in large)]
+    assert len(live) >= max(S - 1, 1)
+    ref, size = expect(q[0, live], kh, vh, [lo[i] for i in live], [pos[i] + 1 for i in live])
+    close(got[0, live], ref, size, dt)
+
+
+@pytest.mark.parametrize('R', [1e9, 1e12, 1e30])
+@pytest.mark.parametrize('at', ['first block', 'last block'])
+@pytest.mark.parametrize('dt,S,hd', [('f32', 1, 64), ('f32', 90, 64), ('bf16', 90, 64), ('f32', 1, 128), ('bf16', 1, 32)])
+def test_large_without_weight(AnyCache, dt, S, hd, at, R):
+    """A large value whose key puts its score at -100."""
+    dt, n, H = DT[dt], 64 * 5 + 40, 1
+    k, v = make(1, n, H, hd, dt, 8)
+    t = {'tail': n - 3, 'first block': 10, 'last block': 64 * 4 + 5}[at]
+    q = torch.randn(1, S, H, hd, generator=torch.Generator().manual_seed(3)).to(dt)
+    q[..., 0] = 1.0
+    k[:, t] = 0
+    k[:, t, :, 0] = -100 * math.sqrt(hd)
+    v[:, t] = torch.where(v[:, t] < 0, -R, R).to(dt)
+    c = AnyCache(1, H, hd, 512, dtype=dt)
+    c.store(k.cuda(), v.cuda(), words(0))
+    got = c.attend(q.cuda(), words(n), causal=False)
+    ref, size = expect(q[0], held(k[0].float()), held(v[0].float()), [0] * S, [n] * S)
+    close(got[0], ref, size, dt)
+
+
+@pytest.mark.parametrize('S', [1, 90])
+@pytest.mark.parametrize('sizes', [[1e30, 1e-8, 1e30, 1e-30, 1.0], [1e-30, 1e30, 1e-30, 1e30, 1e-30], [1e5, 1.0, 1e-5, 1e5, 1.0], [1e-20, 1.0, 1e20, 1.0, 1e-20]])
+@pytest.mark.parametrize('dt', ['f32', 'bf16'])
+def test_blocks_of_other_sizes_keep_their_weight(AnyCache, dt, S, sizes):
+    """Blocks whose values are far apart in size, equal in weight: the small ones add next to nothing to the result and their whole
+    share to the sum that divides it."""
+    dt, n, hd = DT[dt], 64 * 4 + 20, 64
+    k, v = make(1, n, 1, hd, dt, 12)
+    for b, size in enumerate(sizes):
+        v[:, b * BLK:(b + 1) * BLK] *= size
+    q = torch.randn(1, S, 1, hd, generator=torch.Generator().manual_seed(10)).to(dt)
+    c = AnyCache(1, 1, hd, 512, dtype=dt)
+    c.store(k.cuda(), v.cuda(), words(0))
+    for starts in (0, 64, 128):
+        got = c.attend(q.cuda(), words(n), causal=False, starts=words(starts))
+        ref, size = expect(q[0], held(k[0].float()), held(v[0].float()), [starts] * S, [n] * S)
+        close(got[0], ref, size, dt)
