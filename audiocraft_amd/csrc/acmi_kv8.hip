@@ -770,7 +770,7 @@ __device__ __forceinline__ void kv8_tail16(const Kv8AttnArgs& p, const Kv8RowInf
 #pragma unroll
         for (int j = 0; j < 8; ++j) s = __builtin_amdgcn_mfma_f32_16x16x4f32(HD == 16 && kg >= 2 ? 0.f : kx[k][j], x[k][j], s, 0, 0, 0);
     const float f = p.scale * 1.4426950408889634f;
-    float cmax = -INFINITY, vmax = 0.f;
+    float cmax = -INFINITY;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
         const int t = t0 + kg * 4 + r;
@@ -786,6 +786,7 @@ __device__ __forceinline__ void kv8_tail16(const Kv8AttnArgs& p, const Kv8RowInf
     sum += __shfl_xor(sum, 16, 64);
     sum += __shfl_xor(sum, 32, 64);
     c.l = sum;
+    float omax = 0.f;
     bool bad = false;   // a NaN or an infinity among the values: it must not meet the probability 0 of a column that does not see it
 #pragma unroll
     for (int i = 0; i < ND; ++i) {
@@ -795,11 +796,21 @@ __device__ __forceinline__ void kv8_tail16(const Kv8AttnArgs& p, const Kv8RowInf
             const float a = fabsf(vx[i][r]);
             const bool fin = a <= 3.4028234663852886e38f;
             bad |= !fin;
-            vmax = fmaxf(vmax, fin ? a : 0.f);
-            t = __builtin_amdgcn_mfma_f32_16x16x4f32(fin ? vx[i][r] : 0.f, s[r], t, 0, 0, 0);
+            t = __builtin_amdgcn_mfma_f32_16x16x4f32(fin ? vx[i][r] : 0.f, s[r] * 0x1p-12f, t, 0, 0, 0);   // p / 16: at most the largest value
         }
         c.o[i] = t;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) omax = fmaxf(omax, fabsf(t[r]));
     }
+    // o's unit is what the column holds, whatever there is that it does not see: a power of two that brings its largest feature to
+    // [2^14, 2^15), where p = 1 of a block's largest code stands
+    omax = kv8_xmax(omax);
+    const int e = max(omax > 0.f ? ilogbf(omax) : -118, -118);
+    c.w = c.m == -INFINITY ? -INFINITY : (float)(e - 2);
+#pragma unroll
+    for (int i = 0; i < ND; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) c.o[i][r] = ldexpf(c.o[i][r], 14 - e);
     if (__any(bad)) {   // those values one by one, each column for itself
         for (int tok = 0; tok < 16; ++tok) {
             float pr = 0.f;
@@ -820,13 +831,6 @@ __device__ __forceinline__ void kv8_tail16(const Kv8AttnArgs& p, const Kv8RowInf
                 }
         }
     }
-    // in units of a scale like the blocks': largest value / 127
-    const float unit = fmaxf(wave_max(vmax) * (1.f / 127.f), 7.52316384526264e-37f), iu = 1.f / unit;
-    c.w = c.m == -INFINITY ? -INFINITY : __builtin_amdgcn_logf(unit);
-#pragma unroll
-    for (int i = 0; i < ND; ++i)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) c.o[i][r] *= iu;
 }
 
 // The leading arguments are what the first requests need -- query, length word, tail -- and arrive in scalar registers at wave

@@ -86,6 +86,37 @@ def test_large_without_weight(AnyCache, dt, S, hd, at, R):
     close(got[0], ref, size, dt)
 
 
+@pytest.mark.parametrize('dt', ['f32', 'bf16'])
+@pytest.mark.parametrize('n', [100, 700])
+def test_decode_with_a_large_value_in_the_tail(KV8Cache, dt, n):
+    """The new token itself and one in the newest block, both at a score of -100."""
+    dt, hd, H, G = DT[dt], 64, 2, 2
+    k, v = make(2, n + 1, H, hd, dt, 9)
+    q = torch.randn(2, H * G, hd, generator=torch.Generator().manual_seed(4)).to(dt)
+    q[..., 0] = 1.0
+    for r, t in ((0, n), (1, n - 2)):
+        k[r, t] = 0
+        k[r, t, :, 0] = -800.0
+        v[r, t] = torch.where(v[r, t] < 0, -1e14, 1e14).to(dt)
+    c = KV8Cache(2, H, hd, 1024, dtype=dt)
+    c.store(k[:, :n].cuda(), v[:, :n].cuda())
+    got = c.decode(q.cuda(), k[:, n].cuda(), v[:, n].cuda(), words(n, n))
+    for r in range(2):
+        ref, size = expect(q[r][None], held(k[r].float()).repeat_interleave(G, 1), held(v[r].float()).repeat_interleave(G, 1), [0], [n + 1])
+        close(got[r][None], ref, size, dt)
+
+
+@pytest.mark.parametrize('dt', ['f32', 'bf16'])
+@pytest.mark.parametrize('hd', [16, 32, 64, 128])
+def test_a_first_token_comes_back_as_it_is(KV8Cache, dt, hd):
+    """One token, probability 1."""
+    dt = DT[dt]
+    v = (torch.randn(3, 2, hd, generator=torch.Generator().manual_seed(7)) * torch.tensor([1.0, 1e-12, 1e20])[:, None, None]).to(dt).cuda()
+    k, q = (torch.randn(3, 2, hd, generator=torch.Generator().manual_seed(8)).to(dt).cuda() for _ in range(2))
+    got = KV8Cache(3, 2, hd, 100, dtype=dt).decode(q, k, v, words(0, 0, 0))
+    assert torch.equal(got, v)
+
+
 @pytest.mark.parametrize('S', [1, 90])
 @pytest.mark.parametrize('sizes', [[1e30, 1e-8, 1e30, 1e-30, 1.0], [1e-30, 1e30, 1e-30, 1e30, 1e-30], [1e5, 1.0, 1e-5, 1e5, 1.0], [1e-20, 1.0, 1e20, 1.0, 1e-20]])
 @pytest.mark.parametrize('dt', ['f32', 'bf16'])
