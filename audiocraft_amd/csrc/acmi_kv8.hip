@@ -1021,7 +1021,8 @@ __global__ __launch_bounds__(256) void kv8_attn_join_kernel(const Kv8AttnArgs p)
 
 // ---- many queries: a workgroup's 4 waves own QB column tiles each and walk the blocks together.  Every wave converts a quarter of
 // the next block's codes to f16 fragments in LDS while this block is multiplied (two buffers, one barrier per block).  The tail
-// is staged the same way, relative to a power of two, as f16 (bf16 tails: exact down to 2^-30 of the largest) or a pair of f16.
+// is staged the same way, relative to a power of two, as f16 (bf16 tails: exact down to 2^-30 of the largest) or a pair of f16; where
+// a token's features are all below 2^-12 of the tail's largest -- which this column may not see -- it takes kv8_tail_wide instead.
 // Bound by vector issue beside the matrix cores: causal over 4096 tokens, 4 x 16 heads of 64, 571 TFLOP/s (f32 403).  Short calls
 // are latencies one after another: 16 x 32 heads x 251 queries over 0 .. 77 states 20 us, of which the tail's staging is 6.
 // All workgroups of a (row, cache head) run on one XCD (workgroup i on XCD i % 8), whose L2 then holds its codes; the last (causal:
@@ -1030,7 +1031,66 @@ template <int HD> struct Kv8ManyLds {
     f16x8 k[2][4 * Kv8Geo<HD>::NK][64], v[2][2 * Kv8Geo<HD>::ND][64];
     float red[2][4];
     unsigned long long kbad, vbad;   // tokens of the tail that hold a NaN or an infinity
+    int wide;                        // the tail's tokens differ too much in size for one unit
 };
+
+// The tail for one column tile in f32, 16 tokens at a time, straight from memory: a key or a value far larger than the rest
+// must not cost the others their precision.  Values that are not finite are left out, as in the staged form.
+template <int HD, bool QHL>
+__device__ __forceinline__ void kv8_tail_wide(const Kv8AttnArgs& p, const Kv8RowInfo& ri, int row, int kvh, int cidx, Kv8Col<HD, QHL>& c) {
+    constexpr int ND = Kv8Geo<HD>::ND;
+    const int lane = threadIdx.x & 63, nl = lane & 15, kg = lane >> 4, tb = p.c.tail_dtype == ACMI_BF16;
+    const int t0 = (ri.len - 1) / BLK * BLK;
+    const size_t base = ((size_t)row * p.c.H + kvh) * (BLK * HD), qb = kv8_query_at(p, row, kvh, min(cidx, p.S * p.G - 1));
+    const float f = c.sfac == c.sfac ? p.scale * 1.4426950408889634f : c.sfac;   // (NaN: a query that is not finite)
+#pragma unroll 1
+    for (int slot0 = 0; t0 + slot0 < ri.len; slot0 += 16) {
+        f32x4 s = {0.f, 0.f, 0.f, 0.f}, t[ND];
+#pragma unroll 1
+        for (int d = kg; d < HD; d += 4)
+            s = __builtin_amdgcn_mfma_f32_16x16x4f32(kv8_ld(p.c.k_tail, base + (size_t)(slot0 + nl) * HD + d, tb), kv8_ld(p.q, qb + d, p.q_bf16), s, 0, 0, 0);
+        float cmax = -INFINITY, sum = 0.f, omax = 0.f;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int at = t0 + slot0 + kg * 4 + r;
+            s[r] = at >= c.lo && at < c.lim && at < ri.len ? s[r] * f : -INFINITY;
+            cmax = fmaxf(cmax, s[r]);
+        }
+        cmax = kv8_xmax(cmax);
+        const float m_new = fmaxf(cmax, c.m), m_use = m_new == -INFINITY ? 0.f : m_new;
+        const float w_old = m_new > c.m ? c.w - (m_new - c.m) : c.w;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) { s[r] = __builtin_amdgcn_exp2f(s[r] - m_use + KV8_PSHIFT); sum += s[r]; }
+        sum += __shfl_xor(sum, 16, 64);
+        sum += __shfl_xor(sum, 32, 64);
+        c.l = fmaf(c.l, __builtin_amdgcn_exp2f(c.m - m_use), sum);
+        c.m = m_new;
+#pragma unroll
+        for (int i = 0; i < ND; ++i) {
+            t[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int slot = slot0 + kg * 4 + r;
+                const float v = t0 + slot < ri.len ? kv8_ld(p.c.v_tail, base + (size_t)slot * HD + i * 16 + nl, tb) : 0.f;
+                t[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(fabsf(v) <= 3.4028234663852886e38f ? v : 0.f, s[r] * 0x1p-12f, t[i], 0, 0, 0);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) omax = fmaxf(omax, fabsf(t[i][r]));
+        }
+        omax = kv8_xmax(omax);
+        // (o may stay in a unit far above what it holds: this is f32)
+        const float w_new = fmaxf(w_old, omax > 0.f ? (float)(max(ilogbf(omax), -118) - 2) : m_new == -INFINITY ? -INFINITY : -120.f);
+        const float sh = w_old == -INFINITY ? 0.f : w_old - w_new;
+        const bool far = sh < -100.f;
+        const float f0 = __builtin_amdgcn_exp2f(far ? 0.5f * sh : sh), f1 = far ? f0 : 1.f;
+        const float up = w_new == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(-w_new);
+#pragma unroll
+        for (int i = 0; i < ND; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) c.o[i][r] = fmaf(t[i][r] * up, 4096.f, c.o[i][r] * f0 * f1);
+        c.w = w_new;
+    }
+}
 
 // Waves per SIMD: what the registers allow without spilling more than a few (hd 64, two tiles: 3 55.6 us, 2 66.3, for 600 tokens x
 // 16 rows x 24 heads).
@@ -1110,7 +1170,7 @@ __global__ __launch_bounds__(256, (kv8_many_wpe<HD, QB>())) void kv8_attn_many_k
         float kx[NK][8], vx[UN][4][4], ka = 0.f, va = 0.f;
         bool kb = false;
         unsigned long long vb = 0;
-        if (threadIdx.x == 0) { sm.kbad = 0; sm.vbad = 0; }
+        if (threadIdx.x == 0) { sm.kbad = 0; sm.vbad = 0; sm.wide = 0; }
         const int tk = wave * 16 + nl;   // this lane's token of K
         auto from = [&](auto* kt, auto* vt) {   // every load of the tail in flight at once (places past the length are masked below)
 #pragma unroll
@@ -1166,7 +1226,8 @@ __global__ __launch_bounds__(256, (kv8_many_wpe<HD, QB>())) void kv8_attn_many_k
                     }
             }
         }
-        ka = wave_max(ka);
+        const float kt = kv8_xmax(ka);   // of the token
+        ka = wave_max(kt);
         va = wave_max(va);
         if (lane == 0) { sm.red[0][wave] = ka; sm.red[1][wave] = va; }
         __syncthreads();
@@ -1174,6 +1235,27 @@ __global__ __launch_bounds__(256, (kv8_many_wpe<HD, QB>())) void kv8_attn_many_k
         if (vb != 0) atomicOr(&sm.vbad, vb);
         ka = fmaxf(fmaxf(sm.red[0][0], sm.red[0][1]), fmaxf(sm.red[0][2], sm.red[0][3]));
         va = fmaxf(fmaxf(sm.red[1][0], sm.red[1][1]), fmaxf(sm.red[1][2], sm.red[1][3]));
+        bool wide = kt > 0.f && kt < ka * 0x1p-12f, few = false;
+        float vt[UN][4];
+#pragma unroll
+        for (int u = 0; u < UN; ++u)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                vt[u][r] = fmaxf(fmaxf(fabsf(vx[u][r][0]), fabsf(vx[u][r][1])), fmaxf(fabsf(vx[u][r][2]), fabsf(vx[u][r][3])));
+                few |= vt[u][r] > 0.f && vt[u][r] < va * 0x1p-12f;
+            }
+        if (__any(few)) {   // four features of a token: is it all of them (on the HD / 4 lanes next to each other)
+#pragma unroll
+            for (int u = 0; u < UN; ++u)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    float t = vt[u][r];
+#pragma unroll
+                    for (int x = 1; x < HD / 4; x <<= 1) t = fmaxf(t, __shfl_xor(t, x, 64));
+                    wide |= u * 256 + (int)threadIdx.x < HD * 4 && t > 0.f && t < va * 0x1p-12f;
+                }
+        }
+        if (wide) sm.wide = 1;
         const float ku = ldexpf(1.f, min(14 - (ka > 0.f ? ilogbf(ka) : 0), 126)), vu = ldexpf(1.f, min(14 - (va > 0.f ? ilogbf(va) : 0), 126));
 #pragma unroll
         for (int k = 0; k < NK; ++k) {
@@ -1249,7 +1331,10 @@ __global__ __launch_bounds__(256, (kv8_many_wpe<HD, QB>())) void kv8_attn_many_k
             auto V = [&](int i, int u) { return sm.v[0][i * 2 + u][lane]; };
             auto KL = [&](int tt, int k) { return sm.k[1][tt * NK + k][lane]; };
             auto VL = [&](int i, int u) { return sm.v[1][i * 2 + u][lane]; };
-            if (tb) kv8_block<HD, QHL, PHL, false, QB>(c, K, V, 0, 0, ks, vs, t0, none, fix);
+            if (sm.wide) {   // (workgroup uniform)
+#pragma unroll
+                for (int g = 0; g < QB; ++g) kv8_tail_wide<HD, QHL>(p, ri, row, kvh, c0 + g * 16 + nl, c[g]);
+            } else if (tb) kv8_block<HD, QHL, PHL, false, QB>(c, K, V, 0, 0, ks, vs, t0, none, fix);
             else kv8_block<HD, QHL, PHL, true, QB>(c, K, V, KL, VL, ks, vs, t0, none, fix);
 #pragma unroll 1
             for (int t = 0; t < (vbad != 0 ? nt : 0); ++t) {   // values that are not finite one by one, each column for itself

@@ -34,7 +34,7 @@ def close(got, ref, size, dt):
 
 @pytest.mark.parametrize('R', [1e8, 1e12, 3e38])
 @pytest.mark.parametrize('what', ['v', 'k'])
-@pytest.mark.parametrize('place', ['block before starts', 'block before the window'])
+@pytest.mark.parametrize('place', ['newest', 'tail before starts', 'block before starts', 'block before the window'])
 @pytest.mark.parametrize('dt,S,hd', [('f32', 2, 64), ('f32', 100, 64), ('bf16', 100, 64), ('f32', 70, 128), ('bf16', 20, 16)])
 def test_large_and_not_seen(AnyCache, dt, S, hd, place, what, R):
     dt, n, H = DT[dt], 150, 2
@@ -67,7 +67,7 @@ def test_large_and_not_seen(AnyCache, dt, S, hd, place, what, R):
 
 
 @pytest.mark.parametrize('R', [1e9, 1e12, 1e30])
-@pytest.mark.parametrize('at', ['first block', 'last block'])
+@pytest.mark.parametrize('at', ['tail', 'first block', 'last block'])
 @pytest.mark.parametrize('dt,S,hd', [('f32', 1, 64), ('f32', 90, 64), ('bf16', 90, 64), ('f32', 1, 128), ('bf16', 1, 32)])
 def test_large_without_weight(AnyCache, dt, S, hd, at, R):
     """A large value whose key puts its score at -100."""
@@ -117,6 +117,22 @@ def test_a_first_token_comes_back_as_it_is(KV8Cache, dt, hd):
     assert torch.equal(got, v)
 
 
+@pytest.mark.parametrize('R', [2.0 ** 8, 2.0 ** 16, 2.0 ** 40])
+@pytest.mark.parametrize('S', [1, 90])
+def test_one_large_feature(AnyCache, S, R):
+    """A value whose one feature is large and seen: the other features of the result keep their own precision."""
+    n, hd = 64 * 4 + 30, 64
+    k, v = make(1, n, 1, hd, torch.float32, 11)
+    for t in (70, n - 4):
+        v[:, t, :, 3] = R
+    q = torch.randn(1, S, 1, hd, generator=torch.Generator().manual_seed(9))
+    c = AnyCache(1, 1, hd, 512, dtype=torch.float32)
+    c.store(k.cuda(), v.cuda(), words(0))
+    got = c.attend(q.cuda(), words(n), causal=False)
+    ref, size = expect(q[0], held(k[0]), held(v[0]), [0] * S, [n] * S)
+    close(got[0], ref, size, torch.float32)
+
+
 @pytest.mark.parametrize('S', [1, 90])
 @pytest.mark.parametrize('sizes', [[1e30, 1e-8, 1e30, 1e-30, 1.0], [1e-30, 1e30, 1e-30, 1e30, 1e-30], [1e5, 1.0, 1e-5, 1e5, 1.0], [1e-20, 1.0, 1e20, 1.0, 1e-20]])
 @pytest.mark.parametrize('dt', ['f32', 'bf16'])
@@ -134,3 +150,28 @@ def test_blocks_of_other_sizes_keep_their_weight(AnyCache, dt, S, sizes):
         got = c.attend(q.cuda(), words(n), causal=False, starts=words(starts))
         ref, size = expect(q[0], held(k[0].float()), held(v[0].float()), [starts] * S, [n] * S)
         close(got[0], ref, size, dt)
+
+
+@pytest.mark.parametrize('dt,hd', [('f32', 64), ('bf16', 64), ('f32', 128), ('f32', 32)])
+def test_large_and_not_finite_together(AnyCache, dt, hd):
+    """The three newest tokens: a key of 1e10, a value of 1e12, a NaN and an infinity; the queries before them see none of it, those
+    that see the NaN give NaN, and an infinite value stays in its feature."""
+    dt, n, S, H = DT[dt], 150, 40, 2
+    k, v = make(1, n, H, hd, dt, 13)
+    k[:, 146, :, 1] = 1e10
+    v[:, 147] = 1e12
+    v[:, 148, :, 5] = math.inf
+    k[:, 149] = math.nan
+    q = torch.randn(1, S, H, hd, generator=torch.Generator().manual_seed(11)).to(dt)
+    q[..., 1] = -q[..., 1].abs()                     # the large key has no weight
+    c = AnyCache(1, H, hd, 256, dtype=dt)
+    c.store(k.cuda(), v.cuda(), words(0))
+    got = c.attend(q.cuda(), words(n)).cpu()
+    v[:, 148, :, 5] = 0
+    kh, vh = held(k[0].float()), held(v[0].float())
+    kh[149] = 0
+    hi = [n - S + i + 1 for i in range(S)]
+    ref, size = expect(q[0], kh, vh, [0] * S, hi)
+    assert got[0, S - 1].isnan().all() and (got[0, S - 2, :, 5] == math.inf).all()
+    got[0, S - 2, :, 5] = ref[S - 2, :, 5].to(dt)
+    close(got[0, :S - 1], ref[:S - 1], size[:S - 1], dt)
