@@ -365,6 +365,14 @@ constexpr float KV8_PSHIFT = 8.f, KV8_LAG = 7.f;
 // not seen or have no weight may have made large, so it says little about what o holds; o is f32 and may grow to 2^110.
 constexpr float KV8_SINK = -10.f;
 
+// 2^w = up / down: a unit near the largest number, times what a lagging maximum adds (2^7), leaves f32, and so may the quotient of an o
+// that holds next to nothing in such a unit
+struct Kv8Unit { float up, down; };
+__device__ __forceinline__ Kv8Unit kv8_unit(float w) {
+    const bool large = w > 64.f;
+    return Kv8Unit{__builtin_amdgcn_exp2f(large ? w - 32.f : w), large ? 0x1p-32f : 1.f};
+}
+
 // one column tile's state: lane (kg, n) belongs to column n
 template <int HD, bool QHL> struct Kv8Col {
     f16x8 qh[Kv8Geo<HD>::NK], ql[QHL ? Kv8Geo<HD>::NK : 1];
@@ -805,7 +813,7 @@ __device__ __forceinline__ void kv8_tail16(const Kv8AttnArgs& p, const Kv8RowInf
     // o's unit is what the column holds, whatever there is that it does not see: a power of two that brings its largest feature to
     // [2^14, 2^15), where p = 1 of a block's largest code stands
     omax = kv8_xmax(omax);
-    const int e = max(omax > 0.f ? ilogbf(omax) : -118, -118);
+    const int e = max(omax > 0.f ? ilogbf(omax) : -18, -118);
     c.w = c.m == -INFINITY ? -INFINITY : (float)(e - 2);
 #pragma unroll
     for (int i = 0; i < ND; ++i)
@@ -833,6 +841,13 @@ __device__ __forceinline__ void kv8_tail16(const Kv8AttnArgs& p, const Kv8RowInf
     }
 }
 
+// Parts of a column are joined as they are, each in its unit: p v summed in absolute numbers would pass f32 where the quotient does not.
+// dm: a part's maximum against the largest, w its unit, W the largest unit.
+struct Kv8Joint { float l, o; };
+__device__ __forceinline__ Kv8Joint kv8_joint(float dm, float w, float W) {
+    return Kv8Joint{__builtin_amdgcn_exp2f(dm), __builtin_amdgcn_exp2f(dm + w - (W == -INFINITY ? 0.f : W))};
+}
+
 // The leading arguments are what the first requests need -- query, length word, tail -- and arrive in scalar registers at wave
 // start (kernarg preload); the rest of the descriptor is fetched behind those requests.
 //   g0 = H | G << 16   g1 = column tiles | q bf16 << 16 | tail bf16 << 17 | length per row << 18   query strides in elements
@@ -842,7 +857,7 @@ __global__ __launch_bounds__(NW * 64, kv8_wpe<HD>()) void kv8_attn_split_kernel(
                                                                                 const Kv8AttnArgs p) {
     constexpr int NK = Kv8Geo<HD>::NK, ND = Kv8Geo<HD>::ND, KW = Kv8Geo<HD>::KW, PITCH = HD + 4;
     __shared__ __attribute__((aligned(16))) float sm_o[NW][16][PITCH];
-    __shared__ float sm_m[NW][16], sm_l[NW][16];
+    __shared__ float sm_m[NW][16], sm_l[NW][16], sm_w[NW][16];
     __shared__ Kv8QuantLds<HD> sm_q;
     // (chunk slowest: the workgroups that a shorter row does not need come last, and leave at once)
     const int split = blockIdx.z, row = blockIdx.y;
@@ -909,16 +924,22 @@ __global__ __launch_bounds__(NW * 64, kv8_wpe<HD>()) void kv8_attn_split_kernel(
         get_v(rq);
         b = nb;
     }
-    // relative to the wave's maximum (a column that has seen nothing has o = 0)
-    const float unit = __builtin_amdgcn_exp2f(c[0].w) * (1.f / 256.f);
+    // relative to the wave's maximum, in a unit near what the column holds (a scale may have set another: kv8_block)
+    float omax = 0.f;
+#pragma unroll
+    for (int i = 0; i < ND; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) omax = fmaxf(omax, fabsf(c[0].o[i][r]));
+    omax = kv8_xmax(omax);
+    const int up = omax > 0.f && omax < INFINITY ? max(14 - ilogbf(omax), 0) : 0;
 #pragma unroll
     for (int i = 0; i < ND; ++i) {
         f32x4 o = c[0].o[i];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) o[r] *= unit;
+        for (int r = 0; r < 4; ++r) o[r] = ldexpf(o[r], up);
         *reinterpret_cast<f32x4*>(&sm_o[wave][nl][i * 16 + kg * 4]) = o;
     }
-    if (kg == 0) { sm_m[wave][nl] = c[0].m; sm_l[wave][nl] = c[0].l * (1.f / 256.f); }
+    if (kg == 0) { sm_m[wave][nl] = c[0].m; sm_l[wave][nl] = c[0].l; sm_w[wave][nl] = omax > 0.f ? c[0].w - (float)up : -INFINITY; }
     // the row's newest token and a block it completes (column tile 0 alone)
     if (mine && qt == 0 && ri.len > 0 && (ri.fresh || p.complete)) {
         const int tb = p.c.tail_dtype == ACMI_BF16;
@@ -950,26 +971,31 @@ __global__ __launch_bounds__(NW * 64, kv8_wpe<HD>()) void kv8_attn_split_kernel(
 #pragma unroll
         for (int w = 0; w < NW; ++w) M = fmaxf(M, sm_m[w][n]);
         const float Mu = M == -INFINITY ? 0.f : M;
+        float W = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) W = fmaxf(W, sm_m[w][n] - Mu + sm_w[w][n]);
         f32x4 o = {0.f, 0.f, 0.f, 0.f};
         float den = 0.f;
 #pragma unroll
         for (int w = 0; w < NW; ++w) {
-            const float f = __builtin_amdgcn_exp2f(sm_m[w][n] - Mu);
+            const Kv8Joint j = kv8_joint(sm_m[w][n] - Mu, sm_w[w][n], W);
             const f32x4 y = *reinterpret_cast<const f32x4*>(&sm_o[w][n][d]);
-            den = fmaf(f, sm_l[w][n], den);
+            den = fmaf(j.l, sm_l[w][n], den);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) o[r] = fmaf(f, y[r], o[r]);
+            for (int r = 0; r < 4; ++r) o[r] = fmaf(j.o, y[r], o[r]);
         }
         if (sp.eff == 1) {
             const int s = kv8_query(p, cidx), g = cidx - s * p.G;
             const bool none = s >= ri.qlen || den == 0.f;
+            const Kv8Unit unit = kv8_unit(W);
+            den *= unit.down;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) o[r] = none ? 0.f : o[r] / den;
+            for (int r = 0; r < 4; ++r) o[r] = none ? 0.f : o[r] / den * unit.up;
             kv8_put4(p, row, s, kvh * p.G + g, HD, d, o);
-        } else {   // partial: [row][cache head x tile][column][split][features | max | sum]
+        } else {   // partial: [row][cache head x tile][column][split][features | max, sum, unit]
             float* w = p.work + ((((size_t)row * gridDim.x + blockIdx.x) * 16 + n) * p.splits + split) * (HD + 4);
             *reinterpret_cast<f32x4*>(w + d) = o;
-            if (d == 0) { w[HD] = M; w[HD + 1] = den; }
+            if (d == 0) { w[HD] = M; w[HD + 1] = den; w[HD + 2] = W; }
         }
     }
 }
@@ -989,18 +1015,18 @@ __global__ __launch_bounds__(256) void kv8_attn_join_kernel(const Kv8AttnArgs p)
     const float* w = p.work + (((size_t)row * gridDim.y + blockIdx.y) * 16 + n) * p.splits * (HD + 4);
     const int f4 = threadIdx.x % F4, grp = threadIdx.x / F4;
     const int lane = threadIdx.x & 63;
-    const float M = wave_max(lane < sp.eff ? w[(size_t)lane * (HD + 4) + HD] : -INFINITY);   // (KV8_MAX_SPLITS = 64)
-    const float Mu = M == -INFINITY ? 0.f : M;
+    const f32x4 mine = lane < sp.eff ? *reinterpret_cast<const f32x4*>(w + (size_t)lane * (HD + 4) + HD) : f32x4{-INFINITY, 0.f, -INFINITY, 0.f};   // (KV8_MAX_SPLITS = 64)
+    const float M = wave_max(mine[0]), Mu = M == -INFINITY ? 0.f : M, W = wave_max(mine[0] - Mu + mine[2]);
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
     float den = 0.f;
 #pragma unroll 4
     for (int k = grp; k < sp.eff; k += NG) {
         const float* y = w + (size_t)k * (HD + 4);
-        const float f = __builtin_amdgcn_exp2f(y[HD] - Mu);
+        const Kv8Joint j = kv8_joint(y[HD] - Mu, y[HD + 2], W);
         const f32x4 v = *reinterpret_cast<const f32x4*>(y + f4 * 4);
-        den = fmaf(f, y[HD + 1], den);
+        den = fmaf(j.l, y[HD + 1], den);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) o[r] = fmaf(f, v[r], o[r]);
+        for (int r = 0; r < 4; ++r) o[r] = fmaf(j.o, v[r], o[r]);
     }
     so[grp][f4] = o;
     if (f4 == 0) sd[grp] = den;
@@ -1014,8 +1040,10 @@ __global__ __launch_bounds__(256) void kv8_attn_join_kernel(const Kv8AttnArgs p)
     }
     const int s = kv8_query(p, cidx), g = cidx - s * p.G;
     const bool none = s >= ri.qlen || den == 0.f;
+    const Kv8Unit unit = kv8_unit(W);
+    den *= unit.down;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) o[r] = none ? 0.f : o[r] / den;
+    for (int r = 0; r < 4; ++r) o[r] = none ? 0.f : o[r] / den * unit.up;
     kv8_put4(p, row, s, kvh * p.G + g, HD, f4 * 4, o);
 }
 
@@ -1359,12 +1387,13 @@ __global__ __launch_bounds__(256, (kv8_many_wpe<HD, QB>())) void kv8_attn_many_k
         const int cidx = c0 + g * 16 + nl, s = kv8_query(p, cidx), h = cidx - s * p.G;
         if (cidx >= cols) continue;
         const bool zero = s >= ri.qlen || c[g].l == 0.f;
-        const float inv = 1.f / c[g].l, unit = __builtin_amdgcn_exp2f(c[g].w);
+        const Kv8Unit unit = kv8_unit(c[g].w);
+        const float inv = 1.f / (c[g].l * unit.down);
 #pragma unroll
         for (int i = 0; i < ND; ++i) {
             f32x4 o;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) o[r] = zero ? 0.f : c[g].o[i][r] * inv * unit;
+            for (int r = 0; r < 4; ++r) o[r] = zero ? 0.f : c[g].o[i][r] * inv * unit.up;
             kv8_put4(p, row, s, kvh * p.G + h, HD, i * 16 + kg * 4, o);
         }
     }

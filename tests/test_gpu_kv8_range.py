@@ -106,6 +106,21 @@ def test_decode_with_a_large_value_in_the_tail(KV8Cache, dt, n):
         close(got[r][None], ref, size, dt)
 
 
+@pytest.mark.parametrize('S', [1, 100])
+@pytest.mark.parametrize('n', [1, 30, 64, 200, 6000])
+def test_values_near_the_largest_number(AnyCache, S, n):
+    """3e38 of one sign: the sum of probabilities times values passes what f32 holds, the result does not."""
+    k, v = make(1, n, 1, 64, torch.float32, 10)
+    k = k * 0.1
+    v = 1e38 + 2e38 * torch.rand(v.shape, generator=torch.Generator().manual_seed(5))
+    q = torch.randn(1, S, 1, 64, generator=torch.Generator().manual_seed(6))
+    c = AnyCache(1, 1, 64, n, dtype=torch.float32)
+    c.store(k.cuda(), v.cuda(), words(0))
+    got = c.attend(q.cuda(), words(n), causal=False)
+    ref, size = expect(q[0], held(k[0]), held(v[0]), [0] * S, [n] * S)
+    close(got[0], ref, size, torch.float32)
+
+
 @pytest.mark.parametrize('dt', ['f32', 'bf16'])
 @pytest.mark.parametrize('hd', [16, 32, 64, 128])
 def test_a_first_token_comes_back_as_it_is(KV8Cache, dt, hd):
@@ -175,3 +190,19 @@ def test_large_and_not_finite_together(AnyCache, dt, hd):
     assert got[0, S - 1].isnan().all() and (got[0, S - 2, :, 5] == math.inf).all()
     got[0, S - 2, :, 5] = ref[S - 2, :, 5].to(dt)
     close(got[0, :S - 1], ref[:S - 1], size[:S - 1], dt)
+
+
+@pytest.mark.parametrize('R', [1e8, 1e20, 3e38])
+@pytest.mark.parametrize('dt,hd', [('f32', 64), ('bf16', 64), ('bf16', 128)])
+def test_large_and_later_in_a_block(AnyCache, dt, hd, R):
+    """Queries in the middle of the second block, whose last tokens, which they do not see, set its scales."""
+    dt, n, S, H = DT[dt], 300, 230, 1
+    k, v = make(1, n, H, hd, dt, 14)
+    v[:, 120:124] = torch.where(v[:, 120:124] < 0, -R, R).to(dt)
+    k[:, 124:126] = torch.where(k[:, 124:126] < 0, -R, R).to(dt)
+    q = torch.randn(1, S, H, hd, generator=torch.Generator().manual_seed(12)).to(dt)
+    c = AnyCache(1, H, hd, 512, dtype=dt)
+    c.store(k.cuda(), v.cuda(), words(0))
+    got = c.attend(q.cuda(), words(n))
+    ref, size = expect(q[0, :50], held(k[0].float()), held(v[0].float()), [0] * 50, [71 + i for i in range(50)])
+    close(got[0, :50], ref, size, dt)
