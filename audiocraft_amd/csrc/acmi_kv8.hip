@@ -1587,6 +1587,7 @@ extern "C" int acmi_kv8_attn(const acmi_kv8_cache* cache, const acmi_kv8_attn_de
     // hd 32 8 x 16 x 2048 101 / 100
     const int QB = cache->hd == 64 && !out_f32 && !qhl && pairs * ((qtiles + 7) / 8) >= 768 ? 2 : 1;
     a.tiles = (qtiles + 4 * QB - 1) / (4 * QB);
+    a.splits = a.chunk = 1;   // (kv8_span divides by them)
     ACMI_REQUIRE(pairs * a.tiles <= 0x7fffffffLL, "acmi_kv8_attn: %lld workgroups", pairs * a.tiles);
     const dim3 mgrid((unsigned)(pairs * a.tiles));
 #define KV8_MANY(HDv, Q, P, QBv) hipLaunchKernelGGL((kv8_attn_many_kernel<HDv, Q, P, QBv>), mgrid, dim3(256), 0, st, a)
