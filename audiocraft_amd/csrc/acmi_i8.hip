@@ -300,7 +300,7 @@ __global__ __launch_bounds__(NW * 64) void lin_i8_kernel(const I8Args p) {
         for (int k = 0; k < NW; ++k) sum += reinterpret_cast<const int*>(&part[k][m][(n >> 2) * 16 + rl])[n & 3];
         const float sa = FUSED ? fscale[FUSED ? rl : 0] : p.a_scale[row];
         float y = fmaf((float)sum, sa * p.w_scale[c], p.bias != nullptr ? p.bias[c] : 0.f);
-        if (p.act == 1) y = i8_gelu(y);
+        if (p.act == 1) y = p.out_bf16 ? i8_gelu_bf16(y) : i8_gelu(y);
         if (p.residual != nullptr) y += p.residual[(size_t)row * p.N + c];
         const size_t at = (size_t)(row * p.ldo) + c;
         if (p.out_bf16) reinterpret_cast<bf16_t*>(p.out)[at] = f32_to_bf16(y);

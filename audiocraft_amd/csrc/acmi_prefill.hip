@@ -324,7 +324,7 @@ __global__ __launch_bounds__(BigTile<BIG>::NW * 64, BIG ? 1 : 2) void lin_big_ke
                 if (p.act == 1) {
                     if (p.out_bf16) {
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) v[r] = big_gelu_bf16(v[r]);
+                        for (int r = 0; r < 4; ++r) v[r] = i8_gelu_bf16(v[r]);
                     } else {
 #pragma unroll
                         for (int r = 0; r < 4; ++r) v[r] = big_gelu(v[r]);

@@ -17,7 +17,7 @@ _DTYPES = (torch.float32, torch.bfloat16)
 
 class Int8Linear:
     """Built once from a weight [N, K] (nn.Linear layout, f32 or bf16, on the GPU) and an optional bias [N]; the int8 weight is laid
-    out for the matrix cores (include/acmi.h, "int8 fragments").  activation: 'none' or 'gelu' (exact).
+    out for the matrix cores (include/acmi.h, "int8 fragments").  activation: 'none' or 'gelu' (by erf).
 
     A token (channel) that holds a NaN or an infinity gives NaN in its whole output row (column)."""
 

@@ -702,7 +702,9 @@ int acmi_kv8_attn(const acmi_kv8_cache* cache, const acmi_kv8_attn_desc* desc, v
 int acmi_quantize_rows_i8(const void* x, int dtype, long long ldx, int R, int K, void* codes, float* scale, void* stream);
 
 /* out[M, N] = act(a_scale[m] * w_scale[n] * sum_k a[m, k] w[n, k] + bias[n]) + residual[m, n]: the sum exact in 32-bit integers
- * (K <= 131072; M, N <= 2^30, M N <= 2^38), one f32 product by a_scale * w_scale.  act: 0 none, 1 exact (erf) GELU.  bias [N] f32 or NULL; residual
+ * (K <= 131072; M, N <= 2^30, M N <= 2^38), one f32 product by a_scale * w_scale.  act: 0 none, 1 GELU by
+ * erf, the same in every form that serves the call (f32 results: 1 + erff; bf16 ones: erfc by a polynomial, within 2^-15 of the result itself
+ * down to y = -12).  bias [N] f32 or NULL; residual
  * [M, N] f32 (pitch N) or NULL.  out: row-major, pitch ldo, out_dtype f32 / bf16.
  * The activation is given quantised (a, a_scale) or as it is (x [M, K] in x_dtype, pitch ldx; a, a_scale NULL): its rows are then
  * quantised by the same rule within the call, with acmi_linear_i8_work_bytes(M, K) bytes of 16-byte aligned `work` of this call
