@@ -40,7 +40,7 @@ class Int8Linear:
         if bias is not None:
             if bias.shape != (self.out_features,) or bias.device != weight.device:
                 raise ValueError(f"Int8Linear: bias {tuple(bias.shape)} on {bias.device}, expected [{self.out_features}] on {weight.device}")
-            self.bias = bias.detach().float().contiguous()
+            self.bias = bias.detach().to(torch.float32, copy=True).contiguous()   # (its own: the weight's codes do not follow the caller's tensors either)
 
     @classmethod
     def from_linear(cls, linear: nn.Linear, activation: str = 'none') -> 'Int8Linear':

@@ -77,3 +77,14 @@ def test_gelu_in_bfloat16_to_its_own_size(Int8Linear, M):
     want = 0.5 * lin * torch.special.erfc(-lin / math.sqrt(2))
     bound = (2.0 ** -8 + 2.0 ** -18 + 6 * 2.0 ** -24 * (lin.abs() + 1) * lin.abs().clamp_min(1)) * want.abs()
     assert ((got - want).abs() <= bound).all(), ((got - want).abs() / want.abs().clamp_min(1e-300)).max().item()
+
+
+def test_the_layer_keeps_its_own_bias(Int8Linear):
+    """Built once: neither the weight nor the bias follows what the caller does to its tensors later."""
+    x, w, bias = make(4, 32, 64, torch.float32, 9)
+    wd, bd = w.cuda(), bias.cuda()
+    layer = Int8Linear(wd, bd)
+    want = layer(x.cuda())
+    wd.zero_()
+    bd.zero_()
+    assert torch.equal(layer(x.cuda()), want)
