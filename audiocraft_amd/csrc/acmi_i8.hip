@@ -150,6 +150,8 @@ __global__ __launch_bounds__(512) void quant_row_wide_kernel(const QuantRowsArgs
 static RowSrc row_src(const void* x, int dtype, long long ldx, int R, int K) {
     return RowSrc{x, ldx, dtype == ACMI_BF16, R, K};
 }
+// rows of one launch: its work items, 64 a row, are counted in 32 bits (more are dropped without an error)
+constexpr int QUANT_MAX_ROWS = 1 << 25;
 static int launch_quant_rows(const RowSrc& s, uint8_t* codes, float* scale, hipStream_t st) {
     QuantRowsArgs a = {s, (s.K + 63) / 64, 0, codes, scale};
     a.kchunk = min(a.nkc * 64, 8192);
@@ -165,6 +167,14 @@ static int launch_quant_rows(const RowSrc& s, uint8_t* codes, float* scale, hipS
                            hipFuncSetAttribute(reinterpret_cast<const void*>(&quant_rows_kernel<2>), hipFuncAttributeMaxDynamicSharedMemorySize, 16 * (8192 + 16)) == hipSuccess &&
                            hipFuncSetAttribute(reinterpret_cast<const void*>(&quant_rows_kernel<16>), hipFuncAttributeMaxDynamicSharedMemorySize, 16 * (8192 + 16)) == hipSuccess;
     ACMI_REQUIRE(ok, "acmi_quantize_rows_i8: cannot set the dynamic LDS limit");
+    if (s.R > QUANT_MAX_ROWS) {
+        for (int r0 = 0; r0 < s.R; r0 += QUANT_MAX_ROWS) {
+            const int n = min(s.R - r0, QUANT_MAX_ROWS);
+            const void* x = reinterpret_cast<const char*>(s.x) + (size_t)(r0 * s.ldx) * (s.bf16 ? 2 : 4);
+            if (int rc = launch_quant_rows(RowSrc{x, s.ldx, s.bf16, n, s.K}, codes + (size_t)(r0 / 16) * a.nkc * 1024, scale + r0, st)) return rc;
+        }
+        return ACMI_OK;
+    }
     if (s.K <= 512) hipLaunchKernelGGL(quant_rows_kernel<2>, dim3((s.R + 15) / 16), dim3(1024), lds, st, a);
     // (16 x 256 columns in registers halve the workgroups per CU; us 8 x 256 / 16 x 256: 9600 x 6144 f32 77 / 65, bf16 62 / 53, 4096 x 8000
     // bf16 31 / 28; 8192 x 4096 bf16 21.5 / 26, 9600 x 2100 16.3 / 25.9)
@@ -325,6 +335,7 @@ extern "C" int acmi_linear_i8(const acmi_linear_i8_desc* desc, void* stream) {
     ACMI_REQUIRE(d.act == 0 || d.act == 1, "acmi_linear_i8: act %d", d.act);
     if (d.M == 0) return ACMI_OK;
     ACMI_REQUIRE(d.M <= 1 << 30 && d.N <= 1 << 30 && (long long)d.M * d.N <= 1LL << 38, "acmi_linear_i8: M=%d N=%d (each at most 2^30, M N at most 2^38)", d.M, d.N);
+    ACMI_REQUIRE(d.N <= 1 << 25, "acmi_linear_i8: N=%d (at most 2^25: a launch counts its work items in 32 bits)", d.N);
     ACMI_REQUIRE(d.w && d.w_scale && d.out && d.ldo >= d.N, "acmi_linear_i8: null operand or ldo=%lld < N=%d", d.ldo, d.N);
     ACMI_REQUIRE((d.x != nullptr) != (d.a != nullptr && d.a_scale != nullptr), "acmi_linear_i8: either x or the quantised a, a_scale");
     ACMI_REQUIRE(((reinterpret_cast<size_t>(d.a) | reinterpret_cast<size_t>(d.w) | reinterpret_cast<size_t>(d.work)) & 15) == 0,

@@ -1405,7 +1405,7 @@ __global__ __launch_bounds__(256, (kv8_many_wpe<HD, QB>())) void kv8_attn_many_k
 static int kv8_check(const acmi_kv8_cache* c, const char* who) {
     ACMI_REQUIRE(c != nullptr, "%s: null cache", who);
     ACMI_REQUIRE(c->hd == 16 || c->hd == 32 || c->hd == 64 || c->hd == 128, "%s: head dim %d unsupported (16, 32, 64, 128)", who, c->hd);
-    ACMI_REQUIRE(c->rows > 0 && c->rows <= 65535 && c->H > 0 && c->H <= 65535 && c->nblk > 0 && c->nblk <= (1 << 24),
+    ACMI_REQUIRE(c->rows > 0 && c->rows <= 65535 && c->H > 0 && c->H <= 65535 && c->nblk > 0 && c->nblk < (1 << 24),
                  "%s: bad cache shape rows=%d H=%d nblk=%d", who, c->rows, c->H, c->nblk);
     ACMI_REQUIRE(c->tail_dtype == ACMI_F32 || c->tail_dtype == ACMI_BF16, "%s: tail_dtype %d", who, c->tail_dtype);
     ACMI_REQUIRE(c->k_codes && c->v_codes && c->k_scale && c->v_scale && c->k_tail && c->v_tail, "%s: null cache buffer", who);
@@ -1588,7 +1588,7 @@ extern "C" int acmi_kv8_attn(const acmi_kv8_cache* cache, const acmi_kv8_attn_de
     const int QB = cache->hd == 64 && !out_f32 && !qhl && pairs * ((qtiles + 7) / 8) >= 768 ? 2 : 1;
     a.tiles = (qtiles + 4 * QB - 1) / (4 * QB);
     a.splits = a.chunk = 1;   // (kv8_span divides by them)
-    ACMI_REQUIRE(pairs * a.tiles <= 0x7fffffffLL, "acmi_kv8_attn: %lld workgroups", pairs * a.tiles);
+    ACMI_REQUIRE(pairs * a.tiles * 256 <= 0xffffffffLL, "acmi_kv8_attn: %lld workgroups (a launch counts its work items in 32 bits)", pairs * a.tiles);
     const dim3 mgrid((unsigned)(pairs * a.tiles));
 #define KV8_MANY(HDv, Q, P, QBv) hipLaunchKernelGGL((kv8_attn_many_kernel<HDv, Q, P, QBv>), mgrid, dim3(256), 0, st, a)
 #define KV8_CASE(HDv)                                            \

@@ -526,6 +526,7 @@ int acmi_launch_big_i8(BigArgs& a, hipStream_t st) {
     const int t256 = ((a.M + 255) >> 8) * ((a.N + 255) >> 8), rounds = (t256 + 255) >> 8;
     const int big = t256 * 100 >= rounds * 256 * 85;
     const int tiles = big_grid(a.M, a.N, big ? 8 : 7);
+    ACMI_REQUIRE((long long)tiles * (big ? 512 : 256) <= 0xffffffffLL, "acmi_linear_i8: %d tiles", tiles);
     const int rc = big ? launch_big_k<int8_t, ACMI_BIG_I8, 1>(a, tiles, st) : launch_big_k<int8_t, ACMI_BIG_I8, 0>(a, tiles, st);
     return rc ? rc : acmi_check_launch("lin_big_kernel");
 }

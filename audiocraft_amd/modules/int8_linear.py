@@ -28,6 +28,8 @@ class Int8Linear:
             raise ValueError(f"Int8Linear: weight {tuple(weight.shape)} {weight.dtype} on {weight.device}: [N, K] float32 or bfloat16 on the GPU")
         if weight.shape[1] > 131072:
             raise ValueError(f"Int8Linear: K {weight.shape[1]} (at most 131072: the 32-bit integer sums)")
+        if weight.shape[0] > 1 << 25:
+            raise ValueError(f"Int8Linear: N {weight.shape[0]} (at most 2^25)")
         if activation not in self.ACTIVATIONS:
             raise ValueError(f"Int8Linear: activation {activation!r} ({', '.join(self.ACTIVATIONS)})")
         self.out_features, self.in_features = weight.shape

@@ -41,8 +41,8 @@ class KV8Cache:
             raise ValueError(f"KV8Cache: rows {rows}, heads {heads}, capacity {capacity}")
         self.rows, self.heads, self.head_dim, self.dtype = rows, heads, head_dim, dtype
         self.blocks = -(-capacity // _C.KV8_BLOCK)
-        if self.blocks > 1 << 24:
-            raise ValueError(f"KV8Cache: capacity {capacity} (at most {_C.KV8_BLOCK << 24})")
+        if self.blocks >= 1 << 24:
+            raise ValueError(f"KV8Cache: capacity {capacity} (at most {_C.KV8_BLOCK * ((1 << 24) - 1)})")
         self.capacity = self.blocks * _C.KV8_BLOCK
         if torch.device(device).type != 'cuda':
             raise ValueError(f"KV8Cache: device {device} (libacmi has no CPU fallback)")

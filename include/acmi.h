@@ -633,7 +633,7 @@ int acmi_attn_decode_ex(const acmi_attn_desc* desc, void* stream);
  * A block is quantised ONCE, from its exact tokens, by the call that stores its 64th token; that call also leaves it in the
  * tail, which attention reads for the row's block (length - 1) / 64 until a token of the next block overwrites it.  So a token
  * is exact while it is among the newest 1 .. 64 of its row, |error| <= scale / 2 afterwards, and never rounded twice.
- * The caller zeroes the buffers once.  hd: 16, 32, 64 or 128.  A row holds nblk * 64 tokens; tokens past that are dropped.
+ * The caller zeroes the buffers once.  hd: 16, 32, 64 or 128; nblk < 2^24.  A row holds nblk * 64 tokens; tokens past that are dropped.
  * A row's length is the caller's (device int32), so every call here can be captured and replayed; nothing is kept in the
  * library.  Lengths are clamped to [0, nblk * 64]. */
 #define ACMI_KV8_BLOCK 64
@@ -702,7 +702,7 @@ int acmi_kv8_attn(const acmi_kv8_cache* cache, const acmi_kv8_attn_desc* desc, v
 int acmi_quantize_rows_i8(const void* x, int dtype, long long ldx, int R, int K, void* codes, float* scale, void* stream);
 
 /* out[M, N] = act(a_scale[m] * w_scale[n] * sum_k a[m, k] w[n, k] + bias[n]) + residual[m, n]: the sum exact in 32-bit integers
- * (K <= 131072; M, N <= 2^30, M N <= 2^38), one f32 product by a_scale * w_scale.  act: 0 none, 1 GELU by
+ * (K <= 131072; M <= 2^30, N <= 2^25, M N <= 2^38), one f32 product by a_scale * w_scale.  act: 0 none, 1 GELU by
  * erf, the same in every form that serves the call (f32 results: 1 + erff; bf16 ones: erfc by a polynomial, within 2^-15 of the result itself
  * down to y = -12).  bias [N] f32 or NULL; residual
  * [M, N] f32 (pitch N) or NULL.  out: row-major, pitch ldo, out_dtype f32 / bf16.

@@ -88,3 +88,20 @@ def test_the_layer_keeps_its_own_bias(Int8Linear):
     wd.zero_()
     bd.zero_()
     assert torch.equal(layer(x.cuda()), want)
+
+
+def test_very_many_rows(Int8Linear):
+    """2^26 rows and some: more work items than one launch takes."""
+    if torch.cuda.mem_get_info()[0] < 20 << 30:
+        pytest.skip("needs 20 GB")
+    M = (1 << 26) + 5
+    w = torch.tensor([[1.5], [-0.5], [3.0]])
+    layer = Int8Linear(w.cuda())
+    x = torch.zeros(M, 1, dtype=torch.bfloat16, device='cuda')
+    for at in (0, 1 << 25, (1 << 26) - 1, M - 5, M - 1):
+        x[at] = 2.0 + at % 7
+    got = layer(x)
+    for at in (0, 1 << 25, (1 << 26) - 1, M - 5, M - 1):
+        assert ((got[at].cpu().double() - x[at].cpu().double() * w[:, 0].double()).abs() <= 2.0 ** -7 * (2.0 + at % 7) * 3).all()
+        x[at] = 0
+    assert (layer(x) == 0).all()
