@@ -55,6 +55,8 @@ class Int8Linear:
             raise ValueError(f"Int8Linear: x {tuple(x.shape)} {x.dtype} on {x.device}: [..., {self.in_features}] float32 or bfloat16 on {self.codes.device}")
         rows = x if x.dim() == 2 else x.reshape(-1, self.in_features)
         M = rows.shape[0]
+        if M > 1 << 30:
+            raise ValueError(f"Int8Linear: {M} tokens in one call (at most 2^30)")
         if rows.stride(1) != 1 or (M > 1 and rows.stride(0) < self.in_features):
             rows = rows.contiguous()
         if residual is not None:

@@ -90,6 +90,10 @@ class KV8Cache:
     def _work(self, S: int, Hq: int) -> int:
         n = self._work_floats.get((S, Hq))
         if n is None:
+            cols = S * (Hq // self.heads)                   # query columns of a cache head, 64 to a workgroup
+            if S > 1 << 20 or Hq > 65535 or cols > 1 << 21 or (-(-self.rows * self.heads // 8) * 8 * -(-cols // 64)) >= 1 << 24:
+                raise ValueError(f"KV8Cache: {S} queries x {Hq} heads x {self.rows} rows in one call (2^20 queries, 65535 heads, 2^21 of both per "
+                                 f"cache head, 2^24 groups of 64 in all)")
             n = self._work_floats[S, Hq] = _C.kv8_attn_work_floats(self.desc, S, Hq)
         return n
 
@@ -132,10 +136,13 @@ class KV8Cache:
         if k.dtype != v.dtype:
             raise ValueError(f"KV8Cache.decode: k is {k.dtype}, v is {v.dtype}")
         lens, starts = self._words('decode', 'lens', lens, True), self._words('decode', 'starts', starts, False)
-        past, qs = self._past('decode', past_context), q.stride()
+        past, qs, work = self._past('decode', past_context), q.stride(), self._work(1, Hq)
+        if (qs[0] | qs[1]) >> 31:                            # (few queries: strides in 32 bits)
+            q = q.contiguous()
+            qs = q.stride()
         with _C.device_lock:
             out = torch.empty(self.rows, Hq, self.head_dim, device=self.device, dtype=q.dtype)
-            return _C.kv8_attn(self.desc, self._work(1, Hq), q, (qs[0], 0, qs[1]), 1, out, lens, 1, True, past, None, starts, k, v)
+            return _C.kv8_attn(self.desc, work, q, (qs[0], 0, qs[1]), 1, out, lens, 1, True, past, None, starts, k, v)
 
     def attend(self, q: torch.Tensor, lens: torch.Tensor, causal: bool = True, past_context: int = 0,
                q_lens: tp.Optional[torch.Tensor] = None, starts: tp.Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -151,10 +158,15 @@ class KV8Cache:
             raise ValueError("KV8Cache.attend: past_context needs causal=True")
         lens, starts = self._words('attend', 'lens', lens, True), self._words('attend', 'starts', starts, False)
         q_lens = self._words('attend', 'q_lens', q_lens, False)
+        work = self._work(S, Hq) if S else 0
+        qs = q.stride()
+        if (qs[0] | qs[1] | qs[2]) >> 31:                    # (few queries: strides in 32 bits)
+            q = q.contiguous()
+            qs = q.stride()
         with _C.device_lock:
             out = torch.empty(self.rows, S, Hq, self.head_dim, device=self.device, dtype=q.dtype)
             if S:
-                _C.kv8_attn(self.desc, self._work(S, Hq), q, q.stride()[:3], S, out, lens, 0, bool(causal), past, q_lens, starts)
+                _C.kv8_attn(self.desc, work, q, qs[:3], S, out, lens, 0, bool(causal), past, q_lens, starts)
         return out
 
     def _queries(self, who: str, q: torch.Tensor, dims: int) -> tp.Tuple[torch.Tensor, int]:
