@@ -148,6 +148,30 @@ def test_one_large_feature(AnyCache, S, R):
     close(got[0], ref, size, torch.float32)
 
 
+@pytest.mark.parametrize('H,past', [(384, 0), (200, 90)])
+def test_bf16_results_to_their_own_size(KV8Cache, H, past):
+    """Prompts on a full grid (two column tiles per wave, and one): tight enough that a token left out would show."""
+    S, n, hd = 70, 333, 64
+    k, v = make(1, n, H, hd, torch.bfloat16, 41)
+    q = torch.randn(1, S, H, hd, generator=torch.Generator().manual_seed(42)).bfloat16()
+    c = KV8Cache(2, H, hd, n)
+    c.store(torch.cat([k, k]).cuda(), torch.cat([v, v]).cuda())
+    got = c.attend(torch.cat([q, q]).cuda(), words(n, n), past_context=past)
+    hi = [n - S + i + 1 for i in range(S)]
+    lo = [max(0, h - 1 - past) if past else 0 for h in hi]
+    kh, vh = held(k[0].float()), held(v[0].float())
+    ref, size = expect(q[0], kh, vh, lo, hi)
+    close(got[0], ref, size, torch.bfloat16)
+    close(got[1], ref, size, torch.bfloat16)
+    # the bound is one: without one of the tokens most results leave it
+    s = torch.einsum('shd,thd->hst', q[0].double(), kh) / math.sqrt(hd)
+    t = torch.arange(n)[None]
+    seen = (t >= torch.tensor(lo)[:, None]) & (t < torch.tensor(hi)[:, None]) & (t != 250)
+    p = torch.softmax(s.masked_fill(~seen, -math.inf), -1)
+    off = (torch.einsum('hst,thd->shd', p, vh) - ref).abs() > 2.0 ** -11 * size + 2.0 ** -8 * ref.abs()
+    assert off.double().mean() > 0.5
+
+
 @pytest.mark.parametrize('S', [1, 90])
 @pytest.mark.parametrize('sizes', [[1e30, 1e-8, 1e30, 1e-30, 1.0], [1e-30, 1e30, 1e-30, 1e30, 1e-30], [1e5, 1.0, 1e-5, 1e5, 1.0], [1e-20, 1.0, 1e20, 1.0, 1e-20]])
 @pytest.mark.parametrize('dt', ['f32', 'bf16'])
