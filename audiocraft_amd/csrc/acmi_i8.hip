@@ -155,9 +155,10 @@ constexpr int QUANT_MAX_ROWS = 1 << 25;
 static int launch_quant_rows(const RowSrc& s, uint8_t* codes, float* scale, hipStream_t st) {
     QuantRowsArgs a = {s, (s.K + 63) / 64, 0, codes, scale};
     a.kchunk = min(a.nkc * 64, 8192);
-    // A workgroup per row until they are many; then 16 rows to one, whose wave keeps 2048 columns of its row -- longer rows are read
-    // again, so those change over later.  us, per row / 16 rows (kernels): 384 x 1536 f32 3.9 / 4.3, 1000 x 1000 5.4 / 4.6; (calls)
-    // 1024 x 6144 9.1 / 12.7, 2048 x 6144 16.9 / 21.2, 4096 x 6144 31.9 / 27.9, 2048 x 2048 9.3 / 6.9, 4096 x 1536 14.2 / 7.2
+    // A workgroup per row until they are many; then 16 rows to one, whose wave keeps 2048 columns of its row, 4096 where K is more, and
+    // reads the rest again: those change over later.  us in a graph, per row / 16 rows: 384 x 1536 f32 4.2 / 4.6, 1000 x 1000 5.7 / 4.9,
+    // 2048 x 2048 9.8 / 5.6, 4096 x 1536 15.1 / 5.9; 1024 x 4096 8.0 / 8.9, 2048 x 4096 12.8 / 10.5, 1024 x 6144 9.5 / 11.5, 2048 x 6144
+    // 17.3 / 16.4 (bf16 15.3 / 17.4), 4096 x 6144 32.4 / 24.1, 2048 x 8000 bf16 19.5 / 23.2
     if (s.R <= (s.K > 2048 ? 2048 : 512)) {
         hipLaunchKernelGGL(quant_row_wide_kernel, dim3(s.R), dim3(512), (size_t)a.kchunk, st, a);
         return acmi_check_launch("quant_row_wide_kernel");

@@ -647,7 +647,8 @@ __device__ __forceinline__ void kv8_column(const Kv8AttnArgs& p, const Kv8RowInf
 struct Kv8Span { int bf, bt, eff; bool live, tail; };
 constexpr int KV8_MAX_SPLITS = 64;
 // Workgroups that a split call aims at: two per CU, what its registers let run at once.  4 rows x 8 cache heads of 128 features, up
-// to 32768 tokens: 512 35.5 us (256 34.6, within the noise, but half as many on a call whose rows differ in length), 1024 41.6.
+// to 32768 tokens, with the join: 512 40.8 us (256 40.3, within the noise, but half as many on a call whose rows differ in length),
+// 1024 45.8.
 constexpr int KV8_TARGET = 512;
 __device__ __forceinline__ Kv8Span kv8_span(const Kv8AttnArgs& p, const Kv8RowInfo& ri, int c0, int c1) {   // columns [c0, c1)
     Kv8Span s;
@@ -688,9 +689,9 @@ __device__ __forceinline__ void kv8_put4(const Kv8AttnArgs& p, int row, int s, i
 // ---- few queries: one workgroup per (split, column tile of a cache head, row); its NW waves take the blocks in turn, the last four of
 // them 16 tokens of the tail each, and are joined through LDS.  A wave keeps one block in flight: the next block's K is requested as
 // soon as this block's K has been multiplied, its V likewise.  Bound by the codes' bytes: 4 rows of 9001 to 32768 tokens x 8 heads of
-// 128, 171 MB in 35.2 us = 4.9 TB/s, the rate of a large copy; 64 rows of 1400 x 24 heads of 64 4.4 TB/s; 16 rows of 750 2.5 TB/s.
-// Launch bound per SIMD: a wave's block in flight takes 128 registers at 64 features, 240 at 128.  16 rows of 500 to 1251 tokens x
-// 24 heads of 64, 8 waves: 4 per SIMD 15.6 us, 2 17.2; 32768 tokens, hd 128: 2 per SIMD 35.5 us, 1 42.2, 8 waves per workgroup 40.2.
+// 128, 171 MB in 35.6 us = 4.8 TB/s, the rate of a large copy; 64 rows of 750 x 24 heads of 64 3.9 TB/s; 16 rows of 750 2.3 TB/s.
+// Launch bound per SIMD: a wave's block in flight takes 128 registers at 64 features, 226 at 128.  64 rows of 750 tokens x 24 heads of
+// 64: 4 per SIMD 38 us, 2 41; up to 32768 tokens, hd 128, with the join: 2 per SIMD 40.8 us, 1 47.5.
 template <int HD> constexpr int kv8_wpe() { return HD == 128 ? 2 : 4; }
 
 __device__ __forceinline__ float raw8(bf16_t v) { return bf16_to_f32(v); }
@@ -1051,7 +1052,7 @@ __global__ __launch_bounds__(256) void kv8_attn_join_kernel(const Kv8AttnArgs p)
 // the next block's codes to f16 fragments in LDS while this block is multiplied (two buffers, one barrier per block).  The tail
 // is staged the same way, relative to a power of two, as f16 (bf16 tails: exact down to 2^-30 of the largest) or a pair of f16; where
 // a token's features are all below 2^-12 of the tail's largest -- which this column may not see -- it takes kv8_tail_wide instead.
-// Bound by vector issue beside the matrix cores: causal over 4096 tokens, 4 x 16 heads of 64, 571 TFLOP/s (f32 403).  Short calls
+// Bound by vector issue beside the matrix cores: causal over 4096 tokens, 4 x 16 heads of 64, 605 TFLOP/s (f32 443).  Short calls
 // are latencies one after another: 16 x 32 heads x 251 queries over 0 .. 77 states 20 us, of which the tail's staging is 6.
 // All workgroups of a (row, cache head) run on one XCD (workgroup i on XCD i % 8), whose L2 then holds its codes; the last (causal:
 // longest) tiles of all pairs go first, the short ones fill the end.
@@ -1120,7 +1121,7 @@ __device__ __forceinline__ void kv8_tail_wide(const Kv8AttnArgs& p, const Kv8Row
     }
 }
 
-// Waves per SIMD: what the registers allow without spilling more than a few (hd 64, two tiles: 3 55.6 us, 2 66.3, for 600 tokens x
+// Waves per SIMD: what the registers allow without spilling more than a few (hd 64, two tiles: 3 52.7 us, 2 61.9, for 600 tokens x
 // 16 rows x 24 heads).
 template <int HD, int QB> constexpr int kv8_many_wpe() { return HD == 128 ? 2 : QB == 2 ? 3 : 4; }
 template <int HD, bool QHL, bool PHL, int QB>
@@ -1467,9 +1468,9 @@ extern "C" int acmi_kv8_load(const acmi_kv8_cache* cache, const int* len, int T,
 
 // The split form: one query per head (it alone stores a new token), one column tile, or few workgroups, three per CU -- a workgroup of
 // it has a column tile and its waves share the blocks, where the prompt form's waves walk all blocks with a tile each.  Measured, us
-// split / prompt form, in a graph: 4 x 8 heads x 128 queries of 300 (256 workgroups) 8.9 / 12.8, 1 x 16 x 600 of 600 (608) 13.1 /
-// 18.4, 1 x 8 x 128 of 8000 (64) 23.8 / 137, 16 x 24 x 29 of 600 (768) 20.8 / 24.6; 8 x 8 x 200 of 600 (832) 19.5 / 18.9,
-// 16 x 12 x 77 of 251 (960) 19.6 / 15.7, 64 x 8 x 4 x 16 of 1000 (2048) 65.6 / 38.8
+// split / prompt form, in a graph: 4 x 8 heads x 128 queries of 300 (256 workgroups) 7.1 / 10.8, 1 x 16 x 600 of 600 (608) 11.1 /
+// 15.5, 1 x 8 x 128 of 8000 (64) 19.1 / 116, 16 x 24 x 29 of 600 (768) 15.4 / 19.7; 8 x 8 x 200 of 600 (832) 16.1 / 16.0,
+// 16 x 12 x 77 of 251 (960) 13.0 / 12.0, 64 x 8 x 4 x 16 of 1000 (2048) 52.1 / 28.5
 constexpr int KV8_SPLIT_WGS = 768;
 static bool kv8_few(const acmi_kv8_cache* c, int S, int G) {
     const long long tiles = ((long long)S * G + 15) / 16;
@@ -1478,8 +1479,8 @@ static bool kv8_few(const acmi_kv8_cache* c, int S, int G) {
 // Blocks per workgroup: the longest possible row in so many chunks that the call has about KV8_TARGET workgroups; one chunk (and
 // no second launch) when the tiles alone fill the chip.  The rows' lengths are not known here: shorter rows take fewer chunks of
 // the same size, so that all workgroups take equally long.  A chunk is at least a block per wave, and a row of less than four per wave
-// is not split: the second launch costs 4 us.  us in a graph, unsplit or chunks of four per wave / as here: 2 rows x 16 heads of 64 x
-// 2800 tokens 14.9 / 11.6, 7 x 2 x 3700 17.6 / 11.2, 4 x 8 x 4 heads of 128 x 2000 20.4 / 14.3; 2 x 16 x 1400 unsplit 10.9, split 12.7
+// is not split: the second launch costs 4 us.  us in a graph, caches cold, unsplit / as here: 2 rows x 16 heads of 64 x 2800
+// tokens 15.9 / 12.3, 7 x 2 x 3700 18.5 / 10.9, 4 x 8 x 4 heads of 128 x 2000 22.4 / 16.9; 2 x 16 x 1400 unsplit 11.1, split 12.7
 static void kv8_split_plan(const acmi_kv8_cache* c, int S, int G, int* splits, int* chunk) {
     const long long tiles = (long long)c->H * ((S * G + 15) / 16) * c->rows;
     long long n = 1;
@@ -1550,8 +1551,8 @@ extern "C" int acmi_kv8_attn(const acmi_kv8_cache* cache, const acmi_kv8_attn_de
         // A grid of at most one workgroup per CU is one chain of latencies: 8 waves share the blocks, and the tail is requested before
         // the row's length is known.  Larger grids are bytes: 4 waves, twice the workgroups in flight, and only the part of the tail
         // that is needed, by the split that needs it.  us in a graph, caches cold, 8 waves / 4: 16 rows x 24 heads of 64, 750 tokens
-        // 16.5 / 15.4 (bf16 15.7 / 14.2), 64 rows 41.8 / 38.5, 16 rows x 200 tokens 8.9 / 10.2; tail early / late: 64 rows x 200 tokens
-        // f32 28.2 / 23.2, 2 rows x 16 heads x 700 tokens 8.6 / 9.1, 128 rows x 8 x 4 heads of 128 x 1000 tokens 72.6 / 62.2
+        // 16.1 / 16.0 (bf16 15.1 / 13.9), 64 rows 45 / 38, 8 rows x 16 heads x 200 tokens 7.9 / 9.2, 16 x 16 x 700 11.2 / 12.5; tail early /
+        // late: 64 rows x 200 tokens f32 28.0 / 22.8, 2 rows x 16 heads x 700 tokens 8.4 / 9.1
         const long long wgs = (long long)grid.x * grid.y * grid.z;
         const bool early = a.splits == 1 && wgs <= 256, wide = cache->hd <= 64 && wgs <= 256;
         const unsigned g1 = (unsigned)qtiles | (unsigned)a.q_bf16 << 16 | (unsigned)(cache->tail_dtype == ACMI_BF16) << 17 | (unsigned)d.len_stride << 18 |
@@ -1582,9 +1583,9 @@ extern "C" int acmi_kv8_attn(const acmi_kv8_cache* cache, const acmi_kv8_attn_de
     }
     const long long pairs = ((long long)cache->rows * cache->H + 7) / 8 * 8;
     // two column tiles per wave where bf16 results at 64 features leave the registers for it and the workgroups still fill the chip,
-    // three per CU.  Measured, us one / two: 4 x 16 heads x 4096 tokens (2048 workgroups of two) 273 / 241, 16 x 24 x 600 (1920)
-    // 58.8 / 56.6, 8 x 8 x 4 x 512 of 2048 (1024) 120 / 114; 16 x 16 x 100 of 1500 (256) 36.9 / 44.4; f32 4 x 16 x 4096 341 / 344;
-    // hd 32 8 x 16 x 2048 101 / 100
+    // three per CU.  Measured, us one / two: 4 x 16 heads x 4096 tokens (2048 workgroups of two) 246 / 228, 16 x 24 x 600 (1920)
+    // 52.3 / 53.0, 8 x 8 x 4 x 512 of 2048 (1024) 110 / 105; 16 x 16 x 100 of 1500 (256) 32.6 / 40.8; f32 results and 32 features, where
+    // tried, gained nothing (4 x 16 x 4096 341 / 344, 8 x 16 x 2048 101 / 100)
     const int QB = cache->hd == 64 && !out_f32 && !qhl && pairs * ((qtiles + 7) / 8) >= 768 ? 2 : 1;
     a.tiles = (qtiles + 4 * QB - 1) / (4 * QB);
     a.splits = a.chunk = 1;   // (kv8_span divides by them)

@@ -127,7 +127,7 @@ int acmi_launch_big_i8(BigArgs& a, hipStream_t st);
 
 // GELU for a bf16 result of the int8 projection, in all its forms: erfc(z) = t Q(t) e^(-z^2), t = 1 / (1 + p z), with Q fitted here to
 // the RELATIVE error (2^-20; e^(-z^2) in f32 makes it 2^-18 down to x = -5 and 2^-16 to -12), so that the negative tail keeps a bf16
-// rounding too, where 1 + erff(..) has nothing left.  9600 x 6144 x 1536: 2 us more than the absolute form of the prefill GEMMs (152).
+// rounding too, where 1 + erff(..) has nothing left.  9600 x 6144 x 1536: 3 us more than with the prefill GEMMs' form, whose error is absolute (152).
 __device__ __forceinline__ float i8_gelu_bf16(float x) {
     const float z = fabsf(x) * 0.70710678118654752440f;
     const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.37895159f, z, 1.0f));

@@ -520,9 +520,9 @@ int acmi_launch_big_i8(BigArgs& a, hipStream_t st) {
     const size_t align = a.out_bf16 ? 7 : 15;
     a.vec = a.N % 4 == 0 && a.ldo64 % 4 == 0 && (reinterpret_cast<size_t>(a.out) & align) == 0;
     // 256 x 256 tiles (one workgroup per CU) where they fill whole rounds of the 256 CUs to 85 %, else 128 x 128 (two per CU).
-    // Measured, us large / small, bf16 results: 9600 x 1536 x 6144 (228 tiles) 101 / 117; 2048 x 8192 x 2048 (256) 38.1 / 43.7;
-    // 9600 x 6144 x 1536 (912) 115 / 118; 8192^3 (1024) 451 / 512; but 4800 x 4096 x 1024 (304) 44.0 / 35.9; 1000 x 4608 x 1536
-    // (72) 25.9 / 17.0
+    // Measured in a graph, us large / small, bf16 results: 9600 x 1536 x 6144 (228 tiles) 86 / 97; 2048 x 8192 x 2048 (256) 38.6 / 43.3;
+    // 9600 x 6144 x 1536 (912) 107 / 108 (with GELU 137 / 127); 8192^3 (1024) 395 / 462; but 4800 x 4096 x 1024 (304) 42.2 / 36.4;
+    // 1000 x 4608 x 1536 (72) 26.1 / 18.0
     const int t256 = ((a.M + 255) >> 8) * ((a.N + 255) >> 8), rounds = (t256 + 255) >> 8;
     const int big = t256 * 100 >= rounds * 256 * 85;
     const int tiles = big_grid(a.M, a.N, big ? 8 : 7);

@@ -671,8 +671,10 @@ int acmi_kv8_load(const acmi_kv8_cache* cache, const int* len, int T, void* k_ou
  * out: out_mode ACMI_OUT_F32 / ACMI_OUT_BF16 = [rows][S][Hq][hd]; ACMI_OUT_TILED (S = 1) = tiled activation of `rows` rows in
  * out_dtype with out_rbs K tiles per 16-row block, first column out_col0.
  * q, k_new and v_new rows are 16-byte aligned (element strides).
- * The products of probabilities and values take f16 probabilities (2^-12 of each) for bf16 results, a pair of f16 for f32 ones;
- * scores, softmax statistics and sums are f32.
+ * The products of probabilities and values take f16 probabilities (2^-12 of each) for bf16 results, a pair of f16 for f32 ones, relative
+ * to the largest of their block of 64 tokens (one below 2^-32 of it counts as 0); scores, softmax statistics and sums are f32.  What a
+ * query does not see, or gives no weight, leaves its result alone, however large or NaN it is (a whole block is NaN once it is
+ * quantised with one); values up to the largest number give finite results.
  * work: acmi_kv8_attn_work_floats(cache, S, Hq) floats of scratch of this call alone (NULL when that is 0). */
 typedef struct {
     const void* q; int q_dtype; long long q_row, q_tok, q_head;
