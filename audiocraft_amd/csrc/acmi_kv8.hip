@@ -1076,8 +1076,8 @@ __device__ __forceinline__ void kv8_tail_wide(const Kv8AttnArgs& p, const Kv8Row
     for (int slot0 = 0; t0 + slot0 < ri.len; slot0 += 16) {
         f32x4 s = {0.f, 0.f, 0.f, 0.f}, t[ND];
 #pragma unroll 1
-        for (int d = kg; d < HD; d += 4)
-            s = __builtin_amdgcn_mfma_f32_16x16x4f32(kv8_ld(p.c.k_tail, base + (size_t)(slot0 + nl) * HD + d, tb), kv8_ld(p.q, qb + d, p.q_bf16), s, 0, 0, 0);
+        for (int d = 0; d < HD; d += 4)
+            s = __builtin_amdgcn_mfma_f32_16x16x4f32(kv8_ld(p.c.k_tail, base + (size_t)(slot0 + nl) * HD + d + kg, tb), kv8_ld(p.q, qb + d + kg, p.q_bf16), s, 0, 0, 0);
         float cmax = -INFINITY, sum = 0.f, omax = 0.f;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
